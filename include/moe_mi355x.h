@@ -369,6 +369,72 @@ int moe_layer_run(const moe_layer* layer, const moe_layer* shared, const void* h
 int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64_t R, int64_t M, int64_t N,
                         int64_t scale_ld, void* out_bf16, int64_t out_ld, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The experts' products in 16-bit floats with their gradients, and in 8-bit
+ * integers.  No counterpart in the reference's FP8 layer; the int8 forms are
+ * vLLM's fused_moe use_int8_w8a8 with per_channel_quant.  dtype: MOE_BF16 or
+ * MOE_FP16.  Sums are fp32 (int8: exact in 32-bit integers) and rounded once, to
+ * nearest even.  Any sizes; rows of whole 16-byte chunks (16-byte aligned bases,
+ * widths and strides of whole chunks) take the faster kernels. */
+#define MOE_BF16 0
+#define MOE_FP16 1
+
+/* The slots of a batch grouped by expert: align over E + 1 experts, the last of
+ * which takes the slots whose id is outside [0, E), kept in slot_ids [S] int32.
+ * topk_ids [S] int32 or int64 (id_bytes 4 or 8).  E <= 1023; max_padded and
+ * workspace as for moe_align_block_size with E + 1 experts. */
+int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t S, int32_t E, int32_t block_size_m,
+                     int32_t* slot_ids, int32_t* sorted_ids, int32_t* expert_ids, int32_t* ntpp, int64_t max_padded,
+                     void* workspace, void* stream);
+
+/* y[s, n] = sum_k x[s / top_k, k] * w[e(s), n, k], e(s) the expert of slot s's
+ * block; zero rows where it is outside [0, E).  x [ceil(S/top_k), K] with row
+ * stride ldx (elements), w [E, N, K], y [S, N]. */
+int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const int32_t* sorted_ids, const int32_t* expert_ids,
+                   const int32_t* ntpp, int64_t S, int32_t top_k, int64_t N, int64_t K, int32_t E,
+                   int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
+
+/* Its gradient by the rows, one for each slot: dx[s, k] = sum_n dy[s, n] *
+ * w[e(s), n, k].  dy [S, N], dx [S, K]. */
+int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_ids, const int32_t* expert_ids,
+                         const int32_t* ntpp, int64_t S, int64_t N, int64_t K, int32_t E, int32_t block_size_m,
+                         int64_t max_padded, int32_t dtype, void* dx, void* stream);
+
+/* Its gradient by the weights: dw[e, n, k] = sum over the slots s of e of
+ * dy[s, n] * x[s / top_k, k]; zeros for experts without slots.  expert_ids must
+ * ascend over the blocks, as align without an expert map writes them. */
+int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, const int32_t* sorted_ids,
+                         const int32_t* expert_ids, const int32_t* ntpp, int64_t S, int32_t top_k, int64_t N,
+                         int64_t K, int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* dw,
+                         void* stream);
+
+/* The sum of each token's slot rows: y[t] = sum_i d[t * top_k + i].  d
+ * [T * top_k, H], y [T, H]. */
+int moe_slot_sum(const void* d, int64_t T, int32_t top_k, int64_t H, int32_t dtype, void* y, void* stream);
+
+/* Dynamic int8 quant with a scale a row: s = max(amax / 127, 1e-12), q =
+ * clamp(rint(x / s), +-127).  A row that holds an infinity or a NaN gets it as
+ * its scale, and zero codes.  x [T, H] of dtype, row stride ldx; q [T, H] int8,
+ * scales [T]. */
+int moe_quant_int8(const void* x, int64_t ldx, int64_t T, int64_t H, int32_t dtype, void* q_int8, float* scales,
+                   void* stream);
+
+/* y[m, n] = (sum_k a[m, k] * b[n, k]) * a_scale[m] * b_scale[n] + bias[n].
+ * a [M, K], b [N, K] int8 (row strides lda, ldb), bias [N] of dtype or NULL, y
+ * [M, N] of dtype, row stride ldy.  K <= 131071. */
+int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_scale, const void* b, int64_t ldb,
+                       const float* b_scale, const void* bias, int64_t M, int64_t N, int64_t K, int32_t dtype, void* y,
+                       int64_t ldy, void* stream);
+
+/* The same by slots: y[s, n] = (sum_k a[row, k] * b[e(s), n, k]) * a_scale[row] *
+ * b_scale[e(s), n] (* topk_weights[s] where not NULL), row = s / top_k, or the
+ * sorted position with a_by_pos; zero rows for blocks of experts outside [0, E).
+ * a [rows, K], a_scale [rows], b [E, N, K], b_scale [E, N], y [S, N]. */
+int moe_grouped_gemm_int8(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                          const int32_t* sorted_ids, const int32_t* expert_ids, const int32_t* ntpp,
+                          const float* topk_weights, int64_t S, int32_t top_k, int32_t a_by_pos, int64_t N, int64_t K,
+                          int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

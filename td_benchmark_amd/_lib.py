@@ -92,6 +92,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moe_layer_run": (ctypes.c_int, [_LAYER, _LAYER, _P, _P, _P, _i64, _P, _P]),
     "moe_silu_and_mul": (ctypes.c_int, [_P, _i64, _i64, _P, _P]),
     "moe_reduce_topk": (ctypes.c_int, [_P, _i64, _i32, _i64, _P, _P]),
+    "moe_expert_slots": (ctypes.c_int, [_P, _i32, _i64, _i32, _i32, _P, _P, _P, _P, _i64, _P, _P]),
+    "moe_grouped_mm": (ctypes.c_int, [_P, _i64, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32, _P,
+                                      _P]),
+    "moe_grouped_mm_dgrad": (ctypes.c_int, [_P, _P, _P, _P, _P, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _P, _P]),
+    "moe_grouped_mm_wgrad": (ctypes.c_int, [_P, _P, _i64, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32,
+                                            _P, _P]),
+    "moe_slot_sum": (ctypes.c_int, [_P, _i64, _i32, _i64, _i32, _P, _P]),
+    "moe_quant_int8": (ctypes.c_int, [_P, _i64, _i64, _i64, _i32, _P, _P, _P]),
+    "moe_int8_scaled_mm": (ctypes.c_int, [_P, _i64, _P, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _P, _i64, _P]),
+    "moe_grouped_gemm_int8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _i64, _i32, _i32, _i64, _i64, _i32, _i32,
+                                             _i64, _i32, _P, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -640,3 +640,39 @@ extern "C" int moe_align_block_size_noalloc(const int32_t* topk_ids, int64_t S, 
   if (rc != kOk) return rc;
   return align_impl(topk_ids, S, E, BM, nullptr, sorted_ids, expert_ids, ntpp, max_padded, ws, stream);
 }
+
+// ---------------------------------------------------------------------------
+// The slots of a batch grouped by expert for the grouped products: align over
+// E + 1 experts, the last of which takes the slots whose id is outside [0, E)
+// (dropped, or on another device), so that they too have blocks, whose rows the
+// products set to zero.
+
+namespace moe {
+
+template <class ID>
+__global__ __launch_bounds__(256) void slot_ids_kernel(const ID* __restrict__ ids, int64_t S, int E,
+                                                       int32_t* __restrict__ out) {
+  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (s >= S) return;
+  const ID id = ids[s];
+  out[s] = id >= 0 && id < E ? (int32_t)id : E;
+}
+
+}  // namespace moe
+
+extern "C" int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t S, int32_t E, int32_t BM,
+                                int32_t* slot_ids, int32_t* sorted_ids, int32_t* expert_ids, int32_t* ntpp,
+                                int64_t max_padded, void* workspace, void* stream) {
+  if (id_bytes != 4 && id_bytes != 8) return kErrBadShape;
+  if (E <= 0 || E >= kAlignMaxExperts) return kErrBadExperts;
+  if (S > 0 && !topk_ids) return kErrNullPointer;
+  const int rc = align_args(slot_ids, S, E + 1, BM, sorted_ids, expert_ids, ntpp, max_padded, true, workspace);
+  if (rc != kOk) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)((S + 255) / 256));
+  if (S > 0 && id_bytes == 8)
+    hipLaunchKernelGGL(slot_ids_kernel<int64_t>, grid, dim3(256), 0, st, (const int64_t*)topk_ids, S, (int)E, slot_ids);
+  else if (S > 0)
+    hipLaunchKernelGGL(slot_ids_kernel<int32_t>, grid, dim3(256), 0, st, (const int32_t*)topk_ids, S, (int)E, slot_ids);
+  return align_impl(slot_ids, S, E + 1, BM, nullptr, sorted_ids, expert_ids, ntpp, max_padded, workspace, stream);
+}

@@ -1,0 +1,133 @@
+// Operand types and the arguments of the grouped products (grouped_mm.hip).
+#pragma once
+
+#include "common.hpp"
+#include "internal.hpp"
+#include "mfma_frag.hpp"
+
+#include <type_traits>
+
+namespace moe {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v2f32 __attribute__((ext_vector_type(2)));
+
+// Operand element types.  A fragment is 16 bytes a lane: lane (fr = lane mod 16,
+// kseg = lane / 16) holds row fr's 16 bytes at kseg * 16 of a 64-byte run of the
+// contraction, 32 values of 16 bits or 64 of 8, for one 16x16 instruction.  The
+// two operands place the contraction alike, so its order inside the instruction
+// does not matter.
+struct Bf16 {
+  static constexpr int BYTES = 2;
+  typedef v4f Acc;
+  static MOE_DEVICE Acc mfma(v4i a, v4i b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+};
+struct Fp16 {
+  static constexpr int BYTES = 2;
+  typedef v4f Acc;
+  static MOE_DEVICE Acc mfma(v4i a, v4i b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+};
+// Sums of 8-bit products in 32 bits are exact: |sum| <= 2^14 K < 2^31 for K < 2^17.
+struct Int8 {
+  static constexpr int BYTES = 1;
+  typedef v4i Acc;
+  static MOE_DEVICE Acc mfma(v4i a, v4i b, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+};
+
+// Two fp32 -> a packed pair of the output type, round to nearest even.
+template <bool FP16>
+MOE_DEVICE uint32_t pack2(float a, float b) {
+  if constexpr (FP16) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f32){a, b}, v2h));
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+// A 16-bit output value as fp32.
+template <bool FP16>
+MOE_DEVICE float from16(uint16_t v) {
+  if constexpr (FP16) return (float)__builtin_bit_cast(_Float16, v);
+  else return bf16_to_f32(v);
+}
+
+// One launch of a product.  With sorted, eids and ntpp (as moe_align_block_size
+// writes them): position p of block p / bm belongs to expert eids[p / bm] and
+// slot sorted[p] (S or more: none).  Without: S rows of one expert, slot p.
+//
+// Rows form: out[slot][j] = sum_c A[row][c] * B[e][j][c], row = the position with
+// a_by_pos, else slot / top_k.  Blocks of an expert outside [0, E) get zero rows.
+// Weights form (wgrad): out[e][n][j] = sum over the slots of e of
+// A[slot][n] * B[slot / top_k][j].
+// Lengths and strides are in elements.
+struct MmArgs {
+  const uint8_t* A;
+  const uint8_t* B;
+  uint8_t* C;
+  const int32_t* sorted;
+  const int32_t* eids;
+  const int32_t* ntpp;
+  const float* As;      // int8: a scale for each row of A
+  const float* Bs;      // int8: a scale for each column of each expert, [E, J]
+  const uint16_t* bias; // [J] in the output type, or null
+  const float* topk_w;  // a factor for each slot, or null
+  int64_t S;
+  int64_t J;            // columns of the output
+  int64_t Cn;           // rows form: length of the contraction; weights form: rows of an expert's output
+  int64_t lda;          // row stride of A
+  int64_t sbj, sbc;     // rows form: B's strides along j and c; weights form: sbc is B's row stride
+  int64_t b_es;         // B's expert stride
+  int64_t ldc;          // row stride of the output
+  int64_t n_jt;         // column tiles
+  int64_t n_blocks;     // blocks that fit in max_padded
+  int bm, top_k, a_by_pos, E;
+};
+
+// Blocks that hold slots (ntpp is the device's word: kept to what was allocated).
+MOE_DEVICE int64_t live_blocks(const MmArgs& g) {
+  if (!g.ntpp) return g.n_blocks;
+  const int64_t n = (int64_t)*g.ntpp / g.bm;
+  return n < 0 ? 0 : (n < g.n_blocks ? n : g.n_blocks);
+}
+
+// The first of n ascending words that is at least v: 64 probes a round by the
+// lanes of the calling wave.
+MOE_DEVICE int64_t lower_bound(const int32_t* a, int64_t n, int32_t v) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = n;  // the answer is in [lo, hi]
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64;
+    const int64_t i = lo + step * (lane + 1) - 1;  // the lane's probe: the last of its step words
+    const uint64_t ge = __ballot(i >= hi || a[i < hi ? i : hi - 1] >= v);
+    // words before the first lane's run that reaches v are all smaller
+    const int first = ge ? __ffsll((unsigned long long)ge) - 1 : 64;
+    const int64_t nlo = lo + step * first, nhi = nlo + step - 1;
+    lo = nlo < hi ? nlo : hi;
+    hi = nhi < hi ? nhi : hi;
+  }
+  return lo;
+}
+
+// Positions [pos0, pos0 + count) of the slots of expert e: its blocks are
+// consecutive and ascending in e, and only the last of them has padding.
+struct Run {
+  int64_t pos0, count;
+};
+MOE_DEVICE Run run_of(const MmArgs& g, int e) {
+  const int64_t nb = live_blocks(g);
+  const int64_t b0 = lower_bound(g.eids, nb, e), b1 = lower_bound(g.eids + b0, nb - b0, e + 1) + b0;
+  Run r = {b0 * g.bm, 0};
+  if (b1 == b0) return r;
+  const int lane = threadIdx.x & 63;
+  int64_t last = 0;  // slots of the last block
+  for (int p = 0; p < g.bm; p += 64)
+    last += __popcll(__ballot(p + lane < g.bm && (uint32_t)g.sorted[(b1 - 1) * g.bm + p + lane] < g.S));
+  r.count = (b1 - b0 - 1) * g.bm + last;
+  return r;
+}
+
+}  // namespace moe

@@ -188,3 +188,157 @@ extern "C" int moe_quant_block128(const float* w, int64_t E, int64_t N, int64_t 
                      (hipStream_t)stream, w, (uint8_t*)q_fp8, scales, N, K, NB, KB);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
+
+// ---------------------------------------------------------------------------
+// Dynamic int8 quant with one scale a row: s = max(amax / 127, 1e-12) by IEEE
+// division (the floor of the FP8 quant), code = clamp(RNE(x / s), +-127).  A row
+// with an infinity or a NaN gets that as its scale and zero codes, so that
+// products with it are NaN.  HBM-bound: 2 bytes in, 1 out per element.  A row is
+// read once and kept in registers: by one wave up to 4096 columns, by four up to
+// 16384, in two passes beyond.
+
+namespace moe {
+
+template <bool FP16>
+MOE_DEVICE float act_f32(uint32_t bits16) {
+  if constexpr (FP16) return (float)__builtin_bit_cast(_Float16, (uint16_t)bits16);
+  else return bf16_to_f32(bits16);
+}
+
+// The larger magnitude as fp32 bits; a NaN's are above all numbers'.
+MOE_DEVICE uint32_t max_abs_bits(uint32_t m, float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b > m ? b : m;
+}
+
+struct Int8RowScale {
+  float s, inv;
+  bool finite;
+};
+MOE_DEVICE Int8RowScale int8_scale(uint32_t amax_bits) {
+  Int8RowScale r;
+  r.finite = amax_bits < 0x7F800000u;
+  const float s = __uint_as_float(amax_bits) / 127.0f;
+  r.s = s < kScaleFloor ? kScaleFloor : s;
+  r.inv = 1.0f / r.s;
+  return r;
+}
+MOE_DEVICE uint32_t int8_code(float x, const Int8RowScale& r) {
+  const float q = __builtin_rintf(div_by(x, r.s, r.inv));
+  return r.finite ? (uint32_t)(int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f) & 0xFFu : 0u;
+}
+
+// WAVES waves a row, IT 16-byte chunks of the row a lane (0: two passes over the row).
+template <bool FP16, int WAVES, int IT>
+__global__ __launch_bounds__(256) void quant_int8_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t T,
+                                                         int64_t H, uint8_t* __restrict__ q, float* __restrict__ s) {
+  __shared__ uint32_t part[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (t >= T) return;  // whole waves, and whole workgroups where they share a row
+  const int at = WAVES == 1 ? lane : (int)threadIdx.x;
+  constexpr int STRIDE = 64 * WAVES;
+  const int chunks = (int)(H / 8);
+  const v4i* src = reinterpret_cast<const v4i*>(x + t * ldx);
+  auto bits_of = [](const v4i& c, int i) { return ((uint32_t)c[i >> 1] >> (16 * (i & 1))) & 0xFFFFu; };
+  uint32_t m = 0;
+  v4i rows[IT > 0 ? IT : 1];
+  if constexpr (IT > 0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      rows[i] = at + i * STRIDE < chunks ? src[at + i * STRIDE] : (v4i){0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max_abs_bits(m, act_f32<FP16>(bits_of(rows[i], j)));
+  } else {
+    for (int c = at; c < chunks; c += STRIDE) {
+      const v4i v = src[c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max_abs_bits(m, act_f32<FP16>(bits_of(v, j)));
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)m, o);
+    m = y > m ? y : m;
+  }
+  if constexpr (WAVES > 1) {
+    if (lane == 0) part[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = part[w] > m ? part[w] : m;
+  }
+  const Int8RowScale r = int8_scale(m);
+  if (at == 0) s[t] = r.s;
+  auto codes = [&](const v4i& c) {
+    v2u w = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j >> 2] |= int8_code(act_f32<FP16>(bits_of(c, j)), r) << (8 * (j & 3));
+    return w;
+  };
+  v2u* dst = reinterpret_cast<v2u*>(q + t * H);
+  if constexpr (IT > 0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      if (at + i * STRIDE < chunks) dst[at + i * STRIDE] = codes(rows[i]);
+  } else {
+    for (int c = at; c < chunks; c += STRIDE) dst[c] = codes(src[c]);
+  }
+}
+
+// Rows that are not whole 16-byte chunks: a workgroup a row, an element at a time.
+template <bool FP16>
+__global__ __launch_bounds__(256) void quant_int8_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t H,
+                                                             uint8_t* __restrict__ q, float* __restrict__ s) {
+  __shared__ uint32_t part[4];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t m = 0;
+  for (int64_t c = threadIdx.x; c < H; c += 256) m = max_abs_bits(m, act_f32<FP16>(x[t * ldx + c]));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)m, o);
+    m = y > m ? y : m;
+  }
+  if (lane == 0) part[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = part[w] > m ? part[w] : m;
+  const Int8RowScale r = int8_scale(m);
+  if (threadIdx.x == 0) s[t] = r.s;
+  for (int64_t c = threadIdx.x; c < H; c += 256) q[t * H + c] = (uint8_t)int8_code(act_f32<FP16>(x[t * ldx + c]), r);
+}
+
+template <bool FP16>
+static int quant_int8(const uint16_t* x, int64_t ldx, int64_t T, int64_t H, uint8_t* q, float* s, hipStream_t st) {
+  const bool vec = H % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 7) == 0;
+  const dim3 by_wave((unsigned)((T + 3) / 4)), by_group((unsigned)T), threads(256);
+  if (!vec)
+    hipLaunchKernelGGL((quant_int8_any_kernel<FP16>), by_group, threads, 0, st, x, ldx, H, q, s);
+  else if (H <= 1024)
+    hipLaunchKernelGGL((quant_int8_kernel<FP16, 1, 2>), by_wave, threads, 0, st, x, ldx, T, H, q, s);
+  else if (H <= 4096)
+    hipLaunchKernelGGL((quant_int8_kernel<FP16, 1, 8>), by_wave, threads, 0, st, x, ldx, T, H, q, s);
+  else if (H <= 8192)
+    hipLaunchKernelGGL((quant_int8_kernel<FP16, 4, 4>), by_group, threads, 0, st, x, ldx, T, H, q, s);
+  else if (H <= 16384)
+    hipLaunchKernelGGL((quant_int8_kernel<FP16, 4, 8>), by_group, threads, 0, st, x, ldx, T, H, q, s);
+  else
+    hipLaunchKernelGGL((quant_int8_kernel<FP16, 4, 0>), by_group, threads, 0, st, x, ldx, T, H, q, s);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+}  // namespace moe
+
+extern "C" int moe_quant_int8(const void* x, int64_t ldx, int64_t T, int64_t H, int32_t dtype, void* q, float* scales,
+                              void* stream) {
+  using namespace moe;
+  if (T < 0 || H < 0 || T > 0x7FFFFFFF || ldx < H || (dtype != MOE_BF16 && dtype != MOE_FP16)) return kErrBadShape;
+  if (T == 0) return kOk;
+  if (!scales || (H > 0 && (!x || !q))) return kErrNullPointer;
+  if (((uintptr_t)x & 1) != 0 || ((uintptr_t)scales & 3) != 0) return kErrBadShape;
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == MOE_FP16 ? quant_int8<true>((const uint16_t*)x, ldx, T, H, (uint8_t*)q, scales, st)
+                           : quant_int8<false>((const uint16_t*)x, ldx, T, H, (uint8_t*)q, scales, st);
+}

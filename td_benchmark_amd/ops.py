@@ -50,18 +50,18 @@ def _stream(stream: torch.cuda.Stream | None = None) -> ctypes.c_void_p:
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype | None = None,
-          shape: tuple | None = None) -> None:
+          shape: tuple | None = None, anywhere: bool = False) -> None:
     """Checks of a tensor handed to the C ABI, which receives only pointers and
     sizes: a buffer smaller than the sizes say would be read or written out of
     bounds on the device, so dtype and shape are checked here, before the
-    contiguity and device checks."""
+    contiguity and device checks (``anywhere``: the caller checks the device)."""
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if not t.is_cuda:
+    if not t.is_cuda and not anywhere:
         raise ValueError(f"{name} must be a GPU tensor")
 
 
@@ -98,11 +98,11 @@ def _pad_fp8(w: torch.Tensor, dim: int, size: int) -> torch.Tensor:
 
 
 def _need_routing(sorted_token_ids: torch.Tensor, expert_ids: torch.Tensor,
-                  num_tokens_post_padded: torch.Tensor, block_m: int) -> None:
+                  num_tokens_post_padded: torch.Tensor, block_m: int, anywhere: bool = False) -> None:
     """moe_align_block_size outputs: one expert id per block of sorted positions."""
-    _need(sorted_token_ids, "sorted_token_ids", torch.int32)
-    _need(expert_ids, "expert_ids", torch.int32)
-    _need(num_tokens_post_padded, "num_tokens_post_padded", torch.int32)
+    _need(sorted_token_ids, "sorted_token_ids", torch.int32, anywhere=anywhere)
+    _need(expert_ids, "expert_ids", torch.int32, anywhere=anywhere)
+    _need(num_tokens_post_padded, "num_tokens_post_padded", torch.int32, anywhere=anywhere)
     if num_tokens_post_padded.numel() < 1:
         raise ValueError("num_tokens_post_padded must hold one element")
     if expert_ids.numel() * block_m < sorted_token_ids.numel():
@@ -173,7 +173,11 @@ def per_token_group_quant_fp8(x: torch.Tensor, group_size: int = 128,
 def moe_kernel_quantize_input(A: torch.Tensor, A_scale: torch.Tensor | None, quant_dtype: Any,
                               per_act_token_quant: bool, block_shape: list[int] | None = None):
     """Signature of vLLM's moe_kernel_quantize_input as the reference calls it
-    (overlap/overlap_forward.py:257-259): only the dynamic FP8 1x128 form."""
+    (overlap/overlap_forward.py:257-259): the dynamic FP8 1x128 form, and the
+    dynamic int8 form with a scale for each token (quant_dtype torch.int8,
+    per_act_token_quant, no block_shape)."""
+    if A_scale is None and quant_dtype == torch.int8 and per_act_token_quant and block_shape is None:
+        return per_token_quant_int8(A)
     if A_scale is not None or quant_dtype != FP8 or per_act_token_quant or list(block_shape or []) != BLOCK_SHAPE:
         raise NotImplementedError("only dynamic float8_e4m3fn with block_shape [128,128] is implemented")
     return per_token_group_quant_fp8(A)
@@ -282,9 +286,20 @@ def dispatch_fused_moe_kernel(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
     C is [M, top_k, N] or [S, 1, N]; rows are written by slot.  ``tile_order``
     selects the workgroup -> tile order (TILE_ORDERS) and ``tile_m`` the rows
     of a workgroup tile (a multiple of BLOCK_SIZE_M up to 256; 0 = automatic);
-    results depend on neither."""
+    results depend on neither.
+
+    With ``use_int8_w8a8``, ``per_channel_quant`` and not ``use_fp8_w8a8``, A
+    [rows, K] and B [E, N, K] are int8 with a scale for each row (A_scale [rows]
+    or [rows, 1]) and for each output channel (B_scale [E, N] or [E, N, 1]), and
+    C is bf16 or fp16; the tile is BLOCK_SIZE_M rows in expert order, so neither
+    ``tile_order`` nor ``tile_m`` is taken."""
+    if use_int8_w8a8 and per_channel_quant and not (use_fp8_w8a8 or use_int8_w8a16 or use_int4_w4a16):
+        _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_ids, expert_ids,
+                       num_tokens_post_padded, mul_routed_weight, top_k, config, block_shape, B_bias, a_by_pos,
+                       tile_order, tile_m)
+        return
     if not use_fp8_w8a8 or use_int8_w8a8 or use_int8_w8a16 or use_int4_w4a16 or per_channel_quant:
-        raise NotImplementedError("only fp8_w8a8 block-scaled GEMM is implemented")
+        raise NotImplementedError("only the fp8_w8a8 block-scaled and the int8_w8a8 per-channel GEMM are implemented")
     if B_zp is not None or B_bias is not None:
         raise NotImplementedError("zero points / bias are not on this path")
     if block_shape is not None and list(block_shape) != BLOCK_SHAPE:
@@ -1279,3 +1294,324 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
     check(L.moe_layer_run(layer, None, hidden_states.data_ptr(), topk_weights.data_ptr(), topk_ids.data_ptr(), H,
                           y.data_ptr(), _stream_handle()), "moe_layer_run")
     return y
+
+
+# ---------------------------------------------------------------------------
+# Products in 16-bit floats, grouped by expert, with their gradients
+# ---------------------------------------------------------------------------
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _need_here(*named: tuple[str, torch.Tensor | None]) -> None:
+    """The tensors are on the current device, whose current stream the launch
+    goes to: a pointer of another device would be read through the wrong one."""
+    for name, t in named:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{name} must be a GPU tensor")
+    here = torch.cuda.current_device()
+    for name, t in named:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are contiguous."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    if rows <= 1 or cols == 0:
+        return cols
+    if t.stride(0) < cols:
+        raise ValueError(f"{name} must have rows that do not overlap")
+    return t.stride(0)
+
+
+class ExpertSlots:
+    """The slots of a batch grouped by expert: what ``grouped_mm`` and its
+    gradients read, made once a batch for all of a layer's products.
+
+    ``topk_ids`` [T, top_k] int32 or int64 holds each slot's expert in [0,
+    num_experts); slots with any other id (dropped over a capacity, or on another
+    device) have no expert, and the products give them zero rows.
+    num_experts <= 1023.  ``block_size_m``: the align block size, by default from
+    the average slots of an expert.  The ids are copied, so ``topk_ids`` may
+    change afterwards."""
+
+    def __init__(self, topk_ids: torch.Tensor, num_experts: int, block_size_m: int | None = None):
+        if topk_ids.dim() != 2:
+            raise ValueError(f"topk_ids must be [T, top_k], got {tuple(topk_ids.shape)}")
+        if topk_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"topk_ids must be torch.int32 or torch.int64, got {topk_ids.dtype}")
+        if not 1 <= num_experts <= 1023:
+            raise ValueError(f"num_experts must be in [1, 1023], got {num_experts}")
+        self.T, self.top_k = topk_ids.shape
+        if self.top_k < 1:
+            raise ValueError("topk_ids has no slots for a token")
+        self.S, self.E = self.T * self.top_k, int(num_experts)
+        self.block_size_m = block_size_m or slots_block_m(self.S, self.E)
+        if self.block_size_m not in SUPPORTED_BLOCK_M:
+            raise ValueError(f"block_size_m must be one of {SUPPORTED_BLOCK_M}")
+        _need_here(("topk_ids", topk_ids))
+        self.device = topk_ids.device
+        # slot ids, sorted ids, block experts, the positions' count and align's workspace in one allocation
+        self.max_padded = align_max_padded(self.S, self.E + 1, self.block_size_m)
+        blocks = (self.max_padded + self.block_size_m - 1) // self.block_size_m
+        work = align_workspace_bytes(self.S, self.E + 1)
+        sizes = [max(n + 3, 4) // 4 * 4 for n in (self.S, self.max_padded, blocks, 1, (work + 3) // 4)]
+        buf = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
+        self._slot_ids, sorted_ids, expert_ids, ntpp, workspace = buf.split(sizes)
+        self.sorted_ids, self.expert_ids = sorted_ids[: max(self.max_padded, 1)], expert_ids[: max(blocks, 1)]
+        self.ntpp = ntpp[:1]
+        ids = topk_ids.contiguous()
+        check(lib().moe_expert_slots(_ptr(ids), ids.element_size(), self.S, self.E, self.block_size_m,
+                                     _ptr(self._slot_ids), _ptr(self.sorted_ids), _ptr(self.expert_ids),
+                                     _ptr(self.ntpp), self.max_padded, _ptr(workspace), _stream()),
+              "moe_expert_slots")
+
+
+def slots_block_m(num_slots: int, num_experts: int) -> int:
+    """The align block size of ExpertSlots, which is the rows of a tile of the
+    grouped products, from the average slots of an expert."""
+    avg = num_slots / max(num_experts, 1)
+    return 32 if avg <= 28 else 64 if avg <= 44 else 128 if avg <= 100 else 256
+
+
+def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> int:
+    """-> the slots of a row of x: top_k, or 1 where x has a row for each slot."""
+    if w.dim() != 3:
+        raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
+    if w.dtype != x.dtype:
+        raise TypeError(f"w must be {x.dtype} as x, got {w.dtype}")
+    if w.shape[0] != slots.E:
+        raise ValueError(f"w has {w.shape[0]} experts, the slots {slots.E}")
+    if x.dim() != 2 or x.shape[1] != w.shape[2]:
+        raise ValueError(f"x must be [rows, {w.shape[2]}], got {tuple(x.shape)}")
+    if x.shape[0] not in (slots.T, slots.S):
+        raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
+    if not w.is_contiguous():
+        raise ValueError("w must be contiguous")
+    _need_here(("x", x), ("w", w), ("slots", slots.sorted_ids))
+    _row_stride(x, "x")
+    return 1 if x.shape[0] == slots.S else slots.top_k
+
+
+def _grouped_product(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
+    k = _grouped_operands(x, w, slots)
+    E, N, K = w.shape
+    y = torch.empty((slots.S, N), dtype=x.dtype, device=x.device)
+    check(lib().moe_grouped_mm(_ptr(x), _row_stride(x, "x"), _ptr(w), _ptr(slots.sorted_ids), _ptr(slots.expert_ids),
+                               _ptr(slots.ntpp), slots.S, k, N, K, E, slots.block_size_m, slots.max_padded,
+                               _DTYPE_CODE[x.dtype], _ptr(y), _stream()), "moe_grouped_mm")
+    return y
+
+
+def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool = False) -> torch.Tensor:
+    """The gradient of ``grouped_mm`` by its rows: dx[s] = dy[s] @ w[e(s)], [S, K].
+    ``by_token``: summed over each token's slots (fp32, of the rows rounded to
+    dy's type), [T, K]."""
+    if dy.dim() != 2 or w.dim() != 3:
+        raise ValueError(f"dy must be [S, N] and w [E, N, K], got {tuple(dy.shape)} and {tuple(w.shape)}")
+    if dy.dtype not in _DTYPE_CODE:
+        raise TypeError(f"dy must be torch.bfloat16 or torch.float16, got {dy.dtype}")
+    E, N, K = w.shape
+    if E != slots.E:
+        raise ValueError(f"w has {E} experts, the slots {slots.E}")
+    _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
+    _need(w, "w", dy.dtype, anywhere=True)
+    _need_here(("dy", dy), ("w", w), ("slots", slots.sorted_ids))
+    dx = torch.empty((slots.S, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_grouped_mm_dgrad(_ptr(dy), _ptr(w), _ptr(slots.sorted_ids), _ptr(slots.expert_ids),
+                                     _ptr(slots.ntpp), slots.S, N, K, E, slots.block_size_m, slots.max_padded,
+                                     _DTYPE_CODE[dy.dtype], _ptr(dx), _stream()), "moe_grouped_mm_dgrad")
+    if not by_token or slots.top_k == 1:
+        return dx
+    out = torch.empty((slots.T, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_slot_sum(_ptr(dx), slots.T, slots.top_k, K, _DTYPE_CODE[dy.dtype], _ptr(out), _stream()),
+          "moe_slot_sum")
+    return out
+
+
+def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
+    """The gradient of ``grouped_mm`` by its weights: dw[e] = sum over the slots s
+    of e of dy[s]^T x[row(s)], [E, N, K] in dy's type; zeros for experts without
+    slots.  Each value is one fp32 sum in slot order, so equal inputs give equal
+    bits."""
+    if dy.dim() != 2 or x.dim() != 2:
+        raise ValueError(f"dy must be [S, N] and x [rows, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
+    if dy.dtype not in _DTYPE_CODE:
+        raise TypeError(f"dy must be torch.bfloat16 or torch.float16, got {dy.dtype}")
+    if x.dtype != dy.dtype:
+        raise TypeError(f"x must be {dy.dtype} as dy, got {x.dtype}")
+    N, K = dy.shape[1], x.shape[1]
+    _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
+    if x.shape[0] not in (slots.T, slots.S):
+        raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
+    _need_here(("dy", dy), ("x", x), ("slots", slots.sorted_ids))
+    dw = torch.empty((slots.E, N, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_grouped_mm_wgrad(_ptr(dy), _ptr(x), _row_stride(x, "x"), _ptr(slots.sorted_ids),
+                                     _ptr(slots.expert_ids), _ptr(slots.ntpp), slots.S,
+                                     1 if x.shape[0] == slots.S else slots.top_k, N, K, slots.E, slots.block_size_m,
+                                     slots.max_padded, _DTYPE_CODE[dy.dtype], _ptr(dw), _stream()),
+          "moe_grouped_mm_wgrad")
+    return dw
+
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
+        y = _grouped_product(x, w, slots)
+        ctx.save_for_backward(x, w)
+        ctx.slots = slots
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, dy: torch.Tensor):
+        x, w = ctx.saved_tensors
+        slots = ctx.slots
+        dy = dy.contiguous()  # a sum's gradient comes with stride 0
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = grouped_mm_dgrad(dy, w, slots, by_token=x.shape[0] != slots.S)
+        if ctx.needs_input_grad[1]:
+            dw = grouped_mm_wgrad(dy, x, slots)
+        return dx, dw, None
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
+    """y[s] = x[row(s)] @ w[e(s)]^T for every slot, [S, N]: the experts' product in
+    bf16 or fp16 (fp32 sums, rounded once), differentiable in x and w.
+
+    x [T, K] has a row for each token (its slots share it: a layer's first
+    product) or [S, K] for each slot (the second); rows may be strided.  w [E, N,
+    K] contiguous.  Slots without an expert get zero rows and add nothing to the
+    gradients.  Equal inputs give equal bits.  The gradients are once
+    differentiable; see grouped_mm_dgrad and grouped_mm_wgrad."""
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _GroupedMM.apply(x, w, slots)
+    return _grouped_product(x, w, slots)
+
+
+# ---------------------------------------------------------------------------
+# Products in 8-bit integers with a scale for each token and channel
+# ---------------------------------------------------------------------------
+
+INT8_MAX_K = 131071  # 2^14 K stays below 2^31
+
+
+def per_token_quant_int8(x: torch.Tensor, out_q: torch.Tensor | None = None,
+                         out_s: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [T, H] bf16 or fp16 -> (q [T, H] int8, scales [T, 1] fp32): scale =
+    max(amax / 127, 1e-12), q = clamp(rint(x / scale), +-127), ties to even.  Rows
+    of x may be strided.  A row with an infinity or a NaN gets it as its scale and
+    zero codes, so that its products are NaN."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
+    _need_here(("x", x), ("out_q", out_q), ("out_s", out_s))
+    T, H = x.shape
+    q = torch.empty((T, H), dtype=torch.int8, device=x.device) if out_q is None else out_q
+    s = torch.empty((T, 1), dtype=torch.float32, device=x.device) if out_s is None else out_s
+    _need(q, "out_q", torch.int8, (T, H), anywhere=True)
+    _need(s, "out_s", torch.float32, (T, 1), anywhere=True)
+    check(lib().moe_quant_int8(_ptr(x), _row_stride(x, "x"), T, H, _DTYPE_CODE[x.dtype], _ptr(q), _ptr(s), _stream()),
+          "moe_quant_int8")
+    return q, s
+
+
+def _need_scales(t: torch.Tensor, name: str, n: int) -> None:
+    _need(t, name, torch.float32, anywhere=True)
+    if t.numel() != n:
+        raise ValueError(f"{name} must hold {n} scales, got {tuple(t.shape)}")
+
+
+def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
+                   bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = (a @ b^T) * a_scale[m] * b_scale[n] + bias[n], [M, N] in ``out_dtype``
+    (bf16 or fp16): a [M, K] and b [N, K] int8 with a scale for each row of a
+    ([M] or [M, 1] fp32) and each row of b ([N] or [N, 1]).  The integer sums are
+    exact (K <= 131071), the rest is fp32, rounded once.  Rows of a, b and ``out``
+    may be strided; bias [N] in out_dtype."""
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        raise ValueError(f"a must be [M, K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
+    for t, name in ((a, "a"), (b, "b")):
+        if t.dtype != torch.int8:
+            raise TypeError(f"{name} must be torch.int8, got {t.dtype}")
+    M, K = a.shape
+    N = b.shape[0]
+    if K > INT8_MAX_K:
+        raise ValueError(f"K must be at most {INT8_MAX_K}, got {K}")
+    out_dtype = out.dtype if out is not None else out_dtype
+    if out_dtype not in _DTYPE_CODE:
+        raise TypeError(f"the output must be torch.bfloat16 or torch.float16, got {out_dtype}")
+    _need_scales(a_scale, "a_scale", M)
+    _need_scales(b_scale, "b_scale", N)
+    if bias is not None:
+        _need(bias, "bias", out_dtype, (N,), anywhere=True)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    elif tuple(out.shape) != (M, N):
+        raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
+    _need_here(("a", a), ("b", b), ("a_scale", a_scale), ("b_scale", b_scale), ("bias", bias), ("out", out))
+    check(lib().moe_int8_scaled_mm(_ptr(a), _row_stride(a, "a"), _ptr(a_scale), _ptr(b), _row_stride(b, "b"),
+                                   _ptr(b_scale), _ptr(bias), M, N, K, _DTYPE_CODE[out_dtype], _ptr(out),
+                                   _row_stride(out, "out"), _stream()), "moe_int8_scaled_mm")
+    return out
+
+
+def _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_ids, expert_ids,
+                   num_tokens_post_padded, mul_routed_weight, top_k, config, block_shape, B_bias, a_by_pos,
+                   tile_order, tile_m) -> None:
+    """dispatch_fused_moe_kernel's int8 form."""
+    if B_zp is not None or B_bias is not None:
+        raise NotImplementedError("zero points / bias are not on this path")
+    if block_shape is not None:
+        raise NotImplementedError("int8_w8a8 takes a scale for each row and channel, no block_shape")
+    if tile_order or tile_m:
+        raise NotImplementedError("tile_order and tile_m are of the fp8 form")
+    if B.dim() != 3:
+        raise ValueError(f"B must be [E, N, K], got {tuple(B.shape)}")
+    E, N, K = B.shape
+    if K > INT8_MAX_K:
+        raise ValueError(f"K must be at most {INT8_MAX_K}, got {K}")
+    _need(A, "A", torch.int8, anywhere=True)
+    _need(B, "B", torch.int8, anywhere=True)
+    if A.dim() != 2 or A.shape[1] != K:
+        raise ValueError(f"A must be [rows, {K}], got {tuple(A.shape)}")
+    if C.dtype not in _DTYPE_CODE:
+        raise TypeError(f"C must be torch.bfloat16 or torch.float16, got {C.dtype}")
+    _need(C, "C", anywhere=True)
+    if N == 0 or C.numel() % N or C.shape[-1] != N:
+        raise ValueError(f"C must have rows of {N}, got {tuple(C.shape)}")
+    if top_k < 1:
+        raise ValueError("top_k must be >= 1")
+    S = C.numel() // N
+    BM = int((config or {}).get("BLOCK_SIZE_M", 0)) or _block_m_from(sorted_token_ids, expert_ids)
+    if BM not in SUPPORTED_BLOCK_M:
+        raise ValueError(f"BLOCK_SIZE_M must be one of {SUPPORTED_BLOCK_M}")
+    _need_routing(sorted_token_ids, expert_ids, num_tokens_post_padded, BM, anywhere=True)
+    rows = sorted_token_ids.numel() if a_by_pos else (S + top_k - 1) // top_k
+    if A.shape[0] < rows:
+        raise ValueError(f"A has {A.shape[0]} rows, the routing reads {rows}")
+    _need_scales(A_scale, "A_scale", A.shape[0])
+    _need_scales(B_scale, "B_scale", E * N)
+    w = None
+    if mul_routed_weight:
+        if topk_weights is None:
+            raise ValueError("mul_routed_weight requires topk_weights")
+        w = topk_weights.contiguous().view(-1)
+        _need(w, "topk_weights", torch.float32, anywhere=True)
+        if w.numel() < S:
+            raise ValueError(f"topk_weights has {w.numel()} entries for {S} slots")
+    _need_here(("A", A), ("B", B), ("C", C), ("A_scale", A_scale), ("B_scale", B_scale), ("topk_weights", w),
+               ("sorted_token_ids", sorted_token_ids), ("expert_ids", expert_ids),
+               ("num_tokens_post_padded", num_tokens_post_padded))
+    check(lib().moe_grouped_gemm_int8(_ptr(A), _ptr(A_scale), _ptr(B), _ptr(B_scale), _ptr(sorted_token_ids),
+                                      _ptr(expert_ids), _ptr(num_tokens_post_padded), _ptr(w), S, top_k,
+                                      1 if a_by_pos else 0, N, K, E, BM, sorted_token_ids.numel(),
+                                      _DTYPE_CODE[C.dtype], _ptr(C), _stream()), "moe_grouped_gemm_int8")
