@@ -9,7 +9,7 @@
 //   by weights  dw[e, n, k] = sum over the slots s of e of dy[s, n] x[row(s), k]
 //   int8        y[s, n]  = (sum_k a[row, k] b[e, n, k]) * as[row] * bs[e, n] (+ bias[n]) (* w[s])
 // Sums are held in fp32 (int8: exactly, in 32-bit integers) and rounded once.
-#include "grouped_mm.hpp"
+#include "grouped_tile.hpp"
 
 namespace moe {
 
@@ -129,12 +129,14 @@ __global__ __launch_bounds__(256) void any_mm_kernel(MmArgs g) {
       for (int v = 0; v < 4; ++v) {
         const int64_t j = j0 + wn + c * 16 + 4 * kseg + v;
         if (j >= g.J) continue;
-        float f = (float)acc[r][c][v];
+        float f = 0.0f;
         if constexpr (EB == 1) {
-          if (!none) f = f * sa * g.Bs[(int64_t)e * g.J + j];
-          if (g.bias) f += from16<FP16>(g.bias[j]);
+          if (!none)
+            f = int8_out(acc[r][c][v], sa, g.Bs[(int64_t)e * g.J + j], g.bias, g.bias ? from16<FP16>(g.bias[j]) : 0.0f,
+                         g.topk_w, w);
+        } else {
+          f = acc[r][c][v];
         }
-        if (g.topk_w && !none) f *= w;
         reinterpret_cast<uint16_t*>(g.C)[orow * g.ldc + j] = (uint16_t)pack2<FP16>(f, 0.0f);
       }
   }
@@ -151,6 +153,36 @@ static int launch_any(MmArgs g, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
+// ---- whole, aligned chunks ---------------------------------------------------
+template <class OP, bool FP16, int FORM, class T>
+static int launch_tile(MmArgs g, hipStream_t st) {
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)tile_mm_kernel<OP, FP16, FORM, T>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          T::LDS_BYTES);
+  if (attr != hipSuccess) return kErrLaunch;
+  g.n_jt = (g.J + T::TN - 1) / T::TN;
+  const int64_t tiles = (FORM == kWgrad ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt;
+  const int64_t grid = (tiles + 7) / 8 * 8;
+  if (grid > 0x7FFFFFFF) return kErrBadShape;
+  hipLaunchKernelGGL((tile_mm_kernel<OP, FP16, FORM, T>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, st, g);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+template <class OP, bool FP16, int FORM>
+static int launch_rows(const MmArgs& g, hipStream_t st) {
+  switch (g.bm) {
+    case 16: return launch_tile<OP, FP16, FORM, MmTile<16, 256, 1, 3>>(g, st);
+    case 32: return launch_tile<OP, FP16, FORM, MmTile<32, 256, 1, 3>>(g, st);
+    case 64: return launch_tile<OP, FP16, FORM, MmTile<64, 256, 1, 3>>(g, st);
+    case 128: return launch_tile<OP, FP16, FORM, MmTile<128, 256, 2, 3>>(g, st);
+    default: return launch_tile<OP, FP16, FORM, MmTile<256, 256, 4, 2>>(g, st);
+  }
+}
+
+static bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// Whether rows at p with a stride of ld elements of `bytes` are whole 16-byte chunks.
+static bool chunks(const void* p, int64_t ld, int bytes) { return aligned(p, 16) && ld * bytes % 16 == 0; }
+
 constexpr int kBf16 = MOE_BF16, kFp16 = MOE_FP16;
 
 // What every grouped entry checks of the slots.
@@ -162,8 +194,6 @@ static int slots_ok(const int32_t* sorted, const int32_t* eids, const int32_t* n
   if (max_padded > 0 && (!sorted || !eids || !ntpp)) return kErrNullPointer;
   return kOk;
 }
-
-static bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 }  // namespace moe
 
@@ -200,6 +230,8 @@ extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const i
   g.top_k = top_k;
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
+  if (K > 0 && K % 8 == 0 && chunks(x, ldx, 2) && chunks(w, K, 2) && chunks(y, N, 2))
+    return dtype == kFp16 ? launch_rows<Fp16, true, kProduct>(g, st) : launch_rows<Bf16, false, kProduct>(g, st);
   return dtype == kFp16 ? launch_any<Fp16, true, false>(g, st) : launch_any<Bf16, false, false>(g, st);
 }
 
@@ -232,6 +264,8 @@ extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t
   g.top_k = 1;
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
+  if (N > 0 && chunks(dy, N, 2) && chunks(w, K, 2) && chunks(dx, K, 2))
+    return dtype == kFp16 ? launch_rows<Fp16, true, kDgrad>(g, st) : launch_rows<Bf16, false, kDgrad>(g, st);
   return dtype == kFp16 ? launch_any<Fp16, true, false>(g, st) : launch_any<Bf16, false, false>(g, st);
 }
 
@@ -264,11 +298,17 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   g.top_k = top_k;
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
+  if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2)) {
+    using T = MmTile<256, 256, 4, 2>;
+    return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
+  }
   return dtype == kFp16 ? launch_any<Fp16, true, true>(g, st) : launch_any<Bf16, false, true>(g, st);
 }
 
 // a [rows, K] and b [E, N, K] int8 with their scales, y in the output type.
 static int int8_product(MmArgs g, int32_t dtype, hipStream_t st) {
+  if (g.Cn > 0 && g.Cn % 16 == 0 && g.J % 8 == 0 && chunks(g.A, g.lda, 1) && chunks(g.B, g.sbj, 1) && chunks(g.C, g.ldc, 2))
+    return dtype == kFp16 ? launch_rows<Int8, true, kProduct>(g, st) : launch_rows<Int8, false, kProduct>(g, st);
   return dtype == kFp16 ? launch_any<Int8, true, false>(g, st) : launch_any<Int8, false, false>(g, st);
 }
 
@@ -334,8 +374,8 @@ extern "C" int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_sca
   g.sbj = ldb;
   g.sbc = 1;
   g.ldc = ldy;
-  g.bm = kAnyTile;
-  g.n_blocks = (M + kAnyTile - 1) / kAnyTile;
+  g.bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  g.n_blocks = (M + g.bm - 1) / g.bm;
   g.top_k = 1;
   g.E = 1;
   return int8_product(g, dtype, (hipStream_t)stream);

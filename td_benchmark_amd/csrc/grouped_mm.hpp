@@ -55,6 +55,17 @@ MOE_DEVICE float from16(uint16_t v) {
   else return bf16_to_f32(v);
 }
 
+// An int8 output before its rounding: each operation rounded in fp32 by itself,
+// so that every kernel gives the same bits for the same operands.
+MOE_DEVICE float int8_out(int acc, float sa, float sb, bool with_bias, float bias, bool weighted, float w) {
+#pragma clang fp contract(off)
+  float f = (float)acc * sa;
+  f = f * sb;
+  if (with_bias) f = f + bias;
+  if (weighted) f = f * w;
+  return f;
+}
+
 // One launch of a product.  With sorted, eids and ntpp (as moe_align_block_size
 // writes them): position p of block p / bm belongs to expert eids[p / bm] and
 // slot sorted[p] (S or more: none).  Without: S rows of one expert, slot p.

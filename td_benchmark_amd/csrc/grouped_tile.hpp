@@ -1,0 +1,392 @@
+// The LDS-tiled kernel of the grouped products (grouped_mm.hip): operands whose
+// rows are whole, aligned 16-byte chunks.
+//
+// A workgroup of eight waves computes TM x TN outputs.  An operand is staged by
+// rows, R rows of 128 bytes of the contraction, where it is contiguous along the
+// contraction (the product's x and w, the int8 operands, dy by rows), or by
+// columns, 64 contraction rows of R columns, where it is contiguous along the
+// output (w in the gradient by rows, dy and x in the gradient by weights).  Both
+// take R * 128 bytes of a stage and are filled by direct-to-LDS loads, 16 bytes a
+// lane from the lane's own address, so rows are gathered for nothing.  Fragments
+// of a row-staged operand are one ds_read_b128; of a column-staged one two
+// ds_read_b64_tr_b16, which hand each lane four consecutive contraction values of
+// its column.
+//
+// LDS rows hold their 16-byte chunks at index XOR a function of the row
+// (slot_of; col_swz), applied on the global side, so that the lanes read
+// together fall into distinct banks.
+#pragma once
+
+#include "grouped_mm.hpp"
+
+namespace moe {
+
+enum Form { kProduct, kDgrad, kWgrad };
+
+template <int TM_, int TN_, int WM_, int KS_>
+struct MmTile {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, KS = KS_;
+  static constexpr int NW = 8, THREADS = 64 * NW, WN = NW / WM;
+  static constexpr int RS = TM / WM / 16, CS = TN / WN / 16;  // 16-row and 16-column subtiles of a wave
+  static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int NA = TM / 8, NB = TN / 8;              // 1 KiB loads of a stage
+  static constexpr int NA_W = (NA + NW - 1) / NW, NB_W = (NB + NW - 1) / NW;
+  // loads of a stage that every wave issues at least: what may stay in flight of each younger stage
+  static constexpr int VM = NA / NW + NB / NW;
+  static constexpr int OFF_SLOT = KS * STAGE;       // slot of each row, its scale, its factor
+  static constexpr int OFF_IDS = OFF_SLOT + 12 * TM;  // kWgrad: slots of four steps
+  static constexpr int LDS_BYTES = OFF_IDS + 4 * 256;
+  static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && LDS_BYTES <= 160 * 1024, "tile");
+  static_assert(VM * (KS - 2) < 64, "vmcnt immediate");
+};
+
+// Chunk rotation of a column-staged row: the four rows that a group of 16 lanes
+// reads together differ in their two low bits, the groups in bit 3.
+MOE_DEVICE int col_swz(int row) { return ((row & 3) << 1) | (row & 8); }
+
+MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int N>
+MOE_DEVICE void mm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// 16 (or 4) bytes a lane from the lane's address to LDS at a uniform base, lanes
+// in order.  The kernel waits for them itself; M0 is written here only.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+MOE_DEVICE void lds_load16(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+MOE_DEVICE void lds_load4(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Read in the place of chunks past the contraction's end.
+__device__ const v4i kZeroChunk = {0, 0, 0, 0};
+
+typedef __attribute__((address_space(3))) uint8_t* lds_ptr;
+MOE_DEVICE v4i lds_frag(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) v4i*>((lds_ptr)(uintptr_t)at); }
+typedef short v4s __attribute__((ext_vector_type(4)));
+MOE_DEVICE v4i lds_frag_t(uint32_t at, int row_bytes) {
+  typedef __attribute__((address_space(3))) v4s* p4;
+  const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<p4>((lds_ptr)(uintptr_t)at));
+  const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<p4>((lds_ptr)(uintptr_t)(at + 4 * row_bytes)));
+  const v2u l = __builtin_bit_cast(v2u, lo), h = __builtin_bit_cast(v2u, hi);
+  return (v4i){(int)l[0], (int)l[1], (int)h[0], (int)h[1]};
+}
+
+// The workgroup's tile: block b and column tile j of the rows form.  Workgroups
+// are dealt to the XCDs in turn; each XCD takes a contiguous range of the tiles
+// in expert order, and within an expert the column tiles go in groups of four
+// with all its row tiles, so that the workgroups that share weights or rows run
+// together on one XCD's L2.
+MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
+  constexpr int kXcd = 8, kGroup = 4;
+  const int64_t nb = live_blocks(g);
+  const int64_t total = nb * g.n_jt, per = (total + kXcd - 1) / kXcd;
+  const int64_t pid = blockIdx.x;
+  const int64_t t = pid % kXcd * per + pid / kXcd;
+  if (pid / kXcd >= per || t >= total) return false;
+  b = t / g.n_jt;
+  int64_t b0 = 0, n = nb;
+  if (g.eids) {  // the run of blocks with b's expert
+    const int lane = threadIdx.x & 63;
+    const int e = g.eids[b];
+    int64_t back = 0, fwd = 1;
+    for (int64_t base = b - 1;; base -= 64, back += 64) {
+      const int64_t i = base - lane;
+      const uint64_t end = __ballot(!(i >= 0 && g.eids[i >= 0 ? i : 0] == e));
+      if (end) {
+        back += __ffsll((unsigned long long)end) - 1;
+        break;
+      }
+    }
+    for (int64_t base = b + 1;; base += 64, fwd += 64) {
+      const int64_t i = base + lane;
+      const uint64_t end = __ballot(!(i < nb && g.eids[i < nb ? i : 0] == e));
+      if (end) {
+        fwd += __ffsll((unsigned long long)end) - 1;
+        break;
+      }
+    }
+    b0 = b - back;
+    n = back + fwd;
+  }
+  const int64_t in = t - b0 * g.n_jt;
+  const int64_t j0 = in / (kGroup * n) * kGroup;
+  const int64_t w = g.n_jt - j0 < kGroup ? g.n_jt - j0 : kGroup;
+  j = j0 + (in - j0 * n) % w;
+  b = b0 + (in - j0 * n) / w;
+  return true;
+}
+
+template <class OP, bool FP16, int FORM, class T>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_mm_kernel(MmArgs g) {
+  constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS;
+  constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
+  constexpr int STEP = 128 / EB;  // contraction elements of a step
+  static_assert(EB == 2 || FORM == kProduct, "transposing reads are of 16-bit values");
+  static_assert(FORM != kWgrad || KS == 2, "the ring of slots is for two stages");
+  // the fragments' addresses are formed by XOR below 1 KiB
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
+  int32_t* smSlot = reinterpret_cast<int32_t*>(smem + T::OFF_SLOT);
+  float* smSa = reinterpret_cast<float*>(smem + T::OFF_SLOT + 4 * TM);
+  float* smW = reinterpret_cast<float*>(smem + T::OFF_SLOT + 8 * TM);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // ---- which tile ----
+  int64_t pos0, j0, i0 = 0, length;
+  int rows, e = 0, nvalid;
+  if constexpr (FORM == kWgrad) {
+    const int64_t nt = (g.Cn + TM - 1) / TM;
+    const int64_t per_e = nt * g.n_jt;
+    const int64_t total = per_e * g.E, per = (total + 7) / 8;
+    const int64_t t = (int64_t)(blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= per || t >= total) return;
+    e = (int)(t / per_e);
+    i0 = t % per_e / g.n_jt * TM;
+    j0 = t % g.n_jt * TN;
+    rows = nvalid = (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM);
+    const Run r = run_of(g, e);
+    pos0 = r.pos0;
+    length = r.count;
+  } else {
+    int64_t b, j;
+    if (!rows_tile(g, b, j)) return;
+    j0 = j * TN;
+    pos0 = b * TM;
+    rows = TM;
+    if (g.eids) e = g.eids[b];
+    else if (pos0 + rows > g.S) rows = (int)(g.S - pos0);
+    length = g.Cn;
+    // the slots, their scales and factors, for the epilogue and the rows' addresses
+    bool valid = false;
+    if (tid < TM) {
+      const uint32_t slot = tid >= rows ? (uint32_t)g.S : g.sorted ? (uint32_t)g.sorted[pos0 + tid] : (uint32_t)(pos0 + tid);
+      valid = slot < g.S;
+      smSlot[tid] = valid ? (int)slot : -1;
+      if constexpr (EB == 1) smSa[tid] = valid ? g.As[g.a_by_pos ? pos0 + tid : (int)slot / g.top_k] : 0.0f;
+      smW[tid] = valid && g.topk_w ? g.topk_w[slot] : 1.0f;
+    }
+    nvalid = __syncthreads_count(valid);
+    if (nvalid == 0) return;
+  }
+  if (e < 0 || e >= g.E) {  // no expert: zero rows
+    for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
+      const int64_t j = j0 + c % (TN / 8) * 8;
+      if (j < g.J)
+        *reinterpret_cast<v4i*>(g.C + ((int64_t)smSlot[c / (TN / 8)] * g.ldc + j) * 2) = (v4i){0, 0, 0, 0};
+    }
+    return;
+  }
+  const int KB = (int)((length + STEP - 1) / STEP);
+
+  // ---- addresses of this lane's part of the loads ----
+  // Instruction i of a wave is load wave + 8 i of its operand.
+  const uint8_t* a_ptr[T::NA_W];
+  const uint8_t* b_ptr[T::NB_W];
+  constexpr int ACPR = TM / 8, BCPR = TN / 8;  // chunks of a column-staged row
+  const uint8_t* b_base = g.B + (FORM == kWgrad ? 0 : (int64_t)e * g.b_es * EB);
+  const uint8_t* zeros = reinterpret_cast<const uint8_t*>(&kZeroChunk);
+  auto row_chunk = [&](int gi) { return slot_of(lane & 7, 8 * gi + (lane >> 3)); };
+  // contraction row and column chunk of a column-staged load
+  auto col_row = [&](int gi, int cpr) { return gi * (64 / cpr) + lane / cpr; };
+  auto col_of = [&](int gi, int cpr) { return ((lane % cpr) ^ (col_swz(col_row(gi, cpr)) & (cpr - 1))) * 8; };
+#pragma unroll
+  for (int i = 0; i < T::NA_W; ++i) {
+    const int gi = wave + 8 * i;
+    if constexpr (A_COLS) {
+      const int64_t c = i0 + col_of(gi, ACPR);
+      a_ptr[i] = g.A + (c < g.Cn ? c : 0) * EB;
+    } else {
+      const int row = 8 * gi + (lane >> 3);
+      const int slot = gi < T::NA ? smSlot[row] : -1;
+      const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + row : slot / g.top_k;
+      a_ptr[i] = g.A + ar * g.lda * EB + row_chunk(gi) * 16;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < T::NB_W; ++i) {
+    const int gi = wave + 8 * i;
+    if constexpr (B_COLS) {
+      const int64_t c = j0 + col_of(gi, BCPR);
+      b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
+      if constexpr (FORM == kDgrad) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
+    } else {
+      const int64_t j = j0 + 8 * gi + (lane >> 3);
+      b_ptr[i] = b_base + (j < g.J ? j : g.J - 1) * g.sbj * EB + row_chunk(gi) * 16;
+    }
+  }
+  // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
+  const int a_rows = KS == 2 ? (nvalid + 15) / 16 * 16 : TM;
+
+  // Step kk's loads into its stage.  Step 0 is the last, partial run of the
+  // contraction, so that no other step has to look for its end.
+  const int tail = (int)(length - (int64_t)(KB - 1) * STEP);  // elements of step 0
+  auto issue = [&](int kk, int stage) {
+    const uint32_t dst = lds0 + stage * T::STAGE;
+    const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
+    const int left = kk == 0 ? tail : STEP;
+    if constexpr (FORM == kWgrad) {
+      const int32_t* ids = reinterpret_cast<const int32_t*>(smem + T::OFF_IDS) + (kk & 3) * 64;
+#pragma unroll
+      for (int i = 0; i < T::NB_W; ++i) {
+        const int gi = wave + 8 * i, r = col_row(gi, BCPR);
+        const uint32_t slot = (uint32_t)ids[r];
+        const uint8_t* p = r < left ? b_ptr[i] + (int64_t)(slot / (uint32_t)g.top_k) * g.sbc * EB : zeros;
+        if (T::NB % 8 == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < T::NA_W; ++i) {
+        const int gi = wave + 8 * i, r = col_row(gi, ACPR);
+        const uint8_t* p = r < left ? a_ptr[i] + (int64_t)(uint32_t)ids[r] * g.lda * EB : zeros;
+        if (T::NA % 8 == 0 || gi < T::NA) lds_load16(p, dst + gi * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::NB_W; ++i) {
+        const int gi = wave + 8 * i;
+        const uint8_t* p = b_ptr[i] + (FORM == kDgrad ? c0 * g.sbc * EB : c0 * EB);
+        if (left < STEP) {
+          const bool in = FORM == kDgrad ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
+          p = in ? p : zeros;
+        }
+        if (T::NB % 8 == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < T::NA_W; ++i) {
+        const int gi = wave + 8 * i;
+        const uint8_t* p = a_ptr[i] + c0 * EB;
+        if (left < STEP) p = row_chunk(gi) * 16 < left * EB ? p : zeros;
+        if ((T::NA % 8 == 0 || gi < T::NA) && 8 * gi < a_rows) lds_load16(p, dst + gi * 1024);
+      }
+    }
+  };
+  // kWgrad: the slots of step kk, 64 positions, into the ring (the last wave).
+  auto issue_ids = [&](int kk) {
+    if (wave == 7 && kk < KB) {
+      const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
+      const int64_t c = c0 + lane < length ? c0 + lane : length - 1;
+      lds_load4(g.sorted + pos0 + c, lds0 + T::OFF_IDS + (kk & 3) * 256);
+    }
+  };
+
+  // ---- fragments ----
+  const int fr = lane & 15, kseg = lane >> 4;
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int row_base = wm * T::RS * 16, col_base = wn * T::CS * 16;
+  const uint32_t by_row = fr * 128 + (slot_of(kseg, fr) << 4);  // the second half of the step: XOR 64
+  const int t_row = 8 * kseg + (fr >> 2);
+  // column-staged, subtile s of the operand's columns from `base`: XOR s * 32 into the chunk
+  auto by_col = [&](int base, int w) {
+    return (uint32_t)(t_row * w * 2 + (((base / 8 + ((fr & 3) >> 1)) ^ col_swz(t_row)) << 4) + (fr & 1) * 8);
+  };
+  const uint32_t a_lane = A_COLS ? by_col(row_base, TM) : row_base * 128 + by_row;
+  const uint32_t b_lane = T::A_BYTES + (B_COLS ? by_col(col_base, TN) : col_base * 128 + by_row);
+
+  typename OP::Acc acc[T::RS][T::CS] = {};
+  int ra = (nvalid - row_base + 15) / 16;
+  ra = ra < 0 ? 0 : (ra > T::RS ? T::RS : ra);
+
+  if constexpr (FORM == kWgrad) {
+    if (KB > 0) {
+      issue_ids(0);
+      issue_ids(1);
+      mm_wait<0>();
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < KS - 1; ++s)
+    if (s < KB) issue(s, s);
+
+  auto kloop = [&](auto ra_c) {
+    constexpr int RA = decltype(ra_c)::value;
+    int stage = 0;
+    for (int kk = 0; kk < KB; ++kk) {
+      if constexpr (KS == 2) {
+        mm_wait<0>();
+      } else {
+        const int younger = KB - 1 - kk;
+        if (younger >= KS - 2) mm_wait<(KS - 2) * T::VM>();
+        else if (KS > 3 && younger >= KS - 3) mm_wait<(KS > 3 ? KS - 3 : 0) * T::VM>();
+        else mm_wait<0>();
+      }
+      mm_barrier();
+      if (kk + KS - 1 < KB) {
+        issue(kk + KS - 1, stage == 0 ? KS - 1 : stage - 1);
+        if constexpr (FORM == kWgrad) issue_ids(kk + 2);
+      }
+      if constexpr (RA > 0) {
+        const uint32_t st = lds0 + stage * T::STAGE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v4i af[RA];
+#pragma unroll
+          for (int r = 0; r < RA; ++r) {
+            if constexpr (A_COLS) af[r] = lds_frag_t((st + h * 32 * TM * 2 + a_lane) ^ (r * 32), TM * 2);
+            else af[r] = lds_frag((st + a_lane + r * 2048) ^ (h * 64));
+          }
+#pragma unroll
+          for (int c = 0; c < T::CS; ++c) {
+            v4i bf;
+            if constexpr (B_COLS) bf = lds_frag_t((st + h * 32 * TN * 2 + b_lane) ^ (c * 32), TN * 2);
+            else bf = lds_frag((st + b_lane + c * 2048) ^ (h * 64));
+#pragma unroll
+            for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf, af[r], acc[r][c]);
+          }
+        }
+      }
+      stage = stage == KS - 1 ? 0 : stage + 1;
+    }
+  };
+  switch (ra) {
+    case 0: kloop(std::integral_constant<int, 0>{}); break;
+    case 1: kloop(std::integral_constant<int, 1>{}); break;
+    case 2: if constexpr (T::RS >= 2) kloop(std::integral_constant<int, (T::RS >= 2 ? 2 : 1)>{}); break;
+    case 3: if constexpr (T::RS >= 3) kloop(std::integral_constant<int, (T::RS >= 3 ? 3 : 1)>{}); break;
+    default: if constexpr (T::RS >= 4) kloop(std::integral_constant<int, (T::RS >= 4 ? 4 : 1)>{}); break;
+  }
+  mm_barrier();
+
+  // ---- epilogue: rows of 16-bit outputs through LDS, chunks XOR the row ----
+  uint16_t* out = reinterpret_cast<uint16_t*>(smem);
+  constexpr int CH = TN / 8;
+#pragma unroll
+  for (int c = 0; c < T::CS; ++c) {
+    const int col = col_base + c * 16 + 4 * kseg;
+    float sb[4] = {1.0f, 1.0f, 1.0f, 1.0f}, bias[4] = {};
+    if constexpr (EB == 1) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int64_t j = j0 + col + v < g.J ? j0 + col + v : g.J - 1;
+        sb[v] = g.Bs[(int64_t)e * g.J + j];
+        if (g.bias) bias[v] = from16<FP16>(g.bias[j]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < T::RS; ++r) {
+      const int row = row_base + r * 16 + fr;
+      float f[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        if constexpr (EB == 1) f[v] = int8_out(acc[r][c][v], smSa[row], sb[v], g.bias, bias[v], g.topk_w, smW[row]);
+        else f[v] = acc[r][c][v];
+      }
+      v2u pk = {pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
+      *reinterpret_cast<v2u*>(out + row * TN + (((col >> 3) ^ (row & 15)) << 3) + (col & 7)) = pk;
+    }
+  }
+  __syncthreads();
+  for (int c = tid; c < nvalid * CH; c += T::THREADS) {
+    const int row = c / CH, cc = c % CH;
+    const int64_t j = j0 + cc * 8;
+    if (j >= g.J) continue;
+    const int64_t orow = FORM == kWgrad ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
+    *reinterpret_cast<v4i*>(g.C + (orow * g.ldc + j) * 2) =
+        *reinterpret_cast<const v4i*>(out + row * TN + ((cc ^ (row & 15)) << 3));
+  }
+}
+
+}  // namespace moe
