@@ -171,11 +171,11 @@ static int launch_tile(MmArgs g, hipStream_t st) {
 template <class OP, bool FP16, int FORM>
 static int launch_rows(const MmArgs& g, hipStream_t st) {
   switch (g.bm) {
-    case 16: return launch_tile<OP, FP16, FORM, MmTile<16, 256, 1, 3>>(g, st);
-    case 32: return launch_tile<OP, FP16, FORM, MmTile<32, 256, 1, 3>>(g, st);
-    case 64: return launch_tile<OP, FP16, FORM, MmTile<64, 256, 1, 3>>(g, st);
-    case 128: return launch_tile<OP, FP16, FORM, MmTile<128, 256, 2, 3>>(g, st);
-    default: return launch_tile<OP, FP16, FORM, MmTile<256, 256, 4, 2>>(g, st);
+    case 16: return launch_tile<OP, FP16, FORM, MmTile<16, 256, 8, 1, 3, 1>>(g, st);
+    case 32: return launch_tile<OP, FP16, FORM, MmTile<32, 256, 8, 1, 3, 1>>(g, st);
+    case 64: return launch_tile<OP, FP16, FORM, MmTile<64, 256, 8, 1, 3, 1>>(g, st);
+    case 128: return launch_tile<OP, FP16, FORM, MmTile<128, 256, 8, 2, 3, 1>>(g, st);
+    default: return launch_tile<OP, FP16, FORM, MmTile<256, 256, 8, 4, 2, 1>>(g, st);
   }
 }
 
@@ -299,7 +299,7 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
   if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2)) {
-    using T = MmTile<256, 256, 4, 2>;
+    using T = MmTile<256, 256, 8, 4, 2, 1>;
     return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
   }
   return dtype == kFp16 ? launch_any<Fp16, true, true>(g, st) : launch_any<Bf16, false, true>(g, st);

@@ -1,7 +1,7 @@
 // The LDS-tiled kernel of the grouped products (grouped_mm.hip): operands whose
 // rows are whole, aligned 16-byte chunks.
 //
-// A workgroup of eight waves computes TM x TN outputs.  An operand is staged by
+// A workgroup computes TM x TN outputs.  An operand is staged by
 // rows, R rows of 128 bytes of the contraction, where it is contiguous along the
 // contraction (the product's x and w, the int8 operands, dy by rows), or by
 // columns, 64 contraction rows of R columns, where it is contiguous along the
@@ -23,10 +23,12 @@ namespace moe {
 
 enum Form { kProduct, kDgrad, kWgrad };
 
-template <int TM_, int TN_, int WM_, int KS_>
+// TM x TN outputs by NW waves, WM of them along the rows, from a ring of KS
+// stages, WGS workgroups a CU.
+template <int TM_, int TN_, int NW_, int WM_, int KS_, int WGS_>
 struct MmTile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, KS = KS_;
-  static constexpr int NW = 8, THREADS = 64 * NW, WN = NW / WM;
+  static constexpr int TM = TM_, TN = TN_, NW = NW_, WM = WM_, KS = KS_, WGS = WGS_;
+  static constexpr int THREADS = 64 * NW, WN = NW / WM, WPE = NW * WGS < 4 ? 1 : NW * WGS / 4;
   static constexpr int RS = TM / WM / 16, CS = TN / WN / 16;  // 16-row and 16-column subtiles of a wave
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int NA = TM / 8, NB = TN / 8;              // 1 KiB loads of a stage
@@ -36,8 +38,8 @@ struct MmTile {
   static constexpr int OFF_SLOT = KS * STAGE;       // slot of each row, its scale, its factor
   static constexpr int OFF_IDS = OFF_SLOT + 12 * TM;  // kWgrad: slots of four steps
   static constexpr int LDS_BYTES = OFF_IDS + 4 * 256;
-  static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && LDS_BYTES <= 160 * 1024, "tile");
-  static_assert(VM * (KS - 2) < 64, "vmcnt immediate");
+  static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && (LDS_BYTES + 1024) * WGS <= 160 * 1024, "tile");
+  static_assert(VM * (KS - 1) < 64, "vmcnt immediate");
 };
 
 // Chunk rotation of a column-staged row: the four rows that a group of 16 lanes
@@ -47,16 +49,29 @@ MOE_DEVICE int col_swz(int row) { return ((row & 3) << 1) | (row & 8); }
 MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
 MOE_DEVICE void mm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// Waits for the oldest stage in flight: of the `younger` ones behind it, at most
+// MAX, every wave has at least VM loads each.
+template <int MAX, int VM>
+MOE_DEVICE void mm_wait_stages(int younger) {
+  if constexpr (MAX <= 0) {
+    mm_wait<0>();
+  } else {
+    if (younger >= MAX) mm_wait<MAX * VM>();
+    else mm_wait_stages<MAX - 1, VM>(younger);
+  }
+}
 
 // 16 (or 4) bytes a lane from the lane's address to LDS at a uniform base, lanes
-// in order.  The kernel waits for them itself; M0 is written here only.
+// in order.  The kernel waits for them itself; M0 is written here only.  Not a
+// clobber of memory: the fragments' reads may be moved across, which never reads
+// the stage being filled; the barriers, which are, keep both in their step.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 MOE_DEVICE void lds_load16(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "m0");
 }
 MOE_DEVICE void lds_load4(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "m0");
 }
 #pragma clang diagnostic pop
 
@@ -120,7 +135,7 @@ MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
 }
 
 template <class OP, bool FP16, int FORM, class T>
-__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_mm_kernel(MmArgs g) {
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::WPE, T::WPE))) void tile_mm_kernel(MmArgs g) {
   constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS;
   constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
   constexpr int STEP = 128 / EB;  // contraction elements of a step
@@ -162,6 +177,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     length = g.Cn;
     // the slots, their scales and factors, for the epilogue and the rows' addresses
     bool valid = false;
+    static_assert(TM <= T::THREADS, "a thread a row");
     if (tid < TM) {
       const uint32_t slot = tid >= rows ? (uint32_t)g.S : g.sorted ? (uint32_t)g.sorted[pos0 + tid] : (uint32_t)(pos0 + tid);
       valid = slot < g.S;
@@ -183,7 +199,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   const int KB = (int)((length + STEP - 1) / STEP);
 
   // ---- addresses of this lane's part of the loads ----
-  // Instruction i of a wave is load wave + 8 i of its operand.
+  // Instruction i of a wave is load wave + NW i of its operand.
   const uint8_t* a_ptr[T::NA_W];
   const uint8_t* b_ptr[T::NB_W];
   constexpr int ACPR = TM / 8, BCPR = TN / 8;  // chunks of a column-staged row
@@ -195,7 +211,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   auto col_of = [&](int gi, int cpr) { return ((lane % cpr) ^ (col_swz(col_row(gi, cpr)) & (cpr - 1))) * 8; };
 #pragma unroll
   for (int i = 0; i < T::NA_W; ++i) {
-    const int gi = wave + 8 * i;
+    const int gi = wave + T::NW * i;
     if constexpr (A_COLS) {
       const int64_t c = i0 + col_of(gi, ACPR);
       a_ptr[i] = g.A + (c < g.Cn ? c : 0) * EB;
@@ -208,7 +224,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   }
 #pragma unroll
   for (int i = 0; i < T::NB_W; ++i) {
-    const int gi = wave + 8 * i;
+    const int gi = wave + T::NW * i;
     if constexpr (B_COLS) {
       const int64_t c = j0 + col_of(gi, BCPR);
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
@@ -221,51 +237,59 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
   const int a_rows = KS == 2 ? (nvalid + 15) / 16 * 16 : TM;
 
-  // Step kk's loads into its stage.  Step 0 is the last, partial run of the
-  // contraction, so that no other step has to look for its end.
+  // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
+  // partial run of the contraction, so that no other step has to look for its
+  // end; the addresses of the others advance from load to load.
   const int tail = (int)(length - (int64_t)(KB - 1) * STEP);  // elements of step 0
-  auto issue = [&](int kk, int stage) {
+  const int64_t b_step = FORM == kDgrad ? STEP * g.sbc * EB : 128;
+  constexpr int ND = T::NA_W + T::NB_W;
+  auto load = [&](int kk, int stage, auto dc, auto first_c) {
+    constexpr int d = decltype(dc)::value;
+    constexpr bool first = decltype(first_c)::value;
     const uint32_t dst = lds0 + stage * T::STAGE;
-    const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
-    const int left = kk == 0 ? tail : STEP;
+    const int left = first ? tail : STEP;
+    constexpr bool is_b = d < T::NB_W;
+    constexpr int i = is_b ? d : d - T::NB_W;
+    const int gi = wave + T::NW * i;
     if constexpr (FORM == kWgrad) {
-      const int32_t* ids = reinterpret_cast<const int32_t*>(smem + T::OFF_IDS) + (kk & 3) * 64;
-#pragma unroll
-      for (int i = 0; i < T::NB_W; ++i) {
-        const int gi = wave + 8 * i, r = col_row(gi, BCPR);
-        const uint32_t slot = (uint32_t)ids[r];
-        const uint8_t* p = r < left ? b_ptr[i] + (int64_t)(slot / (uint32_t)g.top_k) * g.sbc * EB : zeros;
-        if (T::NB % 8 == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
+      const int r = col_row(gi, is_b ? BCPR : ACPR);
+      const uint32_t slot = (uint32_t)reinterpret_cast<const int32_t*>(smem + T::OFF_IDS)[(kk & 3) * 64 + r];
+      const uint8_t* p;
+      if constexpr (is_b) p = b_ptr[i] + (int64_t)(slot / (uint32_t)g.top_k) * g.sbc * EB;
+      else p = a_ptr[i] + (int64_t)slot * g.lda * EB;
+      p = r < left ? p : zeros;
+      if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
+        lds_load16(p, dst + (is_b ? T::A_BYTES : 0) + gi * 1024);
+    } else if constexpr (is_b) {
+      const uint8_t* p = b_ptr[i];
+      if constexpr (first) {
+        p += (KB - 1) * b_step;
+        const bool in = FORM == kDgrad ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
+        p = in ? p : zeros;
+      } else {
+        b_ptr[i] += b_step;
       }
-#pragma unroll
-      for (int i = 0; i < T::NA_W; ++i) {
-        const int gi = wave + 8 * i, r = col_row(gi, ACPR);
-        const uint8_t* p = r < left ? a_ptr[i] + (int64_t)(uint32_t)ids[r] * g.lda * EB : zeros;
-        if (T::NA % 8 == 0 || gi < T::NA) lds_load16(p, dst + gi * 1024);
-      }
+      if (T::NB % T::NW == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
     } else {
-#pragma unroll
-      for (int i = 0; i < T::NB_W; ++i) {
-        const int gi = wave + 8 * i;
-        const uint8_t* p = b_ptr[i] + (FORM == kDgrad ? c0 * g.sbc * EB : c0 * EB);
-        if (left < STEP) {
-          const bool in = FORM == kDgrad ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
-          p = in ? p : zeros;
-        }
-        if (T::NB % 8 == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
+      const uint8_t* p = a_ptr[i];
+      if constexpr (first) {
+        p += (int64_t)(KB - 1) * 128;
+        p = row_chunk(gi) * 16 < left * EB ? p : zeros;
+      } else {
+        a_ptr[i] += 128;
       }
-#pragma unroll
-      for (int i = 0; i < T::NA_W; ++i) {
-        const int gi = wave + 8 * i;
-        const uint8_t* p = a_ptr[i] + c0 * EB;
-        if (left < STEP) p = row_chunk(gi) * 16 < left * EB ? p : zeros;
-        if ((T::NA % 8 == 0 || gi < T::NA) && 8 * gi < a_rows) lds_load16(p, dst + gi * 1024);
-      }
+      if ((T::NA % T::NW == 0 || gi < T::NA) && 8 * gi < a_rows) lds_load16(p, dst + gi * 1024);
     }
+  };
+  // Loads [from, to) of step kk.
+  auto loads = [&](int kk, int stage, auto from, auto to, auto first) {
+    [&]<int... D>(std::integer_sequence<int, D...>) {
+      (load(kk, stage, std::integral_constant<int, decltype(from)::value + D>{}, first), ...);
+    }(std::make_integer_sequence<int, decltype(to)::value - decltype(from)::value>{});
   };
   // kWgrad: the slots of step kk, 64 positions, into the ring (the last wave).
   auto issue_ids = [&](int kk) {
-    if (wave == 7 && kk < KB) {
+    if (wave == T::NW - 1 && kk < KB) {
       const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
       const int64_t c = c0 + lane < length ? c0 + lane : length - 1;
       lds_load4(g.sorted + pos0 + c, lds0 + T::OFF_IDS + (kk & 3) * 256);
@@ -291,54 +315,102 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 
   if constexpr (FORM == kWgrad) {
     if (KB > 0) {
-      issue_ids(0);
-      issue_ids(1);
+      for (int s = 0; s <= KS; ++s) issue_ids(s);
       mm_wait<0>();
     }
     __syncthreads();
   }
+  const std::integral_constant<int, 0> none;
+  const std::integral_constant<int, ND> all;
+  if (KB > 0) loads(0, 0, none, all, std::true_type{});
 #pragma unroll
-  for (int s = 0; s < KS - 1; ++s)
-    if (s < KB) issue(s, s);
+  for (int s = 1; s < KS; ++s)
+    if (s < KB) loads(s, s, none, all, std::false_type{});
 
+  // A step is 2 CS slots of RS matrix instructions, one weight fragment each, which
+  // is read two slots ahead.  The barrier that hands over the next stage stands two
+  // slots before the step's end, when every fragment of this stage has been read:
+  // the last two slots' instructions cover the reads of the next stage's first
+  // fragments, and this stage's buffer is filled again from there on, a load a slot.
+  constexpr int NQ = 2 * T::CS;
+  constexpr int DPQ = (ND + NQ - 1) / NQ;  // loads of a slot
+  static_assert(NQ >= 4 && NQ % 4 == 0, "four fragment registers in turn");
   auto kloop = [&](auto ra_c) {
     constexpr int RA = decltype(ra_c)::value;
+    if (KB == 0) return;
+    v4i af[2][RA > 0 ? RA : 1], bf[4];
+    auto read_a = [&](int stage, int h, int r) {
+      const uint32_t st = lds0 + stage * T::STAGE;
+      if constexpr (A_COLS) af[h][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 32 * TM * 2, TM * 2);
+      else af[h][r] = lds_frag(st + (a_lane ^ (h * 64)) + r * 2048);
+    };
+    auto read_b = [&](int stage, int q) {
+      const uint32_t st = lds0 + stage * T::STAGE;
+      const int h = q / T::CS, c = q % T::CS;
+      if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 32 * TN * 2, TN * 2);
+      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 64)) + c * 2048);
+    };
+    // stage 0; of the others every wave has at least so many loads behind it
+    mm_wait_stages<KS - 1, KS == 2 ? T::NB / T::NW : T::VM>(KB - 1);
+    mm_barrier();
+    if constexpr (RA > 0) {
+#pragma unroll
+      for (int r = 0; r < RA; ++r) read_a(0, 0, r);
+      read_b(0, 0);
+      read_b(0, 1);
+    }
     int stage = 0;
     for (int kk = 0; kk < KB; ++kk) {
-      if constexpr (KS == 2) {
-        mm_wait<0>();
-      } else {
-        const int younger = KB - 1 - kk;
-        if (younger >= KS - 2) mm_wait<(KS - 2) * T::VM>();
-        else if (KS > 3 && younger >= KS - 3) mm_wait<(KS > 3 ? KS - 3 : 0) * T::VM>();
-        else mm_wait<0>();
-      }
-      mm_barrier();
-      if (kk + KS - 1 < KB) {
-        issue(kk + KS - 1, stage == 0 ? KS - 1 : stage - 1);
-        if constexpr (FORM == kWgrad) issue_ids(kk + 2);
-      }
-      if constexpr (RA > 0) {
-        const uint32_t st = lds0 + stage * T::STAGE;
+      const int next = stage == KS - 1 ? 0 : stage + 1, prev = stage == 0 ? KS - 1 : stage - 1;
+      auto slot = [&](auto qc) {
+        constexpr int Q = decltype(qc)::value;
+        if constexpr (Q == NQ - 2) {
+          if (kk + 1 < KB) {
+            mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
+            mm_barrier();
+            if constexpr (RA > 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          v4i af[RA];
-#pragma unroll
-          for (int r = 0; r < RA; ++r) {
-            if constexpr (A_COLS) af[r] = lds_frag_t((st + h * 32 * TM * 2 + a_lane) ^ (r * 32), TM * 2);
-            else af[r] = lds_frag((st + a_lane + r * 2048) ^ (h * 64));
-          }
-#pragma unroll
-          for (int c = 0; c < T::CS; ++c) {
-            v4i bf;
-            if constexpr (B_COLS) bf = lds_frag_t((st + h * 32 * TN * 2 + b_lane) ^ (c * 32), TN * 2);
-            else bf = lds_frag((st + b_lane + c * 2048) ^ (h * 64));
-#pragma unroll
-            for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf, af[r], acc[r][c]);
+              for (int r = 0; r < RA; ++r) read_a(next, 0, r);
+              read_b(next, 0);
+              read_b(next, 1);
+            }
+            if constexpr (FORM == kWgrad)
+              if (kk + KS < KB) issue_ids(kk + KS + 1);
           }
         }
-      }
-      stage = stage == KS - 1 ? 0 : stage + 1;
+        if constexpr (RA > 0 && Q < NQ - 2) {
+          read_b(stage, Q + 2);
+          // the second half's rows: one a slot up to two slots ahead, or together
+          if constexpr (T::CS > RA + 1 && Q + RA >= T::CS - 1 && Q < T::CS - 1) read_a(stage, 1, Q + RA - (T::CS - 1));
+          if constexpr (T::CS <= RA + 1 && Q == 0) {
+#pragma unroll
+            for (int r = 0; r < RA; ++r) read_a(stage, 1, r);
+          }
+        }
+        // loads of stage kk + KS in this step's last two slots, of the stage before it in the others
+        constexpr int from = (Q + 2) % NQ * DPQ, to = from + DPQ < ND ? from + DPQ : ND;
+        if constexpr (from < ND) {
+          const std::integral_constant<int, from> f;
+          const std::integral_constant<int, to> t;
+          if constexpr (Q >= NQ - 2) {
+            if (kk + KS < KB) loads(kk + KS, stage, f, t, std::false_type{});
+          } else {
+            if (kk > 0 && kk - 1 + KS < KB) loads(kk - 1 + KS, prev, f, t, std::false_type{});
+          }
+        }
+        // the reads stay ahead of the instructions, which the compiler would undo
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (RA > 0) {
+          constexpr int h = Q / T::CS, c = Q % T::CS;
+#pragma unroll
+          for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf[Q & 3], af[h][r], acc[r][c]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      [&]<int... Q>(std::integer_sequence<int, Q...>) {
+        (slot(std::integral_constant<int, Q>{}), ...);
+      }(std::make_integer_sequence<int, NQ>{});
+      stage = next;
     }
   };
   switch (ra) {
