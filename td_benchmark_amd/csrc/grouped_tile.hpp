@@ -42,9 +42,14 @@ struct MmTile {
   static_assert(VM * (KS - 1) < 64, "vmcnt immediate");
 };
 
+// A step's contraction is split between its two instructions by chunks of 16
+// bytes: lane (fr, kseg) takes chunk 2 kseg of its row for the first and 2 kseg + 1
+// for the second (with slot_of the lanes that a ds_read_b128 serves together then
+// hit distinct banks; 4 h + kseg gave two-way conflicts, half of the LDS cycles),
+// of a column-staged operand rows 16 kseg + 8 h to + 7.
 // Chunk rotation of a column-staged row: the four rows that a group of 16 lanes
-// reads together differ in their two low bits, the groups in bit 3.
-MOE_DEVICE int col_swz(int row) { return ((row & 3) << 1) | (row & 8); }
+// reads together differ in their two low bits, the groups in bit 4.
+MOE_DEVICE int col_swz(int row) { return ((row & 3) << 1) | ((row >> 1) & 8); }
 
 MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
@@ -300,8 +305,8 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   const int fr = lane & 15, kseg = lane >> 4;
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int row_base = wm * T::RS * 16, col_base = wn * T::CS * 16;
-  const uint32_t by_row = fr * 128 + (slot_of(kseg, fr) << 4);  // the second half of the step: XOR 64
-  const int t_row = 8 * kseg + (fr >> 2);
+  const uint32_t by_row = fr * 128 + (slot_of(2 * kseg, fr) << 4);  // the second half of the step: XOR 16
+  const int t_row = 16 * kseg + (fr >> 2);                          // and 8 rows on
   // column-staged, subtile s of the operand's columns from `base`: XOR s * 32 into the chunk
   auto by_col = [&](int base, int w) {
     return (uint32_t)(t_row * w * 2 + (((base / 8 + ((fr & 3) >> 1)) ^ col_swz(t_row)) << 4) + (fr & 1) * 8);
@@ -341,14 +346,14 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     v4i af[2][RA > 0 ? RA : 1], bf[4];
     auto read_a = [&](int stage, int h, int r) {
       const uint32_t st = lds0 + stage * T::STAGE;
-      if constexpr (A_COLS) af[h][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 32 * TM * 2, TM * 2);
-      else af[h][r] = lds_frag(st + (a_lane ^ (h * 64)) + r * 2048);
+      if constexpr (A_COLS) af[h][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 8 * TM * 2, TM * 2);
+      else af[h][r] = lds_frag(st + (a_lane ^ (h * 16)) + r * 2048);
     };
     auto read_b = [&](int stage, int q) {
       const uint32_t st = lds0 + stage * T::STAGE;
       const int h = q / T::CS, c = q % T::CS;
-      if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 32 * TN * 2, TN * 2);
-      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 64)) + c * 2048);
+      if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 8 * TN * 2, TN * 2);
+      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 16)) + c * 2048);
     };
     // stage 0; of the others every wave has at least so many loads behind it
     mm_wait_stages<KS - 1, KS == 2 ? T::NB / T::NW : T::VM>(KB - 1);
