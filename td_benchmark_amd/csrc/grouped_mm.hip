@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void any_mm_kernel(MmArgs g) {
   if constexpr (!WEIGHTS) {
     if (run_r < rows) {
       const int64_t slot = slot_at(pos0 + run_r);
-      if (slot < g.S) a_row = g.A + (g.a_by_pos ? pos0 + run_r : slot / g.top_k) * g.lda * EB;
+      if (slot < g.S) a_row = g.A + (g.a_by_pos ? pos0 + run_r : (int64_t)slot_row(g, (uint32_t)slot)) * g.lda * EB;
     }
     const int64_t j = j0 + (b_by_j ? col_r : run_r);
     if (j < g.J && !none) b_row = g.B + ((int64_t)e * g.b_es + j * g.sbj) * EB;
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void any_mm_kernel(MmArgs g) {
         const int64_t slot = c < length ? slot_at(pos0 + c) : g.S;
         const bool on = slot < g.S;
         a[q] = on && col_r < rows ? reinterpret_cast<const E*>(g.A)[slot * g.lda + i0 + col_r] : (E)0;
-        b[q] = on && j0 + col_r < g.J ? reinterpret_cast<const E*>(g.B)[slot / g.top_k * g.sbc + j0 + col_r] : (E)0;
+        b[q] = on && j0 + col_r < g.J ? reinterpret_cast<const E*>(g.B)[(int64_t)slot_row(g, (uint32_t)slot) * g.sbc + j0 + col_r] : (E)0;
       } else {
         const int64_t ca = c0 + run_c + q, cb = c0 + (b_by_j ? col_c : run_c) + q;
         a[q] = a_row && ca < length ? reinterpret_cast<const E*>(a_row)[ca] : (E)0;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void any_mm_kernel(MmArgs g) {
     } else {
       orow = slot_at(pos0 + row);
       if (orow >= g.S) continue;
-      arow = g.a_by_pos ? pos0 + row : orow / g.top_k;
+      arow = g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)orow);
       if (g.topk_w) w = g.topk_w[orow];
       if constexpr (EB == 1) sa = g.As[arow];
     }
@@ -227,7 +227,7 @@ extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const i
   g.ldc = N;
   g.n_blocks = max_padded / BM;
   g.bm = BM;
-  g.top_k = top_k;
+  set_top_k(g, top_k);
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
   if (K > 0 && K % 8 == 0 && chunks(x, ldx, 2) && chunks(w, K, 2) && chunks(y, N, 2))
@@ -261,7 +261,7 @@ extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t
   g.ldc = K;
   g.n_blocks = max_padded / BM;
   g.bm = BM;
-  g.top_k = 1;
+  set_top_k(g, 1);
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
   if (N > 0 && chunks(dy, N, 2) && chunks(w, K, 2) && chunks(dx, K, 2))
@@ -295,10 +295,11 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   g.ldc = K;
   g.n_blocks = max_padded / BM;
   g.bm = BM;
-  g.top_k = top_k;
+  set_top_k(g, top_k);
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
-  if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2)) {
+  if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2) &&
+      N < (1 << 30) && ldx < (1 << 30)) {
     using T = MmTile<256, 256, 8, 4, 2, 1>;
     return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
   }
@@ -346,7 +347,7 @@ extern "C" int moe_grouped_gemm_int8(const void* a, const float* a_scale, const 
   g.ldc = N;
   g.n_blocks = max_padded / BM;
   g.bm = BM;
-  g.top_k = top_k;
+  set_top_k(g, top_k);
   g.a_by_pos = a_by_pos ? 1 : 0;
   g.E = E;
   return int8_product(g, dtype, (hipStream_t)stream);
@@ -376,7 +377,7 @@ extern "C" int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_sca
   g.ldc = ldy;
   g.bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
   g.n_blocks = (M + g.bm - 1) / g.bm;
-  g.top_k = 1;
+  set_top_k(g, 1);
   g.E = 1;
   return int8_product(g, dtype, (hipStream_t)stream);
 }

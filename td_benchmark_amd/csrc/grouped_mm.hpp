@@ -96,7 +96,24 @@ struct MmArgs {
   int64_t n_jt;         // column tiles
   int64_t n_blocks;     // blocks that fit in max_padded
   int bm, top_k, a_by_pos, E;
+  // slot / top_k = slot * div_mul >> div_shift for slots below 2^31
+  uint32_t div_mul;
+  int div_shift;
 };
+
+// Sets top_k and its division: with l = ceil(log2 k) and m = floor(2^(31+l) / k) + 1
+// the error m k - 2^(31+l) is at most k <= 2^l, so the quotient is exact.
+inline void set_top_k(MmArgs& g, int32_t k) {
+  int l = 0;
+  while (((int64_t)1 << l) < k) ++l;
+  g.top_k = k;
+  g.div_mul = (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)k + 1);
+  g.div_shift = 31 + l;
+}
+// The row of A (weights form: of B) that a slot reads.
+MOE_DEVICE uint32_t slot_row(const MmArgs& g, uint32_t slot) {
+  return (uint32_t)((uint64_t)slot * g.div_mul >> g.div_shift);
+}
 
 // Blocks that hold slots (ntpp is the device's word: kept to what was allocated).
 MOE_DEVICE int64_t live_blocks(const MmArgs& g) {

@@ -35,10 +35,11 @@ struct MmTile {
   static constexpr int NA_W = (NA + NW - 1) / NW, NB_W = (NB + NW - 1) / NW;
   // loads of a stage that every wave issues at least: what may stay in flight of each younger stage
   static constexpr int VM = NA / NW + NB / NW;
-  static constexpr int OFF_SLOT = KS * STAGE;       // slot of each row, its scale, its factor
-  static constexpr int OFF_IDS = OFF_SLOT + 12 * TM;  // kWgrad: slots of four steps
-  static constexpr int LDS_BYTES = OFF_IDS + 4 * 256;
-  static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && (LDS_BYTES + 1024) * WGS <= 160 * 1024, "tile");
+  // LDS: the rows' table (slot, scale, factor), or kWgrad's ring of slots of four
+  // steps; then the ring of stages, whose addresses are formed by XOR below 1 KiB.
+  static constexpr int TABLE = (12 * TM + 1023) / 1024 * 1024;
+  static constexpr int LDS_BYTES = TABLE + KS * STAGE;
+  static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && (LDS_BYTES + 1024) * WGS <= 160 * 1024 && TABLE >= 1024, "tile");
   static_assert(VM * (KS - 1) < 64, "vmcnt immediate");
 };
 
@@ -139,68 +140,25 @@ MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
   return true;
 }
 
-template <class OP, bool FP16, int FORM, class T>
-__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::WPE, T::WPE))) void tile_mm_kernel(MmArgs g) {
+// One tile: rows [i0, i0 + nvalid) of the output, or the nvalid slots of the
+// table, by columns j0 on, over `length` of the contraction.  K: the tile of the
+// launch, which T is or is shorter than.
+template <class OP, bool FP16, int FORM, class K, class T>
+MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int e, int nvalid,
+                        int64_t length) {
   constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS;
   constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
   constexpr int STEP = 128 / EB;  // contraction elements of a step
   static_assert(EB == 2 || FORM == kProduct, "transposing reads are of 16-bit values");
-  static_assert(FORM != kWgrad || KS == 2, "the ring of slots is for two stages");
-  // the fragments' addresses are formed by XOR below 1 KiB
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
-  int32_t* smSlot = reinterpret_cast<int32_t*>(smem + T::OFF_SLOT);
-  float* smSa = reinterpret_cast<float*>(smem + T::OFF_SLOT + 4 * TM);
-  float* smW = reinterpret_cast<float*>(smem + T::OFF_SLOT + 8 * TM);
+  static_assert(FORM != kWgrad || (KS == 2 && TM == TN), "the ring of slots is for two stages");
+  static_assert(T::THREADS == K::THREADS && T::LDS_BYTES <= K::LDS_BYTES && T::TABLE <= K::TABLE, "a part of the launch's tile");
+  const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
+  const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
+  const float* smW = reinterpret_cast<const float*>(smem) + 2 * K::TM;
+  uint8_t* const ring = smem + K::TABLE;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)ring;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  // ---- which tile ----
-  int64_t pos0, j0, i0 = 0, length;
-  int rows, e = 0, nvalid;
-  if constexpr (FORM == kWgrad) {
-    const int64_t nt = (g.Cn + TM - 1) / TM;
-    const int64_t per_e = nt * g.n_jt;
-    const int64_t total = per_e * g.E, per = (total + 7) / 8;
-    const int64_t t = (int64_t)(blockIdx.x % 8) * per + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= per || t >= total) return;
-    e = (int)(t / per_e);
-    i0 = t % per_e / g.n_jt * TM;
-    j0 = t % g.n_jt * TN;
-    rows = nvalid = (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM);
-    const Run r = run_of(g, e);
-    pos0 = r.pos0;
-    length = r.count;
-  } else {
-    int64_t b, j;
-    if (!rows_tile(g, b, j)) return;
-    j0 = j * TN;
-    pos0 = b * TM;
-    rows = TM;
-    if (g.eids) e = g.eids[b];
-    else if (pos0 + rows > g.S) rows = (int)(g.S - pos0);
-    length = g.Cn;
-    // the slots, their scales and factors, for the epilogue and the rows' addresses
-    bool valid = false;
-    static_assert(TM <= T::THREADS, "a thread a row");
-    if (tid < TM) {
-      const uint32_t slot = tid >= rows ? (uint32_t)g.S : g.sorted ? (uint32_t)g.sorted[pos0 + tid] : (uint32_t)(pos0 + tid);
-      valid = slot < g.S;
-      smSlot[tid] = valid ? (int)slot : -1;
-      if constexpr (EB == 1) smSa[tid] = valid ? g.As[g.a_by_pos ? pos0 + tid : (int)slot / g.top_k] : 0.0f;
-      smW[tid] = valid && g.topk_w ? g.topk_w[slot] : 1.0f;
-    }
-    nvalid = __syncthreads_count(valid);
-    if (nvalid == 0) return;
-  }
-  if (e < 0 || e >= g.E) {  // no expert: zero rows
-    for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
-      const int64_t j = j0 + c % (TN / 8) * 8;
-      if (j < g.J)
-        *reinterpret_cast<v4i*>(g.C + ((int64_t)smSlot[c / (TN / 8)] * g.ldc + j) * 2) = (v4i){0, 0, 0, 0};
-    }
-    return;
-  }
   const int KB = (int)((length + STEP - 1) / STEP);
 
   // ---- addresses of this lane's part of the loads ----
@@ -223,7 +181,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     } else {
       const int row = 8 * gi + (lane >> 3);
       const int slot = gi < T::NA ? smSlot[row] : -1;
-      const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + row : slot / g.top_k;
+      const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot);
       a_ptr[i] = g.A + ar * g.lda * EB + row_chunk(gi) * 16;
     }
   }
@@ -242,6 +200,14 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
   const int a_rows = KS == 2 ? (nvalid + 15) / 16 * 16 : TM;
 
+  // kWgrad: the slots of this lane's rows of a step, read ahead of its loads
+  uint32_t slot_r[T::NA_W];
+  auto read_slots = [&](int kk) {
+#pragma unroll
+    for (int i = 0; i < T::NA_W; ++i)
+      slot_r[i] = (uint32_t)smSlot[(kk & 3) * 64 + col_row(wave + T::NW * i, ACPR)];
+  };
+
   // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
   // partial run of the contraction, so that no other step has to look for its
   // end; the addresses of the others advance from load to load.
@@ -257,12 +223,10 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     constexpr int i = is_b ? d : d - T::NB_W;
     const int gi = wave + T::NW * i;
     if constexpr (FORM == kWgrad) {
-      const int r = col_row(gi, is_b ? BCPR : ACPR);
-      const uint32_t slot = (uint32_t)reinterpret_cast<const int32_t*>(smem + T::OFF_IDS)[(kk & 3) * 64 + r];
       const uint8_t* p;
-      if constexpr (is_b) p = b_ptr[i] + (int64_t)(slot / (uint32_t)g.top_k) * g.sbc * EB;
-      else p = a_ptr[i] + (int64_t)slot * g.lda * EB;
-      p = r < left ? p : zeros;
+      if constexpr (is_b) p = b_ptr[i] + (uint64_t)slot_row(g, slot_r[i]) * (uint32_t)(g.sbc * EB);
+      else p = a_ptr[i] + (uint64_t)slot_r[i] * (uint32_t)(g.lda * EB);
+      if constexpr (first) p = col_row(gi, is_b ? BCPR : ACPR) < left ? p : zeros;
       if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
         lds_load16(p, dst + (is_b ? T::A_BYTES : 0) + gi * 1024);
     } else if constexpr (is_b) {
@@ -297,7 +261,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     if (wave == T::NW - 1 && kk < KB) {
       const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
       const int64_t c = c0 + lane < length ? c0 + lane : length - 1;
-      lds_load4(g.sorted + pos0 + c, lds0 + T::OFF_IDS + (kk & 3) * 256);
+      lds_load4(g.sorted + pos0 + c, (uint32_t)(uintptr_t)(lds_ptr)smem + (kk & 3) * 256);
     }
   };
 
@@ -327,10 +291,13 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   }
   const std::integral_constant<int, 0> none;
   const std::integral_constant<int, ND> all;
+  if constexpr (FORM == kWgrad) read_slots(0);
   if (KB > 0) loads(0, 0, none, all, std::true_type{});
 #pragma unroll
-  for (int s = 1; s < KS; ++s)
+  for (int s = 1; s < KS; ++s) {
+    if constexpr (FORM == kWgrad) read_slots(s);
     if (s < KB) loads(s, s, none, all, std::false_type{});
+  }
 
   // A step is 2 CS slots of RS matrix instructions, one weight fragment each, which
   // is read two slots ahead.  The barrier that hands over the next stage stands two
@@ -379,8 +346,12 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
               read_b(next, 0);
               read_b(next, 1);
             }
-            if constexpr (FORM == kWgrad)
-              if (kk + KS < KB) issue_ids(kk + KS + 1);
+            if constexpr (FORM == kWgrad) {
+              if (kk + KS < KB) {
+                read_slots(kk + KS);
+                issue_ids(kk + KS + 1);
+              }
+            }
           }
         }
         if constexpr (RA > 0 && Q < NQ - 2) {
@@ -428,7 +399,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   mm_barrier();
 
   // ---- epilogue: rows of 16-bit outputs through LDS, chunks XOR the row ----
-  uint16_t* out = reinterpret_cast<uint16_t*>(smem);
+  uint16_t* out = reinterpret_cast<uint16_t*>(ring);
   constexpr int CH = TN / 8;
 #pragma unroll
   for (int c = 0; c < T::CS; ++c) {
@@ -463,6 +434,66 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     const int64_t orow = FORM == kWgrad ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
     *reinterpret_cast<v4i*>(g.C + (orow * g.ldc + j) * 2) =
         *reinterpret_cast<const v4i*>(out + row * TN + ((cc ^ (row & 15)) << 3));
+  }
+}
+
+template <class OP, bool FP16, int FORM, class T>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::WPE, T::WPE))) void tile_mm_kernel(MmArgs g) {
+  constexpr int TM = T::TM, TN = T::TN;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x;
+  if constexpr (FORM == kWgrad) {
+    // Each XCD takes a contiguous range of the experts' tiles, in groups of four
+    // row tiles with all column tiles: about as many rows of tiles as columns run
+    // at once on one L2.
+    constexpr int kGroup = 4;
+    const int64_t nt = (g.Cn + TM - 1) / TM, per_e = nt * g.n_jt;
+    const int64_t total = per_e * g.E, per = (total + 7) / 8;
+    const int64_t t = (int64_t)(blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= per || t >= total) return;
+    const int e = (int)(t / per_e);
+    const int64_t in = t % per_e, ig = in / (kGroup * g.n_jt) * kGroup;
+    const int64_t w = nt - ig < kGroup ? nt - ig : kGroup, at = in - ig * g.n_jt;
+    const int64_t i0 = (ig + at % w) * TM, j0 = at / w * TN;
+    const Run r = run_of(g, e);
+    mm_tile<OP, FP16, FORM, T, T>(g, smem, r.pos0, i0, j0, e, (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM), r.count);
+  } else {
+    int64_t b, j;
+    if (!rows_tile(g, b, j)) return;
+    const int64_t j0 = j * TN, pos0 = b * TM;
+    const int rows = !g.eids && pos0 + TM > g.S ? (int)(g.S - pos0) : TM;
+    const int e = g.eids ? g.eids[b] : 0;
+    // the rows' slots, their scales and factors, for their addresses and the results
+    int32_t* smSlot = reinterpret_cast<int32_t*>(smem);
+    bool valid = false;
+    static_assert(TM <= T::THREADS, "a thread a row");
+    if (tid < TM) {
+      const uint32_t slot = tid >= rows ? (uint32_t)g.S : g.sorted ? (uint32_t)g.sorted[pos0 + tid] : (uint32_t)(pos0 + tid);
+      valid = slot < g.S;
+      smSlot[tid] = valid ? (int)slot : -1;
+      if constexpr (OP::BYTES == 1) {
+        reinterpret_cast<float*>(smSlot)[TM + tid] = valid ? g.As[g.a_by_pos ? pos0 + tid : slot_row(g, slot)] : 0.0f;
+        reinterpret_cast<float*>(smSlot)[2 * TM + tid] = valid && g.topk_w ? g.topk_w[slot] : 1.0f;
+      }
+    }
+    const int nvalid = __syncthreads_count(valid);
+    if (nvalid == 0) return;
+    if (e < 0 || e >= g.E) {  // no expert: zero rows
+      for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
+        const int64_t jj = j0 + c % (TN / 8) * 8;
+        if (jj < g.J)
+          *reinterpret_cast<v4i*>(g.C + ((int64_t)smSlot[c / (TN / 8)] * g.ldc + jj) * 2) = (v4i){0, 0, 0, 0};
+      }
+      return;
+    }
+    // An expert's last rows: a tile that they fill, whose ring is deeper.
+    if constexpr (TM == 256 && TN == 256) {
+      if (nvalid <= 64) {
+        mm_tile<OP, FP16, FORM, T, MmTile<64, 256, 8, 1, 3, 1>>(g, smem, pos0, 0, j0, e, nvalid, g.Cn);
+        return;
+      }
+    }
+    mm_tile<OP, FP16, FORM, T, T>(g, smem, pos0, 0, j0, e, nvalid, g.Cn);
   }
 }
 
