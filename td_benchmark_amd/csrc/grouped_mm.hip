@@ -162,21 +162,64 @@ static int launch_tile(MmArgs g, hipStream_t st) {
   if (attr != hipSuccess) return kErrLaunch;
   g.n_jt = (g.J + T::TN - 1) / T::TN;
   const int64_t tiles = (FORM == kWgrad ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt;
-  const int64_t grid = (tiles + 7) / 8 * 8;
+  const int64_t deal = FORM == kWgrad ? 8 * kWgradChunk : 8, grid = (tiles + deal - 1) / deal * deal;
   if (grid > 0x7FFFFFFF) return kErrBadShape;
   hipLaunchKernelGGL((tile_mm_kernel<OP, FP16, FORM, T>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
+// The rows form by the align block's rows.  The 256 columns of a wide tile cost
+// the fewest loads, narrower ones give more tiles where there are few: `rounds`
+// weighs the rounds that a width's tiles take on 256 CUs with what one of them
+// costs (a tile of 128 columns about 0.65 and of 64 about 0.5 of one of 256, which
+// measured 118 / 74 / 68 us at 8 experts of 128 rows, 4096 x 2048).  Up to 32 rows
+// the product only streams its weights, which 64 columns and two workgroups a CU
+// with deep rings do best at every count (4 rows an expert of 128: 189 us against
+// 197; one token: 24 against 37); its gradient by rows reads them transposed and
+// stays with wide tiles where they fill the chip (183 against 187, 9 rows of 8
+// experts 221 against 241).
+static double rounds(double blocks, int64_t J, int TN, double cost) {
+  const double r = blocks * (double)((J + TN - 1) / TN) / 256.0;
+  return cost * (r < 1.0 ? 1.0 : (double)(int64_t)(r + 0.999));
+}
+
+// The blocks that hold slots, as far as the host knows: near one an expert where
+// they are short, and half a block over where they are long.
+static double live_blocks_guess(const MmArgs& g) {
+  if (!g.eids) return (double)g.n_blocks;
+  const double used = g.S < g.E ? (double)g.S : (double)g.E;
+  const double b = 2.0 * g.S <= used * g.bm ? used : (double)g.S / g.bm + 0.5 * used;
+  return b < (double)g.n_blocks ? b : (double)g.n_blocks;
+}
+
 template <class OP, bool FP16, int FORM>
 static int launch_rows(const MmArgs& g, hipStream_t st) {
-  switch (g.bm) {
-    case 16: return launch_tile<OP, FP16, FORM, MmTile<16, 256, 8, 1, 3, 1>>(g, st);
-    case 32: return launch_tile<OP, FP16, FORM, MmTile<32, 256, 8, 1, 3, 1>>(g, st);
-    case 64: return launch_tile<OP, FP16, FORM, MmTile<64, 256, 8, 1, 3, 1>>(g, st);
-    case 128: return launch_tile<OP, FP16, FORM, MmTile<128, 256, 8, 2, 3, 1>>(g, st);
-    default: return launch_tile<OP, FP16, FORM, MmTile<256, 256, 8, 4, 2, 1>>(g, st);
+  const double blocks = live_blocks_guess(g);
+  const double wide = rounds(blocks, g.J, 256, 1.0), half = rounds(blocks, g.J, 128, 0.65),
+               slim = rounds(blocks, g.J, 64, 0.5);
+  if (g.bm <= 32) {
+    const bool stream = FORM == kProduct || wide <= 1.0;
+    if (g.bm == 16)
+      return stream ? launch_tile<OP, FP16, FORM, MmTile<16, 64, 2, 1, 4, 2>>(g, st)
+                    : launch_tile<OP, FP16, FORM, MmTile<16, 256, 8, 1, 3, 1>>(g, st);
+    return stream ? launch_tile<OP, FP16, FORM, MmTile<32, 64, 4, 2, 6, 2>>(g, st)
+                  : launch_tile<OP, FP16, FORM, MmTile<32, 256, 8, 1, 3, 1>>(g, st);
   }
+  if (g.bm == 64) {
+    if (FORM == kProduct || half < wide) {
+      if (slim < half) return launch_tile<OP, FP16, FORM, MmTile<64, 64, 4, 2, 4, 2>>(g, st);
+      return launch_tile<OP, FP16, FORM, MmTile<64, 128, 4, 1, 3, 2>>(g, st);
+    }
+    return launch_tile<OP, FP16, FORM, MmTile<64, 256, 8, 2, 3, 1>>(g, st);
+  }
+  if (g.bm == 128) {
+    if (slim < half && slim < wide) return launch_tile<OP, FP16, FORM, MmTile<128, 64, 8, 4, 3, 2>>(g, st);
+    if (half < wide) return launch_tile<OP, FP16, FORM, MmTile<128, 128, 8, 4, 4, 1>>(g, st);
+    return launch_tile<OP, FP16, FORM, MmTile<128, 256, 8, 2, 3, 1>>(g, st);
+  }
+  if (slim < half && slim < wide) return launch_tile<OP, FP16, FORM, MmTile<256, 64, 8, 4, 3, 1>>(g, st);
+  if (half < wide) return launch_tile<OP, FP16, FORM, MmTile<256, 128, 8, 4, 3, 1>>(g, st);
+  return launch_tile<OP, FP16, FORM, MmTile<256, 256, 8, 4, 2, 1>>(g, st);
 }
 
 static bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }

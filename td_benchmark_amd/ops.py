@@ -10,6 +10,7 @@ there is no torch compute and no fallback on the path.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Any
 
 import torch
@@ -1303,15 +1304,23 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
 
 
-def _need_here(*named: tuple[str, torch.Tensor | None]) -> None:
+def _current_device() -> int:
+    return _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+
+
+def _need_here(**named: torch.Tensor | None) -> None:
     """The tensors are on the current device, whose current stream the launch
     goes to: a pointer of another device would be read through the wrong one."""
-    for name, t in named:
-        if t is not None and not t.is_cuda:
+    here = None
+    for name, t in named.items():
+        if t is None:
+            continue
+        at = t.get_device()  # -1: not a GPU tensor
+        if at < 0:
             raise ValueError(f"{name} must be a GPU tensor")
-    here = torch.cuda.current_device()
-    for name, t in named:
-        if t is not None and t.device.index != here:
+        if here is None:
+            here = _current_device()
+        if at != here:
             raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
 
 
@@ -1352,22 +1361,48 @@ class ExpertSlots:
         self.block_size_m = block_size_m or slots_block_m(self.S, self.E)
         if self.block_size_m not in SUPPORTED_BLOCK_M:
             raise ValueError(f"block_size_m must be one of {SUPPORTED_BLOCK_M}")
-        _need_here(("topk_ids", topk_ids))
+        _need_here(topk_ids=topk_ids)
         self.device = topk_ids.device
         # slot ids, sorted ids, block experts, the positions' count and align's workspace in one allocation
-        self.max_padded = align_max_padded(self.S, self.E + 1, self.block_size_m)
-        blocks = (self.max_padded + self.block_size_m - 1) // self.block_size_m
-        work = align_workspace_bytes(self.S, self.E + 1)
-        sizes = [max(n + 3, 4) // 4 * 4 for n in (self.S, self.max_padded, blocks, 1, (work + 3) // 4)]
-        buf = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
-        self._slot_ids, sorted_ids, expert_ids, ntpp, workspace = buf.split(sizes)
-        self.sorted_ids, self.expert_ids = sorted_ids[: max(self.max_padded, 1)], expert_ids[: max(blocks, 1)]
-        self.ntpp = ntpp[:1]
+        self.max_padded, blocks, self._sizes = _slots_layout(self.S, self.E, self.block_size_m)
+        self._buf = torch.empty(sum(self._sizes), dtype=torch.int32, device=self.device)
         ids = topk_ids.contiguous()
-        check(lib().moe_expert_slots(_ptr(ids), ids.element_size(), self.S, self.E, self.block_size_m,
-                                     _ptr(self._slot_ids), _ptr(self.sorted_ids), _ptr(self.expert_ids),
-                                     _ptr(self.ntpp), self.max_padded, _ptr(workspace), _stream()),
-              "moe_expert_slots")
+        at = self._buf.data_ptr()
+        at_sorted = at + 4 * self._sizes[0]
+        at_eids = at_sorted + 4 * self._sizes[1]
+        at_ntpp = at_eids + 4 * self._sizes[2]
+        self._at = (at_sorted, at_eids, at_ntpp)
+        check(lib().moe_expert_slots(ids.data_ptr(), ids.element_size(), self.S, self.E, self.block_size_m, at,
+                                     at_sorted, at_eids, at_ntpp, self.max_padded, at_ntpp + 4 * self._sizes[3],
+                                     _stream_handle()), "moe_expert_slots")
+
+    def _part(self, i: int, n: int) -> torch.Tensor:
+        start = sum(self._sizes[:i])
+        return self._buf[start:start + max(n, 1)]
+
+    @property
+    def sorted_ids(self) -> torch.Tensor:
+        """The slots in expert order with padding, as moe_align_block_size gives them."""
+        return self._part(1, self.max_padded)
+
+    @property
+    def expert_ids(self) -> torch.Tensor:
+        """The expert of each block; num_experts for the slots without one."""
+        return self._part(2, (self.max_padded + self.block_size_m - 1) // self.block_size_m)
+
+    @property
+    def ntpp(self) -> torch.Tensor:
+        """[1]: the sorted positions in use."""
+        return self._part(3, 1)
+
+
+@functools.lru_cache(maxsize=256)
+def _slots_layout(S: int, E: int, block_m: int) -> tuple[int, int, tuple[int, ...]]:
+    """-> sorted positions, blocks, and the int32 words of ExpertSlots' parts (whole 16 bytes each)."""
+    mp = align_max_padded(S, E + 1, block_m)
+    blocks = (mp + block_m - 1) // block_m
+    work = align_workspace_bytes(S, E + 1)
+    return mp, blocks, tuple(max(n + 3, 4) // 4 * 4 for n in (S, mp, blocks, 1, (work + 3) // 4))
 
 
 def slots_block_m(num_slots: int, num_experts: int) -> int:
@@ -1393,8 +1428,7 @@ def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> i
         raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
     if not w.is_contiguous():
         raise ValueError("w must be contiguous")
-    _need_here(("x", x), ("w", w), ("slots", slots.sorted_ids))
-    _row_stride(x, "x")
+    _need_here(x=x, w=w, slots=slots._buf)
     return 1 if x.shape[0] == slots.S else slots.top_k
 
 
@@ -1402,10 +1436,33 @@ def _grouped_product(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> to
     k = _grouped_operands(x, w, slots)
     E, N, K = w.shape
     y = torch.empty((slots.S, N), dtype=x.dtype, device=x.device)
-    check(lib().moe_grouped_mm(_ptr(x), _row_stride(x, "x"), _ptr(w), _ptr(slots.sorted_ids), _ptr(slots.expert_ids),
-                               _ptr(slots.ntpp), slots.S, k, N, K, E, slots.block_size_m, slots.max_padded,
-                               _DTYPE_CODE[x.dtype], _ptr(y), _stream()), "moe_grouped_mm")
+    check(lib().moe_grouped_mm(x.data_ptr(), _row_stride(x, "x"), w.data_ptr(), *slots._at, slots.S, k, N, K, E,
+                               slots.block_size_m, slots.max_padded, _DTYPE_CODE[x.dtype], y.data_ptr(),
+                               _stream_handle()), "moe_grouped_mm")
     return y
+
+
+def _dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool) -> torch.Tensor:
+    E, N, K = w.shape
+    dtype, stream = _DTYPE_CODE[dy.dtype], _stream_handle()
+    dx = torch.empty((slots.S, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_grouped_mm_dgrad(dy.data_ptr(), w.data_ptr(), *slots._at, slots.S, N, K, E, slots.block_size_m,
+                                     slots.max_padded, dtype, dx.data_ptr(), stream), "moe_grouped_mm_dgrad")
+    if not by_token or slots.top_k == 1:
+        return dx
+    out = torch.empty((slots.T, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_slot_sum(dx.data_ptr(), slots.T, slots.top_k, K, dtype, out.data_ptr(), stream), "moe_slot_sum")
+    return out
+
+
+def _wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
+    N, K = dy.shape[1], x.shape[1]
+    dw = torch.empty((slots.E, N, K), dtype=dy.dtype, device=dy.device)
+    check(lib().moe_grouped_mm_wgrad(dy.data_ptr(), x.data_ptr(), _row_stride(x, "x"), *slots._at, slots.S,
+                                     1 if x.shape[0] == slots.S else slots.top_k, N, K, slots.E, slots.block_size_m,
+                                     slots.max_padded, _DTYPE_CODE[dy.dtype], dw.data_ptr(), _stream_handle()),
+          "moe_grouped_mm_wgrad")
+    return dw
 
 
 def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool = False) -> torch.Tensor:
@@ -1421,17 +1478,8 @@ def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_t
         raise ValueError(f"w has {E} experts, the slots {slots.E}")
     _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
     _need(w, "w", dy.dtype, anywhere=True)
-    _need_here(("dy", dy), ("w", w), ("slots", slots.sorted_ids))
-    dx = torch.empty((slots.S, K), dtype=dy.dtype, device=dy.device)
-    check(lib().moe_grouped_mm_dgrad(_ptr(dy), _ptr(w), _ptr(slots.sorted_ids), _ptr(slots.expert_ids),
-                                     _ptr(slots.ntpp), slots.S, N, K, E, slots.block_size_m, slots.max_padded,
-                                     _DTYPE_CODE[dy.dtype], _ptr(dx), _stream()), "moe_grouped_mm_dgrad")
-    if not by_token or slots.top_k == 1:
-        return dx
-    out = torch.empty((slots.T, K), dtype=dy.dtype, device=dy.device)
-    check(lib().moe_slot_sum(_ptr(dx), slots.T, slots.top_k, K, _DTYPE_CODE[dy.dtype], _ptr(out), _stream()),
-          "moe_slot_sum")
-    return out
+    _need_here(dy=dy, w=w, slots=slots._buf)
+    return _dgrad(dy, w, slots, by_token)
 
 
 def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
@@ -1449,14 +1497,8 @@ def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> t
     _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
     if x.shape[0] not in (slots.T, slots.S):
         raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
-    _need_here(("dy", dy), ("x", x), ("slots", slots.sorted_ids))
-    dw = torch.empty((slots.E, N, K), dtype=dy.dtype, device=dy.device)
-    check(lib().moe_grouped_mm_wgrad(_ptr(dy), _ptr(x), _row_stride(x, "x"), _ptr(slots.sorted_ids),
-                                     _ptr(slots.expert_ids), _ptr(slots.ntpp), slots.S,
-                                     1 if x.shape[0] == slots.S else slots.top_k, N, K, slots.E, slots.block_size_m,
-                                     slots.max_padded, _DTYPE_CODE[dy.dtype], _ptr(dw), _stream()),
-          "moe_grouped_mm_wgrad")
-    return dw
+    _need_here(dy=dy, x=x, slots=slots._buf)
+    return _wgrad(dy, x, slots)
 
 
 class _GroupedMM(torch.autograd.Function):
@@ -1475,9 +1517,9 @@ class _GroupedMM(torch.autograd.Function):
         dy = dy.contiguous()  # a sum's gradient comes with stride 0
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = grouped_mm_dgrad(dy, w, slots, by_token=x.shape[0] != slots.S)
+            dx = _dgrad(dy, w, slots, x.shape[0] != slots.S)
         if ctx.needs_input_grad[1]:
-            dw = grouped_mm_wgrad(dy, x, slots)
+            dw = _wgrad(dy, x, slots)
         return dx, dw, None
 
 
@@ -1512,14 +1554,16 @@ def per_token_quant_int8(x: torch.Tensor, out_q: torch.Tensor | None = None,
         raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
     if x.dtype not in _DTYPE_CODE:
         raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _need_here(("x", x), ("out_q", out_q), ("out_s", out_s))
+    _need_here(x=x, out_q=out_q, out_s=out_s)
     T, H = x.shape
     q = torch.empty((T, H), dtype=torch.int8, device=x.device) if out_q is None else out_q
     s = torch.empty((T, 1), dtype=torch.float32, device=x.device) if out_s is None else out_s
-    _need(q, "out_q", torch.int8, (T, H), anywhere=True)
-    _need(s, "out_s", torch.float32, (T, 1), anywhere=True)
-    check(lib().moe_quant_int8(_ptr(x), _row_stride(x, "x"), T, H, _DTYPE_CODE[x.dtype], _ptr(q), _ptr(s), _stream()),
-          "moe_quant_int8")
+    if out_q is not None:
+        _need(q, "out_q", torch.int8, (T, H), anywhere=True)
+    if out_s is not None:
+        _need(s, "out_s", torch.float32, (T, 1), anywhere=True)
+    check(lib().moe_quant_int8(x.data_ptr(), _row_stride(x, "x"), T, H, _DTYPE_CODE[x.dtype], q.data_ptr(),
+                               s.data_ptr(), _stream_handle()), "moe_quant_int8")
     return q, s
 
 
@@ -1557,10 +1601,11 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
     elif tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
-    _need_here(("a", a), ("b", b), ("a_scale", a_scale), ("b_scale", b_scale), ("bias", bias), ("out", out))
-    check(lib().moe_int8_scaled_mm(_ptr(a), _row_stride(a, "a"), _ptr(a_scale), _ptr(b), _row_stride(b, "b"),
-                                   _ptr(b_scale), _ptr(bias), M, N, K, _DTYPE_CODE[out_dtype], _ptr(out),
-                                   _row_stride(out, "out"), _stream()), "moe_int8_scaled_mm")
+    _need_here(a=a, b=b, a_scale=a_scale, b_scale=b_scale, bias=bias, out=out)
+    check(lib().moe_int8_scaled_mm(a.data_ptr(), _row_stride(a, "a"), a_scale.data_ptr(), b.data_ptr(),
+                                   _row_stride(b, "b"), b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                                   M, N, K, _DTYPE_CODE[out_dtype], out.data_ptr(), _row_stride(out, "out"),
+                                   _stream_handle()), "moe_int8_scaled_mm")
     return out
 
 
@@ -1608,9 +1653,7 @@ def _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_i
         _need(w, "topk_weights", torch.float32, anywhere=True)
         if w.numel() < S:
             raise ValueError(f"topk_weights has {w.numel()} entries for {S} slots")
-    _need_here(("A", A), ("B", B), ("C", C), ("A_scale", A_scale), ("B_scale", B_scale), ("topk_weights", w),
-               ("sorted_token_ids", sorted_token_ids), ("expert_ids", expert_ids),
-               ("num_tokens_post_padded", num_tokens_post_padded))
+    _need_here(A=A, B=B, C=C, A_scale=A_scale, B_scale=B_scale, topk_weights=w, sorted_token_ids=sorted_token_ids, expert_ids=expert_ids, num_tokens_post_padded=num_tokens_post_padded)
     check(lib().moe_grouped_gemm_int8(_ptr(A), _ptr(A_scale), _ptr(B), _ptr(B_scale), _ptr(sorted_token_ids),
                                       _ptr(expert_ids), _ptr(num_tokens_post_padded), _ptr(w), S, top_k,
                                       1 if a_by_pos else 0, N, K, E, BM, sorted_token_ids.numel(),

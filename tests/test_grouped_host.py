@@ -23,7 +23,7 @@ def L():
 class FakeSlots:
     """What the checks read of ExpertSlots, without a GPU."""
     T, top_k, S, E, block_size_m, max_padded = 4, 2, 8, 3, 16, 48
-    sorted_ids = torch.zeros(48, dtype=torch.int32)
+    sorted_ids = _buf = torch.zeros(48, dtype=torch.int32)
 
 
 def test_slots_refuse():
