@@ -122,22 +122,18 @@ MOE_DEVICE int64_t live_blocks(const MmArgs& g) {
   return n < 0 ? 0 : (n < g.n_blocks ? n : g.n_blocks);
 }
 
-// The first of n ascending words that is at least v: 64 probes a round by the
-// lanes of the calling wave.
-MOE_DEVICE int64_t lower_bound(const int32_t* a, int64_t n, int32_t v) {
+// One round of a search in ascending words by the calling wave: [lo, hi] holds the
+// place of the first word that is at least v; 64 probes narrow it to a 64th.
+MOE_DEVICE void narrow(const int32_t* a, int32_t v, int64_t& lo, int64_t& hi) {
   const int lane = threadIdx.x & 63;
-  int64_t lo = 0, hi = n;  // the answer is in [lo, hi]
-  while (lo < hi) {
-    const int64_t step = (hi - lo + 63) / 64;
-    const int64_t i = lo + step * (lane + 1) - 1;  // the lane's probe: the last of its step words
-    const uint64_t ge = __ballot(i >= hi || a[i < hi ? i : hi - 1] >= v);
-    // words before the first lane's run that reaches v are all smaller
-    const int first = ge ? __ffsll((unsigned long long)ge) - 1 : 64;
-    const int64_t nlo = lo + step * first, nhi = nlo + step - 1;
-    lo = nlo < hi ? nlo : hi;
-    hi = nhi < hi ? nhi : hi;
-  }
-  return lo;
+  const int64_t step = (hi - lo + 63) / 64;
+  const int64_t i = lo + step * (lane + 1) - 1;  // the lane's probe: the last of its step words
+  const uint64_t ge = __ballot(i >= hi || a[i < hi ? i : hi - 1] >= v);
+  // words before the first lane's run that reaches v are all smaller
+  const int first = ge ? __ffsll((unsigned long long)ge) - 1 : 64;
+  const int64_t nlo = lo + step * first, nhi = nlo + step - 1;
+  lo = nlo < hi ? nlo : hi;
+  hi = nhi < hi ? nhi : hi;
 }
 
 // Positions [pos0, pos0 + count) of the slots of expert e: its blocks are
@@ -147,14 +143,21 @@ struct Run {
 };
 MOE_DEVICE Run run_of(const MmArgs& g, int e) {
   const int64_t nb = live_blocks(g);
-  const int64_t b0 = lower_bound(g.eids, nb, e), b1 = lower_bound(g.eids + b0, nb - b0, e + 1) + b0;
+  int64_t b0 = 0, h0 = nb, b1 = 0, h1 = nb;
+  while (b0 < h0 || b1 < h1) {  // both ends in the same rounds: two up to 4096 blocks
+    if (b0 < h0) narrow(g.eids, e, b0, h0);
+    if (b1 < h1) narrow(g.eids, e + 1, b1, h1);
+  }
   Run r = {b0 * g.bm, 0};
-  if (b1 == b0) return r;
+  if (b1 <= b0) return r;
   const int lane = threadIdx.x & 63;
-  int64_t last = 0;  // slots of the last block
-  for (int p = 0; p < g.bm; p += 64)
-    last += __popcll(__ballot(p + lane < g.bm && (uint32_t)g.sorted[(b1 - 1) * g.bm + p + lane] < g.S));
-  r.count = (b1 - b0 - 1) * g.bm + last;
+  const int32_t* tail = g.sorted + (b1 - 1) * g.bm;
+  uint32_t slot[4];  // blocks have up to 256 positions
+#pragma unroll
+  for (int i = 0; i < 4; ++i) slot[i] = 64 * i + lane < g.bm ? (uint32_t)tail[64 * i + lane] : 0xFFFFFFFFu;
+  r.count = (b1 - b0 - 1) * g.bm;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.count += __popcll(__ballot((int64_t)slot[i] < g.S));
   return r;
 }
 

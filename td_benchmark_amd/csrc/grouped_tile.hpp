@@ -40,9 +40,10 @@ struct MmTile {
   static constexpr int NA_W = (NA + NW - 1) / NW, NB_W = (NB + NW - 1) / NW;
   // loads of a stage that every wave issues at least: what may stay in flight of each younger stage
   static constexpr int VM = NA / NW + NB / NW;
-  // LDS: the rows' table (slot, scale, factor), or kWgrad's ring of slots of four
-  // steps; then the ring of stages, whose addresses are formed by XOR below 1 KiB.
-  static constexpr int TABLE = (12 * TM + 1023) / 1024 * 1024;
+  // LDS: the rows' table (slot, scale, factor) and the columns' (scale, bias), or
+  // kWgrad's ring of slots of four steps; then the ring of stages, whose addresses
+  // are formed by XOR below 1 KiB.
+  static constexpr int TABLE = (12 * TM + 8 * TN + 1023) / 1024 * 1024;
   static constexpr int LDS_BYTES = TABLE + KS * STAGE;
   static_assert(RS >= 1 && CS >= 1 && TM * TN * 2 <= KS * STAGE && (LDS_BYTES + 1024) * WGS <= 160 * 1024 && TABLE >= 1024, "tile");
   static_assert(VM * (KS - 1) < 64, "vmcnt immediate");
@@ -100,11 +101,17 @@ MOE_DEVICE v4i lds_frag_t(uint32_t at, int row_bytes) {
   return (v4i){(int)l[0], (int)l[1], (int)h[0], (int)h[1]};
 }
 
-// The workgroup's tile: block b and column tile j of the rows form.  Workgroups
-// are dealt to the XCDs in turn; each XCD takes a contiguous range of the tiles
-// in expert order, and within an expert the column tiles go in groups of four
-// with all its row tiles, so that the workgroups that share weights or rows run
-// together on one XCD's L2.
+// The workgroup's tile: block b and column tile j of the rows form; workgroups are
+// dealt to the XCDs in turn.
+//
+// Each XCD takes a contiguous range of the live tiles in expert order (dealt out
+// in chunks of four instead, decode through W2 takes 5 % longer and 64 rows an
+// expert of 64 12 %).  Long blocks (GROUPED): within an expert the column tiles go
+// in groups of four with all its row tiles, so that the workgroups that share
+// weights or rows run together on one XCD's L2.  Short ones stream weights that
+// nobody shares, in tiles of a few microseconds: block by block, without the
+// look-up of the expert's run.
+template <bool GROUPED>
 MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
   constexpr int kXcd = 8, kGroup = 4;
   const int64_t nb = live_blocks(g);
@@ -113,6 +120,10 @@ MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
   const int64_t t = pid % kXcd * per + pid / kXcd;
   if (pid / kXcd >= per || t >= total) return false;
   b = t / g.n_jt;
+  if constexpr (!GROUPED) {
+    j = t - b * g.n_jt;
+    return true;
+  }
   int64_t b0 = 0, n = nb;
   if (g.eids) {  // the run of blocks with b's expert
     const int lane = threadIdx.x & 63;
@@ -160,6 +171,8 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
   const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
   const float* smW = reinterpret_cast<const float*>(smem) + 2 * K::TM;
+  const float* smSb = reinterpret_cast<const float*>(smem) + 3 * K::TM;
+  const float* smBias = smSb + K::TN;
   uint8_t* const ring = smem + K::TABLE;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)ring;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -409,22 +422,13 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
 #pragma unroll
   for (int c = 0; c < T::CS; ++c) {
     const int col = col_base + c * 16 + 4 * kseg;
-    float sb[4] = {1.0f, 1.0f, 1.0f, 1.0f}, bias[4] = {};
-    if constexpr (EB == 1) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int64_t j = j0 + col + v < g.J ? j0 + col + v : g.J - 1;
-        sb[v] = g.Bs[(int64_t)e * g.J + j];
-        if (g.bias) bias[v] = from16<FP16>(g.bias[j]);
-      }
-    }
 #pragma unroll
     for (int r = 0; r < T::RS; ++r) {
       const int row = row_base + r * 16 + fr;
       float f[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        if constexpr (EB == 1) f[v] = int8_out(acc[r][c][v], smSa[row], sb[v], g.bias, bias[v], g.topk_w, smW[row]);
+        if constexpr (EB == 1) f[v] = int8_out(acc[r][c][v], smSa[row], smSb[col + v], g.bias, smBias[col + v], g.topk_w, smW[row]);
         else f[v] = acc[r][c][v];
       }
       v2u pk = {pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
@@ -467,7 +471,8 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     mm_tile<OP, FP16, FORM, T, T>(g, smem, r.pos0, i0, j0, e, (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM), r.count);
   } else {
     int64_t b, j;
-    if (!rows_tile(g, b, j)) return;
+    constexpr bool GROUPED = TM == 256;
+    if (!rows_tile<GROUPED>(g, b, j)) return;
     const int64_t j0 = j * TN, pos0 = b * TM;
     const int rows = !g.eids && pos0 + TM > g.S ? (int)(g.S - pos0) : TM;
     const int e = g.eids ? g.eids[b] : 0;
@@ -482,6 +487,14 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
       if constexpr (OP::BYTES == 1) {
         reinterpret_cast<float*>(smSlot)[TM + tid] = valid ? g.As[g.a_by_pos ? pos0 + tid : slot_row(g, slot)] : 0.0f;
         reinterpret_cast<float*>(smSlot)[2 * TM + tid] = valid && g.topk_w ? g.topk_w[slot] : 1.0f;
+      }
+    }
+    if constexpr (OP::BYTES == 1) {
+      float* cols = reinterpret_cast<float*>(smSlot) + 3 * TM;
+      for (int c = tid; c < TN; c += T::THREADS) {
+        const int64_t jj = j0 + c < g.J ? j0 + c : g.J - 1;
+        cols[c] = e >= 0 && e < g.E ? g.Bs[(int64_t)e * g.J + jj] : 0.0f;
+        cols[TN + c] = g.bias ? from16<FP16>(g.bias[jj]) : 0.0f;
       }
     }
     const int nvalid = __syncthreads_count(valid);

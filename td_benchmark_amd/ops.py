@@ -1308,25 +1308,29 @@ def _current_device() -> int:
     return _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
 
 
-def _need_here(**named: torch.Tensor | None) -> None:
-    """The tensors are on the current device, whose current stream the launch
-    goes to: a pointer of another device would be read through the wrong one."""
-    here = None
-    for name, t in named.items():
-        if t is None:
-            continue
-        at = t.get_device()  # -1: not a GPU tensor
-        if at < 0:
+def _need_here(names: str, *tensors: torch.Tensor | None) -> None:
+    """The tensors (``names`` by spaces) are on the current device, whose current
+    stream the launch goes to: a pointer of another device would be read through
+    the wrong one."""
+    here = tensors[0].get_device()  # -1: not a GPU tensor
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            here = -1
+    if here >= 0 and here == _current_device():
+        return
+    for name, t in zip(names.split(), tensors):
+        if t is not None and not t.is_cuda:
             raise ValueError(f"{name} must be a GPU tensor")
-        if here is None:
-            here = _current_device()
-        if at != here:
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
+    for name, t in zip(names.split(), tensors):
+        if t is not None and t.get_device() != _current_device():
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous."""
     rows, cols = t.shape
+    if t.is_contiguous():
+        return cols
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     if rows <= 1 or cols == 0:
@@ -1361,7 +1365,7 @@ class ExpertSlots:
         self.block_size_m = block_size_m or slots_block_m(self.S, self.E)
         if self.block_size_m not in SUPPORTED_BLOCK_M:
             raise ValueError(f"block_size_m must be one of {SUPPORTED_BLOCK_M}")
-        _need_here(topk_ids=topk_ids)
+        _need_here("topk_ids", topk_ids)
         self.device = topk_ids.device
         # slot ids, sorted ids, block experts, the positions' count and align's workspace in one allocation
         self.max_padded, blocks, self._sizes = _slots_layout(self.S, self.E, self.block_size_m)
@@ -1407,9 +1411,15 @@ def _slots_layout(S: int, E: int, block_m: int) -> tuple[int, int, tuple[int, ..
 
 def slots_block_m(num_slots: int, num_experts: int) -> int:
     """The align block size of ExpertSlots, which is the rows of a tile of the
-    grouped products, from the average slots of an expert."""
+    grouped products, from the average slots of an expert, by a sweep over 6 to
+    1024 of them (128 experts of 1536 x 2048, bf16; us of the product and of its
+    gradient by rows): 12 slots 195 and 187 with 32 rows, 205 and 187 with 64; 25:
+    204 and 208, 207 and 193; 62: 218 and 207 with 128, 232 and 223 with 64, 240
+    and 220 with 256; 100: 244 and 238 with 128, 235 and 219 with 256, but 441 and
+    450, 464 and 398 with 8 experts of 28672 x 4096 and 89 and 90, 97 and 90 with 32
+    of 1160 x 2200."""
     avg = num_slots / max(num_experts, 1)
-    return 32 if avg <= 28 else 64 if avg <= 44 else 128 if avg <= 100 else 256
+    return 32 if avg <= 20 else 64 if avg <= 44 else 128 if avg <= 100 else 256
 
 
 def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> int:
@@ -1428,7 +1438,7 @@ def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> i
         raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
     if not w.is_contiguous():
         raise ValueError("w must be contiguous")
-    _need_here(x=x, w=w, slots=slots._buf)
+    _need_here("x w slots", x, w, slots._buf)
     return 1 if x.shape[0] == slots.S else slots.top_k
 
 
@@ -1478,7 +1488,7 @@ def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_t
         raise ValueError(f"w has {E} experts, the slots {slots.E}")
     _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
     _need(w, "w", dy.dtype, anywhere=True)
-    _need_here(dy=dy, w=w, slots=slots._buf)
+    _need_here("dy w slots", dy, w, slots._buf)
     return _dgrad(dy, w, slots, by_token)
 
 
@@ -1497,7 +1507,7 @@ def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> t
     _need(dy, "dy", dy.dtype, (slots.S, N), anywhere=True)
     if x.shape[0] not in (slots.T, slots.S):
         raise ValueError(f"x has {x.shape[0]} rows, expected {slots.T} (one a token) or {slots.S} (one a slot)")
-    _need_here(dy=dy, x=x, slots=slots._buf)
+    _need_here("dy x slots", dy, x, slots._buf)
     return _wgrad(dy, x, slots)
 
 
@@ -1554,7 +1564,7 @@ def per_token_quant_int8(x: torch.Tensor, out_q: torch.Tensor | None = None,
         raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
     if x.dtype not in _DTYPE_CODE:
         raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _need_here(x=x, out_q=out_q, out_s=out_s)
+    _need_here("x out_q out_s", x, out_q, out_s)
     T, H = x.shape
     q = torch.empty((T, H), dtype=torch.int8, device=x.device) if out_q is None else out_q
     s = torch.empty((T, 1), dtype=torch.float32, device=x.device) if out_s is None else out_s
@@ -1601,7 +1611,7 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
     elif tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
-    _need_here(a=a, b=b, a_scale=a_scale, b_scale=b_scale, bias=bias, out=out)
+    _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
     check(lib().moe_int8_scaled_mm(a.data_ptr(), _row_stride(a, "a"), a_scale.data_ptr(), b.data_ptr(),
                                    _row_stride(b, "b"), b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
                                    M, N, K, _DTYPE_CODE[out_dtype], out.data_ptr(), _row_stride(out, "out"),
@@ -1653,8 +1663,10 @@ def _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_i
         _need(w, "topk_weights", torch.float32, anywhere=True)
         if w.numel() < S:
             raise ValueError(f"topk_weights has {w.numel()} entries for {S} slots")
-    _need_here(A=A, B=B, C=C, A_scale=A_scale, B_scale=B_scale, topk_weights=w, sorted_token_ids=sorted_token_ids, expert_ids=expert_ids, num_tokens_post_padded=num_tokens_post_padded)
-    check(lib().moe_grouped_gemm_int8(_ptr(A), _ptr(A_scale), _ptr(B), _ptr(B_scale), _ptr(sorted_token_ids),
-                                      _ptr(expert_ids), _ptr(num_tokens_post_padded), _ptr(w), S, top_k,
+    _need_here("A B C A_scale B_scale topk_weights sorted_token_ids expert_ids num_tokens_post_padded", A, B, C, A_scale,
+               B_scale, w, sorted_token_ids, expert_ids, num_tokens_post_padded)
+    check(lib().moe_grouped_gemm_int8(A.data_ptr(), A_scale.data_ptr(), B.data_ptr(), B_scale.data_ptr(),
+                                      sorted_token_ids.data_ptr(), expert_ids.data_ptr(),
+                                      num_tokens_post_padded.data_ptr(), None if w is None else w.data_ptr(), S, top_k,
                                       1 if a_by_pos else 0, N, K, E, BM, sorted_token_ids.numel(),
-                                      _DTYPE_CODE[C.dtype], _ptr(C), _stream()), "moe_grouped_gemm_int8")
+                                      _DTYPE_CODE[C.dtype], C.data_ptr(), _stream_handle()), "moe_grouped_gemm_int8")
