@@ -168,6 +168,109 @@ static int launch_tile(MmArgs g, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
+// ---- few rows: the weights' stream, split along the contraction ---------------
+// Sixteen columns of one block of up to 16 RT rows a workgroup.  Its waves take the
+// contraction's 128-byte chunks in turn, operands straight to registers (lane fr,
+// kseg: 32 bytes of row fr), U chunks' loads in flight each, and their sums are
+// added in wave order through LDS: several times the workgroups of the narrowest
+// staged tile, where those are too few to draw on the memory.  A CU draws 50-60
+// GB/s of data that is in no cache.
+constexpr int kFewWaves = 8;
+
+template <class OP, bool FP16, int RT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
+  constexpr int EB = OP::BYTES, TM = 16 * RT, U = 4;
+  __shared__ typename OP::Acc part[kFewWaves][RT][64];
+  __shared__ int32_t smSlot[TM];
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, kseg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t b, j;
+  if (!rows_tile<false>(g, b, j)) return;
+  const int64_t j0 = j * 16, pos0 = b * g.bm;
+  const int e = g.eids ? g.eids[b] : 0;
+  bool valid = false;
+  if (tid < TM) {
+    const uint32_t slot = g.sorted ? (uint32_t)g.sorted[pos0 + tid] : (uint32_t)(pos0 + tid);
+    valid = slot < g.S;
+    smSlot[tid] = valid ? (int)slot : -1;
+  }
+  const int nvalid = __syncthreads_count(valid);
+  if (nvalid == 0) return;
+  const bool none = e < 0 || e >= g.E;
+  const uint8_t* a_row[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int slot = smSlot[16 * r + fr];
+    const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + 16 * r + fr : (int64_t)slot_row(g, (uint32_t)slot);
+    a_row[r] = g.A + ar * g.lda * EB + kseg * 32;
+  }
+  const int64_t jb = j0 + fr < g.J ? j0 + fr : g.J - 1;
+  const uint8_t* b_row = g.B + ((int64_t)e * g.b_es + jb * g.sbj) * EB + kseg * 32;
+  typename OP::Acc acc[RT] = {};
+  const int64_t bytes = g.Cn * EB;
+  const int chunks = none ? 0 : (int)((bytes + 127) / 128);
+  auto load = [&](const uint8_t* p, int64_t at) -> v4i {  // 16 bytes at `at` + kseg * 32 of a row, zeros past its end
+    return at + kseg * 32 < bytes ? *reinterpret_cast<const v4i*>(p + at) : (v4i){0, 0, 0, 0};
+  };
+  const bool second = nvalid > 16;  // whether the second 16 rows hold slots
+  for (int c0 = wave; c0 < chunks; c0 += kFewWaves * U) {
+    v4i bf[U][2], af[U][RT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (int64_t)(c0 + u * kFewWaves) * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bf[u][h] = load(b_row, at + 16 * h);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) af[u][r][h] = r == 0 || second ? load(a_row[r], at + 16 * h) : (v4i){0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r] = OP::mfma(bf[u][h], af[u][r][h], acc[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) part[wave][r][lane] = acc[r];
+  __syncthreads();
+  // a lane's four columns of one row again, 64 lanes a 16 x 16 part
+  if (tid < RT * 64) {
+    const int l = tid & 63, r = tid / 64, row = 16 * r + (l & 15);
+    const int64_t jj = j0 + 4 * (l >> 4);
+    if (row >= nvalid || jj >= g.J) return;  // J is a multiple of 8
+    typename OP::Acc sum = part[0][r][l];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) sum = sum + part[w][r][l];
+    const int slot = smSlot[row];
+    float f[4];
+    if constexpr (EB == 1) {
+      const float sa = none ? 0.0f : g.As[g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot)];
+      const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        f[v] = none ? 0.0f
+                    : int8_out(sum[v], sa, g.Bs[(int64_t)e * g.J + jj + v], g.bias,
+                               g.bias ? from16<FP16>(g.bias[jj + v]) : 0.0f, g.topk_w, w);
+    } else {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) f[v] = sum[v];
+    }
+    const v2u pk = {pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
+    *reinterpret_cast<v2u*>(g.C + ((int64_t)slot * g.ldc + jj) * 2) = pk;
+  }
+}
+
+template <class OP, bool FP16, int RT>
+static int launch_few(MmArgs g, hipStream_t st) {
+  g.n_jt = (g.J + 15) / 16;
+  const int64_t grid = (g.n_blocks * g.n_jt + 7) / 8 * 8;
+  if (grid > 0x7FFFFFFF) return kErrBadShape;
+  hipLaunchKernelGGL((few_mm_kernel<OP, FP16, RT>), dim3((unsigned)grid), dim3(64 * kFewWaves), 0, st, g);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
 // The rows form by the align block's rows.  The 256 columns of a wide tile cost
 // the fewest loads, narrower ones give more tiles where there are few: `rounds`
 // weighs the rounds that a width's tiles take on 256 CUs with what one of them
@@ -197,6 +300,14 @@ static int launch_rows(const MmArgs& g, hipStream_t st) {
   const double blocks = live_blocks_guess(g);
   const double wide = rounds(blocks, g.J, 256, 1.0), half = rounds(blocks, g.J, 128, 0.65),
                slim = rounds(blocks, g.J, 64, 0.5);
+  // Few rows on long rows of weights: few tiles, or one or two slots a block (more
+  // rows make it draw as much of A as of the weights).  int8, one row, 7168 x 4096:
+  // 16.3 us, staged 24.5; 16 tokens on 128 experts 126 and 148; 9 slots a block of
+  // 14336 272 and 226; rows of 768 bytes 123 and 79.
+  if constexpr (FORM == kProduct) {
+    if (g.bm <= 32 && g.Cn * OP::BYTES >= 2048 && (blocks * ((g.J + 63) / 64) <= 128.0 || g.S <= 2.0 * blocks))
+      return g.bm == 16 ? launch_few<OP, FP16, 1>(g, st) : launch_few<OP, FP16, 2>(g, st);
+  }
   if (g.bm <= 32) {
     const bool stream = FORM == kProduct || wide <= 1.0;
     if (g.bm == 16)

@@ -1413,13 +1413,13 @@ def slots_block_m(num_slots: int, num_experts: int) -> int:
     """The align block size of ExpertSlots, which is the rows of a tile of the
     grouped products, from the average slots of an expert, by a sweep over 6 to
     1024 of them (128 experts of 1536 x 2048, bf16; us of the product and of its
-    gradient by rows): 12 slots 195 and 187 with 32 rows, 205 and 187 with 64; 25:
+    gradient by rows): 1 slot 126 with 16 rows, 134 with 32; 12 slots 195 and 187 with 32 rows, 205 and 187 with 64; 25:
     204 and 208, 207 and 193; 62: 218 and 207 with 128, 232 and 223 with 64, 240
     and 220 with 256; 100: 244 and 238 with 128, 235 and 219 with 256, but 441 and
     450, 464 and 398 with 8 experts of 28672 x 4096 and 89 and 90, 97 and 90 with 32
     of 1160 x 2200."""
     avg = num_slots / max(num_experts, 1)
-    return 32 if avg <= 20 else 64 if avg <= 44 else 128 if avg <= 100 else 256
+    return 16 if avg <= 4 else 32 if avg <= 20 else 64 if avg <= 44 else 128 if avg <= 100 else 256
 
 
 def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> int:
