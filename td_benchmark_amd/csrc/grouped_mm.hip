@@ -454,7 +454,11 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   hipStream_t st = (hipStream_t)stream;
   if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2) &&
       N < (1 << 30) && ldx < (1 << 30)) {
-    using T = MmTile<256, 256, 8, 4, 2, 1>;
+    // Steps of 32 slots in a ring of four: rows of a column-staged step are whole
+    // lines at any length, so the finer ring costs nothing (256 slots an expert of
+    // 128: 381 us, 403 with steps of 64 in a ring of two; 1024 of 8 even).  The rows
+    // forms lose with it, whose row-staged lines it reads in halves.
+    using T = MmTile<256, 256, 8, 4, 4, 1, 64>;
     return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
   }
   return dtype == kFp16 ? launch_any<Fp16, true, true>(g, st) : launch_any<Bf16, false, true>(g, st);

@@ -29,19 +29,21 @@ enum Form { kProduct, kDgrad, kWgrad };
 constexpr int kWgradChunk = 16;
 
 // TM x TN outputs by NW waves, WM of them along the rows, from a ring of KS
-// stages, WGS workgroups a CU.
-template <int TM_, int TN_, int NW_, int WM_, int KS_, int WGS_>
+// stages of SB bytes a row, WGS workgroups a CU.
+template <int TM_, int TN_, int NW_, int WM_, int KS_, int WGS_, int SB_ = 128>
 struct MmTile {
-  static constexpr int TM = TM_, TN = TN_, NW = NW_, WM = WM_, KS = KS_, WGS = WGS_;
+  static constexpr int TM = TM_, TN = TN_, NW = NW_, WM = WM_, KS = KS_, WGS = WGS_, SB = SB_;
+  static constexpr int H = SB / 64;  // matrix instructions along the contraction in a step
+  static_assert(SB == 64 || SB == 128, "one or two instructions");
   static constexpr int THREADS = 64 * NW, WN = NW / WM, WPE = NW * WGS < 4 ? 1 : NW * WGS / 4;
   static constexpr int RS = TM / WM / 16, CS = TN / WN / 16;  // 16-row and 16-column subtiles of a wave
-  static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int NA = TM / 8, NB = TN / 8;              // 1 KiB loads of a stage
+  static constexpr int A_BYTES = TM * SB, B_BYTES = TN * SB, STAGE = A_BYTES + B_BYTES;
+  static constexpr int NA = A_BYTES / 1024, NB = B_BYTES / 1024;  // 1 KiB loads of a stage
   static constexpr int NA_W = (NA + NW - 1) / NW, NB_W = (NB + NW - 1) / NW;
   // loads of a stage that every wave issues at least: what may stay in flight of each younger stage
   static constexpr int VM = NA / NW + NB / NW;
   // LDS: the rows' table (slot, scale, factor) and the columns' (scale, bias), or
-  // kWgrad's ring of slots of four steps; then the ring of stages, whose addresses
+  // kWgrad's ring of slots of eight steps; then the ring of stages, whose addresses
   // are formed by XOR below 1 KiB.
   static constexpr int TABLE = (12 * TM + 8 * TN + 1023) / 1024 * 1024;
   static constexpr int LDS_BYTES = TABLE + KS * STAGE;
@@ -49,14 +51,23 @@ struct MmTile {
   static_assert(VM * (KS - 1) < 64, "vmcnt immediate");
 };
 
-// A step's contraction is split between its two instructions by chunks of 16
-// bytes: lane (fr, kseg) takes chunk 2 kseg of its row for the first and 2 kseg + 1
-// for the second (with slot_of the lanes that a ds_read_b128 serves together then
-// hit distinct banks; 4 h + kseg gave two-way conflicts, half of the LDS cycles),
-// of a column-staged operand rows 16 kseg + 8 h to + 7.
-// Chunk rotation of a column-staged row: the four rows that a group of 16 lanes
-// reads together differ in their two low bits, the groups in bit 4.
-MOE_DEVICE int col_swz(int row) { return ((row & 3) << 1) | ((row >> 1) & 8); }
+// Where a row-staged stage has logical 16-byte chunk c of a row, and its inverse
+// (an involution).  A step of 128 bytes is split between its two instructions by
+// chunks: lane (fr, kseg) takes chunk 2 kseg of its row for the first and 2 kseg + 1
+// for the second, of one of 64 bytes chunk kseg.  With these places the lanes that
+// a ds_read_b128 serves together hit distinct banks (chunk 4 h + kseg of a 128-byte
+// row gave two-way conflicts, half of the LDS cycles).
+template <int SB>
+MOE_DEVICE int row_place(int c, int row) {
+  return SB == 128 ? slot_of(c, row) : (c ^ (-(row >> 2) & 3));
+}
+// Chunk rotation of a column-staged row, of which an instruction takes rows
+// 16 kseg + 8 h to + 7, or 8 kseg to + 7: the four rows that a group of 16 lanes
+// reads together differ in their two low bits, the groups in bit 4 or 3.
+template <int SB>
+MOE_DEVICE int col_swz(int row) {
+  return ((row & 3) << 1) | ((SB == 128 ? row >> 1 : row) & 8);
+}
 
 MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
@@ -162,11 +173,11 @@ MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
 template <class OP, bool FP16, int FORM, class K, class T>
 MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int e, int nvalid,
                         int64_t length) {
-  constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS;
+  constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS, SB = T::SB;
   constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
-  constexpr int STEP = 128 / EB;  // contraction elements of a step
+  constexpr int STEP = SB / EB;  // contraction elements of a step
   static_assert(EB == 2 || FORM == kProduct, "transposing reads are of 16-bit values");
-  static_assert(FORM != kWgrad || (KS == 2 && TM == TN), "the ring of slots is for two stages");
+  static_assert(FORM != kWgrad || (KS <= 4 && TM == TN && 8 * STEP * 4 <= K::TABLE), "the ring of slots");
   static_assert(T::THREADS == K::THREADS && T::LDS_BYTES <= K::LDS_BYTES && T::TABLE <= K::TABLE, "a part of the launch's tile");
   const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
   const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
@@ -186,10 +197,11 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   constexpr int ACPR = TM / 8, BCPR = TN / 8;  // chunks of a column-staged row
   const uint8_t* b_base = g.B + (FORM == kWgrad ? 0 : (int64_t)e * g.b_es * EB);
   const uint8_t* zeros = reinterpret_cast<const uint8_t*>(&kZeroChunk);
-  auto row_chunk = [&](int gi) { return slot_of(lane & 7, 8 * gi + (lane >> 3)); };
+  constexpr int LPR = SB / 16, RPI = 64 / LPR;  // lanes of a row, rows of a load
+  auto row_chunk = [&](int gi) { return row_place<SB>(lane % LPR, RPI * gi + lane / LPR); };
   // contraction row and column chunk of a column-staged load
   auto col_row = [&](int gi, int cpr) { return gi * (64 / cpr) + lane / cpr; };
-  auto col_of = [&](int gi, int cpr) { return ((lane % cpr) ^ (col_swz(col_row(gi, cpr)) & (cpr - 1))) * 8; };
+  auto col_of = [&](int gi, int cpr) { return ((lane % cpr) ^ (col_swz<SB>(col_row(gi, cpr)) & (cpr - 1))) * 8; };
 #pragma unroll
   for (int i = 0; i < T::NA_W; ++i) {
     const int gi = wave + T::NW * i;
@@ -197,7 +209,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       const int64_t c = i0 + col_of(gi, ACPR);
       a_ptr[i] = g.A + (c < g.Cn ? c : 0) * EB;
     } else {
-      const int row = 8 * gi + (lane >> 3);
+      const int row = RPI * gi + lane / LPR;
       const int slot = gi < T::NA ? smSlot[row] : -1;
       const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot);
       a_ptr[i] = g.A + ar * g.lda * EB + row_chunk(gi) * 16;
@@ -211,7 +223,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
       if constexpr (FORM == kDgrad) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
     } else {
-      const int64_t j = j0 + 8 * gi + (lane >> 3);
+      const int64_t j = j0 + RPI * gi + lane / LPR;
       b_ptr[i] = b_base + (j < g.J ? j : g.J - 1) * g.sbj * EB + row_chunk(gi) * 16;
     }
   }
@@ -223,14 +235,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   auto read_slots = [&](int kk) {
 #pragma unroll
     for (int i = 0; i < T::NA_W; ++i)
-      slot_r[i] = (uint32_t)smSlot[(kk & 3) * 64 + col_row(wave + T::NW * i, ACPR)];
+      slot_r[i] = (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, ACPR)];
   };
 
   // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
   // partial run of the contraction, so that no other step has to look for its
   // end; the addresses of the others advance from load to load.
   const int tail = (int)(length - (int64_t)(KB - 1) * STEP);  // elements of step 0
-  const int64_t b_step = FORM == kDgrad ? STEP * g.sbc * EB : 128;
+  const int64_t b_step = FORM == kDgrad ? STEP * g.sbc * EB : SB;
   constexpr int ND = T::NA_W + T::NB_W;
   auto load = [&](int kk, int stage, auto dc, auto first_c) {
     constexpr int d = decltype(dc)::value;
@@ -260,12 +272,12 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     } else {
       const uint8_t* p = a_ptr[i];
       if constexpr (first) {
-        p += (int64_t)(KB - 1) * 128;
+        p += (int64_t)(KB - 1) * SB;
         p = row_chunk(gi) * 16 < left * EB ? p : zeros;
       } else {
-        a_ptr[i] += 128;
+        a_ptr[i] += SB;
       }
-      if ((T::NA % T::NW == 0 || gi < T::NA) && 8 * gi < a_rows) lds_load16(p, dst + gi * 1024);
+      if ((T::NA % T::NW == 0 || gi < T::NA) && RPI * gi < a_rows) lds_load16(p, dst + gi * 1024);
     }
   };
   // Loads [from, to) of step kk.
@@ -274,12 +286,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       (load(kk, stage, std::integral_constant<int, decltype(from)::value + D>{}, first), ...);
     }(std::make_integer_sequence<int, decltype(to)::value - decltype(from)::value>{});
   };
-  // kWgrad: the slots of step kk, 64 positions, into the ring (the last wave).
+  // kWgrad: the slots of step kk into the ring (the last wave), kAhead steps before
+  // its own loads are issued: by then the waits for the stages have passed it.
+  constexpr int kAhead = 3;
   auto issue_ids = [&](int kk) {
-    if (wave == T::NW - 1 && kk < KB) {
+    if (wave == T::NW - 1 && kk < KB && lane < STEP) {
       const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
       const int64_t c = c0 + lane < length ? c0 + lane : length - 1;
-      lds_load4(g.sorted + pos0 + c, (uint32_t)(uintptr_t)(lds_ptr)smem + (kk & 3) * 256);
+      lds_load4(g.sorted + pos0 + c, (uint32_t)(uintptr_t)(lds_ptr)smem + (kk & 7) * STEP * 4);
     }
   };
 
@@ -287,14 +301,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   const int fr = lane & 15, kseg = lane >> 4;
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int row_base = wm * T::RS * 16, col_base = wn * T::CS * 16;
-  const uint32_t by_row = fr * 128 + (slot_of(2 * kseg, fr) << 4);  // the second half of the step: XOR 16
-  const int t_row = 16 * kseg + (fr >> 2);                          // and 8 rows on
+  const uint32_t by_row = fr * SB + (row_place<SB>(T::H * kseg, fr) << 4);  // the second half of the step: XOR 16
+  const int t_row = 8 * T::H * kseg + (fr >> 2);                            // and 8 rows on
   // column-staged, subtile s of the operand's columns from `base`: XOR s * 32 into the chunk
   auto by_col = [&](int base, int w) {
-    return (uint32_t)(t_row * w * 2 + (((base / 8 + ((fr & 3) >> 1)) ^ (col_swz(t_row) & (w / 8 - 1))) << 4) + (fr & 1) * 8);
+    return (uint32_t)(t_row * w * 2 + (((base / 8 + ((fr & 3) >> 1)) ^ (col_swz<SB>(t_row) & (w / 8 - 1))) << 4) + (fr & 1) * 8);
   };
-  const uint32_t a_lane = A_COLS ? by_col(row_base, TM) : row_base * 128 + by_row;
-  const uint32_t b_lane = T::A_BYTES + (B_COLS ? by_col(col_base, TN) : col_base * 128 + by_row);
+  const uint32_t a_lane = A_COLS ? by_col(row_base, TM) : row_base * SB + by_row;
+  const uint32_t b_lane = T::A_BYTES + (B_COLS ? by_col(col_base, TN) : col_base * SB + by_row);
 
   typename OP::Acc acc[T::RS][T::CS] = {};
   int ra = (nvalid - row_base + 15) / 16;
@@ -302,7 +316,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
 
   if constexpr (FORM == kWgrad) {
     if (KB > 0) {
-      for (int s = 0; s <= KS; ++s) issue_ids(s);
+      for (int s = 0; s < KS + kAhead; ++s) issue_ids(s);
       mm_wait<0>();
     }
     __syncthreads();
@@ -317,40 +331,42 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     if (s < KB) loads(s, s, none, all, std::false_type{});
   }
 
-  // A step is 2 CS slots of RS matrix instructions, one weight fragment each, which
+  // A step is H CS slots of RS matrix instructions, one weight fragment each, which
   // is read two slots ahead.  The barrier that hands over the next stage stands two
   // slots before the step's end, when every fragment of this stage has been read:
   // the last two slots' instructions cover the reads of the next stage's first
   // fragments, and this stage's buffer is filled again from there on, a load a slot.
-  constexpr int NQ = 2 * T::CS;
+  constexpr int NQ = T::H * T::CS;
   constexpr int DPQ = (ND + NQ - 1) / NQ;  // loads of a slot
   static_assert(NQ >= 4 && NQ % 4 == 0, "four fragment registers in turn");
   auto kloop = [&](auto ra_c) {
     constexpr int RA = decltype(ra_c)::value;
     if (KB == 0) return;
     v4i af[2][RA > 0 ? RA : 1], bf[4];
-    auto read_a = [&](int stage, int h, int r) {
+    auto read_a = [&](int to, int stage, int h, int r) {
       const uint32_t st = lds0 + stage * T::STAGE;
-      if constexpr (A_COLS) af[h][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 8 * TM * 2, TM * 2);
-      else af[h][r] = lds_frag(st + (a_lane ^ (h * 16)) + r * 2048);
+      if constexpr (A_COLS) af[to][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 8 * TM * 2, TM * 2);
+      else af[to][r] = lds_frag(st + (a_lane ^ (h * 16)) + r * 16 * SB);
     };
     auto read_b = [&](int stage, int q) {
       const uint32_t st = lds0 + stage * T::STAGE;
       const int h = q / T::CS, c = q % T::CS;
       if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 8 * TN * 2, TN * 2);
-      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 16)) + c * 2048);
+      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 16)) + c * 16 * SB);
     };
     // stage 0; of the others every wave has at least so many loads behind it
     mm_wait_stages<KS - 1, KS == 2 ? T::NB / T::NW : T::VM>(KB - 1);
     mm_barrier();
     if constexpr (RA > 0) {
 #pragma unroll
-      for (int r = 0; r < RA; ++r) read_a(0, 0, r);
+      for (int r = 0; r < RA; ++r) read_a(0, 0, 0, r);
       read_b(0, 0);
       read_b(0, 1);
     }
     int stage = 0;
-    for (int kk = 0; kk < KB; ++kk) {
+    // P: with one instruction a step, which of the two sets of row fragments it takes
+    auto step = [&](int kk, auto pc) {
+      constexpr int P = decltype(pc)::value;
       const int next = stage == KS - 1 ? 0 : stage + 1, prev = stage == 0 ? KS - 1 : stage - 1;
       auto slot = [&](auto qc) {
         constexpr int Q = decltype(qc)::value;
@@ -360,14 +376,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
             mm_barrier();
             if constexpr (RA > 0) {
 #pragma unroll
-              for (int r = 0; r < RA; ++r) read_a(next, 0, r);
+              for (int r = 0; r < RA; ++r) read_a(T::H == 2 ? 0 : P ^ 1, next, 0, r);
               read_b(next, 0);
               read_b(next, 1);
             }
             if constexpr (FORM == kWgrad) {
               if (kk + KS < KB) {
                 read_slots(kk + KS);
-                issue_ids(kk + KS + 1);
+                issue_ids(kk + KS + kAhead);
               }
             }
           }
@@ -375,10 +391,10 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         if constexpr (RA > 0 && Q < NQ - 2) {
           read_b(stage, Q + 2);
           // the second half's rows: one a slot up to two slots ahead, or together
-          if constexpr (T::CS > RA + 1 && Q + RA >= T::CS - 1 && Q < T::CS - 1) read_a(stage, 1, Q + RA - (T::CS - 1));
-          if constexpr (T::CS <= RA + 1 && Q == 0) {
+          if constexpr (T::H == 2 && T::CS > RA + 1 && Q + RA >= T::CS - 1 && Q < T::CS - 1) read_a(1, stage, 1, Q + RA - (T::CS - 1));
+          if constexpr (T::H == 2 && T::CS <= RA + 1 && Q == 0) {
 #pragma unroll
-            for (int r = 0; r < RA; ++r) read_a(stage, 1, r);
+            for (int r = 0; r < RA; ++r) read_a(1, stage, 1, r);
           }
         }
         // loads of stage kk + KS in this step's last two slots, of the stage before it in the others
@@ -395,9 +411,9 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         // the reads stay ahead of the instructions, which the compiler would undo
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (RA > 0) {
-          constexpr int h = Q / T::CS, c = Q % T::CS;
+          constexpr int at = T::H == 2 ? Q / T::CS : P, c = Q % T::CS;
 #pragma unroll
-          for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf[Q & 3], af[h][r], acc[r][c]);
+          for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf[Q & 3], af[at][r], acc[r][c]);
         }
         __builtin_amdgcn_sched_barrier(0);
       };
@@ -405,6 +421,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         (slot(std::integral_constant<int, Q>{}), ...);
       }(std::make_integer_sequence<int, NQ>{});
       stage = next;
+    };
+    if constexpr (T::H == 2) {
+      for (int kk = 0; kk < KB; ++kk) step(kk, std::integral_constant<int, 0>{});
+    } else {
+      for (int kk = 0; kk < KB; kk += 2) {
+        step(kk, std::integral_constant<int, 0>{});
+        if (kk + 1 < KB) step(kk + 1, std::integral_constant<int, 1>{});
+      }
     }
   };
   switch (ra) {
