@@ -1,0 +1,119 @@
+"""GPU: the tiles of the grouped products at the counts where another one is
+taken: few rows on long weights, narrow tiles where there are few, wide ones where
+there are many, an expert's last rows of a long block, and contractions around the
+rings' lengths.  Element by element against 64 bits, as the size tests."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from grouped_cases import make, off, off_int8, products64  # noqa: E402
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def check(T, k, E, K, N, dtype, block_m=None, forms="ydw", **how):
+    from td_benchmark_amd import ops
+    print(f"case: T={T} k={k} E={E} K={K} N={N} {dtype} BM={block_m} {forms} {how}", flush=True)
+    x, w, ids, dy = make(T, k, E, K, N, dtype, **how)
+    slots = ops.ExpertSlots(ids, E, block_m)
+    (y, dx, dw), (my, mx, mw) = products64(x, w, ids, dy)
+    if "y" in forms:
+        assert off(ops.grouped_mm(x, w, slots), y, my, K) <= 0
+    if "d" in forms:
+        assert off(ops.grouped_mm_dgrad(dy, w, slots), dx, mx, N) <= 0
+    if "w" in forms:
+        assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, ids.numel()) <= 0
+
+
+@pytest.mark.parametrize("K", [1024, 1032, 1096, 2040, 2048, 4104, 8200])
+@pytest.mark.parametrize("T,k,E,block_m", [(1, 1, 1, 16), (1, 8, 64, 16), (3, 2, 5, 32), (2, 8, 32, 32), (16, 1, 1, 16),
+                                           (31, 1, 1, 32), (40, 1, 2, 32)])
+def test_few_rows(T, k, E, block_m, K):
+    check(T, k, E, K, 136, BF16 if K % 16 else FP16, block_m, "y")
+    check(T, k, E, K, 24, BF16, block_m, "y", by_slot=True, drop=0.3)
+
+
+@pytest.mark.parametrize("block_m", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("T,E,K,N", [(150, 40, 72, 80), (150, 40, 520, 600), (700, 70, 1032, 1160), (2600, 20, 1288, 776)])
+def test_tile_widths(T, E, K, N, block_m):
+    check(T, 2, E, K, N, BF16, block_m, "yd")
+
+
+def test_wide_tiles_and_last_rows():
+    """256-row blocks by whole 256-column tiles, with last blocks of one row, under
+    and over 64 and 128 rows, and one full."""
+    from td_benchmark_amd import ops
+    K, N, E = 1032, 1288, 7
+    counts = [256 * 5 + 1, 256 * 5 + 63, 256 * 5 + 64, 256 * 5 + 65, 256 * 5 + 129, 256 * 6, 300]
+    ids = torch.cat([torch.full((c,), e) for e, c in enumerate(counts)])
+    ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(4))].view(-1, 1).cuda()
+    x, w, _, dy = make(ids.numel(), 1, E, K, N, FP16)
+    slots = ops.ExpertSlots(ids, E, 256)
+    (y, dx, dw), (my, mx, mw) = products64(x, w, ids, dy)
+    assert off(ops.grouped_mm(x, w, slots), y, my, K) <= 0
+    assert off(ops.grouped_mm_dgrad(dy, w, slots), dx, mx, N) <= 0
+    assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, max(counts)) <= 0
+
+
+@pytest.mark.parametrize("rows", [1, 8, 31, 32, 33, 63, 64, 65, 96, 97, 128, 129, 160, 161, 192, 225, 257, 300])
+def test_weights_gradient_lengths(rows):
+    """One expert's slots around the steps and the ring of the weights' gradient, beside experts with none."""
+    from td_benchmark_amd import ops
+    K, N = 264, 280
+    x, w, _, dy = make(rows, 1, 3, K, N, BF16)
+    ids = torch.ones((rows, 1), dtype=torch.int64, device="cuda")
+    for block_m in (16, 64, 256):
+        slots = ops.ExpertSlots(ids, 3, block_m)
+        (_, _, dw), (_, _, mw) = products64(x, w, ids, dy)
+        assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, rows) <= 0
+
+
+@pytest.mark.parametrize("K", [8, 56, 64, 72, 120, 128, 136, 192, 200, 256, 264, 320, 392, 456, 520])
+@pytest.mark.parametrize("block_m", [16, 32, 64, 128, 256])
+def test_contraction_lengths(K, block_m):
+    """Around the steps and the rings of every tile, both forms (N is the other one's contraction)."""
+    check(90, 2, 2, K, K + 8, BF16, block_m, "yd")
+
+
+@pytest.mark.parametrize("M,N,K", [(2100, 7168, 80), (2100, 1000, 80), (513, 264, 144), (257, 4104, 208), (129, 8200, 64),
+                                   (65, 16392, 64), (33, 520, 2064), (32, 520, 2064), (16, 24, 6160), (1, 8, 16400)])
+def test_int8_tiles(M, N, K):
+    from td_benchmark_amd import ops
+    g = torch.Generator().manual_seed(M + N + K)
+    a = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8).cuda()
+    b = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8).cuda()
+    sa, sb = (torch.rand(M, generator=g) * 1e-2).cuda(), (torch.rand(N, generator=g) * 1e-2).cuda()
+    bias = torch.randn(N, generator=g).to(BF16).cuda()
+    want = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double() + bias.double()
+    assert off_int8(ops.int8_scaled_mm(a, b, sa, sb, bias), want, bias.double().abs()) <= 0
+
+
+def test_int8_forms_give_equal_bits():
+    """The sums are exact and every form rounds alike: the result depends on neither
+    the block size nor the alignment."""
+    from td_benchmark_amd import ops
+    T, k, E, K, N = 70, 2, 6, 2064, 264
+    g = torch.Generator().manual_seed(8)
+    a = torch.randint(-127, 128, (T, K), generator=g, dtype=torch.int8).cuda()
+    b = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+    sa, sb = torch.rand(T, generator=g).cuda(), torch.rand((E, N), generator=g).cuda()
+    ids = torch.topk(torch.rand((T, E), generator=g), k, dim=1).indices.to(torch.int32).cuda()
+    w = torch.rand((T, k), generator=g).cuda()
+    outs = []
+    for bm in (16, 32, 64, 128, 256):
+        y = torch.zeros((T, k, N), dtype=BF16, device="cuda")
+        ops.dispatch_fused_moe_kernel(a, b, y, sa, sb, None, w, *ops.moe_align_block_size(ids, bm, E), True, k,
+                                      {"BLOCK_SIZE_M": bm}, use_fp8_w8a8=False, use_int8_w8a8=True, per_channel_quant=True)
+        outs.append(y)
+    flat = torch.empty(b.numel() + 1, dtype=torch.int8, device="cuda")
+    odd = flat[1:].view(b.shape)
+    odd.copy_(b)
+    y = torch.zeros((T, k, N), dtype=BF16, device="cuda")
+    ops.dispatch_fused_moe_kernel(a, odd, y, sa, sb, None, w, *ops.moe_align_block_size(ids, 64, E), True, k,
+                                  {"BLOCK_SIZE_M": 64}, use_fp8_w8a8=False, use_int8_w8a8=True, per_channel_quant=True)
+    outs.append(y)
+    for y in outs[1:]:
+        assert torch.equal(y, outs[0])
