@@ -382,31 +382,36 @@ int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64_t R, int64
 /* The slots of a batch grouped by expert: align over E + 1 experts, the last of
  * which takes the slots whose id is outside [0, E), kept in slot_ids [S] int32.
  * topk_ids [S] int32 or int64 (id_bytes 4 or 8).  E <= 1023; max_padded and
- * workspace as for moe_align_block_size with E + 1 experts. */
+ * workspace as for moe_align_block_size with E + 1 experts.  It leaves a table in
+ * the workspace, moe_expert_slots_table(S, E) bytes on: [E + 2] the experts' first
+ * sorted positions, then [E + 1] their slots (the last ones' without an expert). */
+int64_t moe_expert_slots_table(int64_t S, int32_t E);
 int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t S, int32_t E, int32_t block_size_m,
                      int32_t* slot_ids, int32_t* sorted_ids, int32_t* expert_ids, int32_t* ntpp, int64_t max_padded,
                      void* workspace, void* stream);
 
 /* y[s, n] = sum_k x[s / top_k, k] * w[e(s), n, k], e(s) the expert of slot s's
  * block; zero rows where it is outside [0, E).  x [ceil(S/top_k), K] with row
- * stride ldx (elements), w [E, N, K], y [S, N]. */
+ * stride ldx (elements), w [E, N, K], y [S, N].  expert_table: the table of
+ * moe_expert_slots, from which long blocks are dealt out more evenly, or NULL; the
+ * results are the same. */
 int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const int32_t* sorted_ids, const int32_t* expert_ids,
-                   const int32_t* ntpp, int64_t S, int32_t top_k, int64_t N, int64_t K, int32_t E,
-                   int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
+                   const int32_t* ntpp, const int32_t* expert_table, int64_t S, int32_t top_k, int64_t N, int64_t K,
+                   int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
 
 /* Its gradient by the rows, one for each slot: dx[s, k] = sum_n dy[s, n] *
  * w[e(s), n, k].  dy [S, N], dx [S, K]. */
 int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_ids, const int32_t* expert_ids,
-                         const int32_t* ntpp, int64_t S, int64_t N, int64_t K, int32_t E, int32_t block_size_m,
-                         int64_t max_padded, int32_t dtype, void* dx, void* stream);
+                         const int32_t* ntpp, const int32_t* expert_table, int64_t S, int64_t N, int64_t K, int32_t E,
+                         int32_t block_size_m, int64_t max_padded, int32_t dtype, void* dx, void* stream);
 
 /* Its gradient by the weights: dw[e, n, k] = sum over the slots s of e of
  * dy[s, n] * x[s / top_k, k]; zeros for experts without slots.  expert_ids must
  * ascend over the blocks, as align without an expert map writes them. */
 int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, const int32_t* sorted_ids,
-                         const int32_t* expert_ids, const int32_t* ntpp, int64_t S, int32_t top_k, int64_t N,
-                         int64_t K, int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* dw,
-                         void* stream);
+                         const int32_t* expert_ids, const int32_t* ntpp, const int32_t* expert_table, int64_t S,
+                         int32_t top_k, int64_t N, int64_t K, int32_t E, int32_t block_size_m, int64_t max_padded,
+                         int32_t dtype, void* dw, void* stream);
 
 /* The sum of each token's slot rows: y[t] = sum_i d[t * top_k + i].  d
  * [T * top_k, H], y [T, H]. */

@@ -93,10 +93,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moe_silu_and_mul": (ctypes.c_int, [_P, _i64, _i64, _P, _P]),
     "moe_reduce_topk": (ctypes.c_int, [_P, _i64, _i32, _i64, _P, _P]),
     "moe_expert_slots": (ctypes.c_int, [_P, _i32, _i64, _i32, _i32, _P, _P, _P, _P, _i64, _P, _P]),
-    "moe_grouped_mm": (ctypes.c_int, [_P, _i64, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32, _P,
+    "moe_expert_slots_table": (ctypes.c_int64, [_i64, _i32]),
+    "moe_grouped_mm": (ctypes.c_int, [_P, _i64, _P, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32, _P,
                                       _P]),
-    "moe_grouped_mm_dgrad": (ctypes.c_int, [_P, _P, _P, _P, _P, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _P, _P]),
-    "moe_grouped_mm_wgrad": (ctypes.c_int, [_P, _P, _i64, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32,
+    "moe_grouped_mm_dgrad": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _P, _P]),
+    "moe_grouped_mm_wgrad": (ctypes.c_int, [_P, _P, _i64, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32,
                                             _P, _P]),
     "moe_slot_sum": (ctypes.c_int, [_P, _i64, _i32, _i64, _i32, _P, _P]),
     "moe_quant_int8": (ctypes.c_int, [_P, _i64, _i64, _i64, _i32, _P, _P, _P]),

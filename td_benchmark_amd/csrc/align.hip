@@ -658,7 +658,55 @@ __global__ __launch_bounds__(256) void slot_ids_kernel(const ID* __restrict__ id
   out[s] = id >= 0 && id < E ? (int32_t)id : E;
 }
 
+// The same in one workgroup, which also counts: off [E + 2] the experts' first
+// sorted positions (runs padded to BM) and cnt [E + 1] their slots, where align's
+// three launches leave them too.  Up to 16384 slots, where align itself is one
+// launch that keeps no counts; a launch of its own for them would cost 2 us.
+template <class ID>
+__global__ __launch_bounds__(kAlignMaxExperts) void slot_ids_table_kernel(const ID* __restrict__ ids, int S, int E,
+                                                                          int BM, int32_t* __restrict__ out,
+                                                                          int32_t* __restrict__ off,
+                                                                          int32_t* __restrict__ cnt) {
+  __shared__ int32_t hist[kAlignMaxExperts];
+  __shared__ int32_t wave_tot[kAlignMaxExperts / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  hist[tid] = 0;
+  __syncthreads();
+  for (int s = tid; s < S; s += kAlignMaxExperts) {
+    const ID id = ids[s];
+    const int e = id >= 0 && id < E ? (int)id : E;
+    out[s] = e;
+    atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  const int c = hist[tid];
+  const int padded = (c + BM - 1) / BM * BM;
+  int incl = padded;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) wave_tot[wave] = incl;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) incl += wave_tot[w];
+  if (tid <= E) {
+    off[tid] = incl - padded;
+    cnt[tid] = c;
+  }
+  if (tid == E) off[E + 1] = incl;
+}
+
 }  // namespace moe
+
+// Words of the workspace before the table that moe_expert_slots leaves there.
+static int64_t slot_table_at(int64_t S, int32_t E) {
+  return (S + kAlignChunk - 1) / kAlignChunk * ((int64_t)E + 1) + S;
+}
+
+extern "C" int64_t moe_expert_slots_table(int64_t S, int32_t E) {
+  return S < 0 || E <= 0 || E >= kAlignMaxExperts ? -1 : 4 * slot_table_at(S, E);
+}
 
 extern "C" int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t S, int32_t E, int32_t BM,
                                 int32_t* slot_ids, int32_t* sorted_ids, int32_t* expert_ids, int32_t* ntpp,
@@ -669,10 +717,23 @@ extern "C" int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t 
   const int rc = align_args(slot_ids, S, E + 1, BM, sorted_ids, expert_ids, ntpp, max_padded, true, workspace);
   if (rc != kOk) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)((S + 255) / 256));
-  if (S > 0 && id_bytes == 8)
-    hipLaunchKernelGGL(slot_ids_kernel<int64_t>, grid, dim3(256), 0, st, (const int64_t*)topk_ids, S, (int)E, slot_ids);
-  else if (S > 0)
-    hipLaunchKernelGGL(slot_ids_kernel<int32_t>, grid, dim3(256), 0, st, (const int32_t*)topk_ids, S, (int)E, slot_ids);
+  const auto ids64 = (const int64_t*)topk_ids;
+  const auto ids32 = (const int32_t*)topk_ids;
+  if (align_one_launch(S, E + 1, nullptr)) {
+    int32_t* off = (int32_t*)workspace + slot_table_at(S, E);
+    int32_t* cnt = off + E + 2;
+    if (id_bytes == 8)
+      hipLaunchKernelGGL(slot_ids_table_kernel<int64_t>, dim3(1), dim3(kAlignMaxExperts), 0, st, ids64, (int)S, (int)E,
+                         (int)BM, slot_ids, off, cnt);
+    else
+      hipLaunchKernelGGL(slot_ids_table_kernel<int32_t>, dim3(1), dim3(kAlignMaxExperts), 0, st, ids32, (int)S, (int)E,
+                         (int)BM, slot_ids, off, cnt);
+  } else {
+    const dim3 grid((unsigned)((S + 255) / 256));
+    if (id_bytes == 8)
+      hipLaunchKernelGGL(slot_ids_kernel<int64_t>, grid, dim3(256), 0, st, ids64, S, (int)E, slot_ids);
+    else
+      hipLaunchKernelGGL(slot_ids_kernel<int32_t>, grid, dim3(256), 0, st, ids32, S, (int)E, slot_ids);
+  }
   return align_impl(slot_ids, S, E + 1, BM, nullptr, sorted_ids, expert_ids, ntpp, max_padded, workspace, stream);
 }

@@ -161,8 +161,27 @@ static int launch_tile(MmArgs g, hipStream_t st) {
                           T::LDS_BYTES);
   if (attr != hipSuccess) return kErrLaunch;
   g.n_jt = (g.J + T::TN - 1) / T::TN;
-  const int64_t tiles = (FORM == kWgrad ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt;
-  const int64_t deal = FORM == kWgrad ? 8 * kWgradChunk : 8, grid = (tiles + deal - 1) / deal * deal;
+  int64_t tiles = (FORM == kWgrad ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt, more = 0;
+  if (FORM != kWgrad) {
+    // The short last tiles apart from the whole ones: even rounds, but an expert's
+    // weights are read once more for its short tile, about 250 / rows of its time.
+    // It pays where the launch has few rounds and the runs are long (8 experts of
+    // 1024 rows, 28672 to 4096 columns, 2.3 rounds: 2200 us by blocks, 1802 so; to
+    // 28672 columns, 16 rounds: 1800 and 1890; 64 of 512 rows 465 and 510; 128 of 256
+    // 311 and 376).
+    const int64_t used = g.S < g.E ? g.S : g.E;
+    if (T::TM != 256 || g.S < 768 * (int64_t)g.E || g.S / 256 * g.n_jt > 1024) g.table = nullptr;
+    if (g.table) {  // whole tiles: at most S / 256 and one more an expert; then the short ones
+      tiles = (g.S / 256 + used + 1) * g.n_jt;
+      if (T::TN == 256) {
+        g.short_parts = used * g.n_jt <= 256 && g.Cn * OP::BYTES >= 64 * 128 ? 4 : 1;
+        more = used * g.n_jt * g.short_parts;
+      }
+    }
+  }
+  const int64_t deal = FORM == kWgrad ? 8 * kWgradChunk : 8;
+  g.shorts = (tiles + deal - 1) / deal * deal;
+  const int64_t grid = g.shorts + more;
   if (grid > 0x7FFFFFFF) return kErrBadShape;
   hipLaunchKernelGGL((tile_mm_kernel<OP, FP16, FORM, T>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
@@ -354,9 +373,9 @@ static int slots_ok(const int32_t* sorted, const int32_t* eids, const int32_t* n
 using namespace moe;
 
 extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const int32_t* sorted_ids,
-                              const int32_t* expert_ids, const int32_t* ntpp, int64_t S, int32_t top_k, int64_t N,
-                              int64_t K, int32_t E, int32_t BM, int64_t max_padded, int32_t dtype, void* y,
-                              void* stream) {
+                              const int32_t* expert_ids, const int32_t* ntpp, const int32_t* table, int64_t S,
+                              int32_t top_k, int64_t N, int64_t K, int32_t E, int32_t BM, int64_t max_padded,
+                              int32_t dtype, void* y, void* stream) {
   const int rc = slots_ok(sorted_ids, expert_ids, ntpp, S, E, BM, max_padded);
   if (rc != kOk) return rc;
   if (N < 0 || K < 0 || ldx < K || (dtype != kBf16 && dtype != kFp16)) return kErrBadShape;
@@ -371,6 +390,7 @@ extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const i
   g.sorted = sorted_ids;
   g.eids = expert_ids;
   g.ntpp = ntpp;
+  g.table = table;
   g.S = S;
   g.J = N;
   g.Cn = K;
@@ -390,8 +410,9 @@ extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const i
 }
 
 extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_ids,
-                                    const int32_t* expert_ids, const int32_t* ntpp, int64_t S, int64_t N, int64_t K,
-                                    int32_t E, int32_t BM, int64_t max_padded, int32_t dtype, void* dx, void* stream) {
+                                    const int32_t* expert_ids, const int32_t* ntpp, const int32_t* table, int64_t S,
+                                    int64_t N, int64_t K, int32_t E, int32_t BM, int64_t max_padded, int32_t dtype,
+                                    void* dx, void* stream) {
   const int rc = slots_ok(sorted_ids, expert_ids, ntpp, S, E, BM, max_padded);
   if (rc != kOk) return rc;
   if (N < 0 || K < 0 || (dtype != kBf16 && dtype != kFp16)) return kErrBadShape;
@@ -405,6 +426,7 @@ extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t
   g.sorted = sorted_ids;
   g.eids = expert_ids;
   g.ntpp = ntpp;
+  g.table = table;
   g.S = S;
   g.J = K;
   g.Cn = N;
@@ -424,9 +446,9 @@ extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t
 }
 
 extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, const int32_t* sorted_ids,
-                                    const int32_t* expert_ids, const int32_t* ntpp, int64_t S, int32_t top_k,
-                                    int64_t N, int64_t K, int32_t E, int32_t BM, int64_t max_padded, int32_t dtype,
-                                    void* dw, void* stream) {
+                                    const int32_t* expert_ids, const int32_t* ntpp, const int32_t* table, int64_t S,
+                                    int32_t top_k, int64_t N, int64_t K, int32_t E, int32_t BM, int64_t max_padded,
+                                    int32_t dtype, void* dw, void* stream) {
   const int rc = slots_ok(sorted_ids, expert_ids, ntpp, S, E, BM, max_padded);
   if (rc != kOk) return rc;
   if (N < 0 || K < 0 || ldx < K || (dtype != kBf16 && dtype != kFp16)) return kErrBadShape;
@@ -441,6 +463,7 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   g.sorted = sorted_ids;
   g.eids = expert_ids;
   g.ntpp = max_padded > 0 ? ntpp : nullptr;  // without positions: no blocks
+  g.table = max_padded > 0 ? table : nullptr;
   g.S = S;
   g.J = K;
   g.Cn = N;

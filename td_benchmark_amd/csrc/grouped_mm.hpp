@@ -95,6 +95,11 @@ struct MmArgs {
   int64_t ldc;          // row stride of the output
   int64_t n_jt;         // column tiles
   int64_t n_blocks;     // blocks that fit in max_padded
+  // [E + 2] first positions and [E + 1] slots of the experts and of the slots
+  // without one, or null
+  const int32_t* table;
+  int64_t shorts;       // rows form with a table: workgroups from this one on take the experts' short last tiles,
+  int short_parts;      // so many of them each
   int bm, top_k, a_by_pos, E;
   // slot / top_k = slot * div_mul >> div_shift for slots below 2^31
   uint32_t div_mul;
@@ -142,6 +147,7 @@ struct Run {
   int64_t pos0, count;
 };
 MOE_DEVICE Run run_of(const MmArgs& g, int e) {
+  if (g.table) return {g.table[e], g.table[g.E + 2 + e]};
   const int64_t nb = live_blocks(g);
   int64_t b0 = 0, h0 = nb, b1 = 0, h1 = nb;
   while (b0 < h0 || b1 < h1) {  // both ends in the same rounds: two up to 4096 blocks

@@ -167,12 +167,82 @@ MOE_DEVICE bool rows_tile(const MmArgs& g, int64_t& b, int64_t& j) {
   return true;
 }
 
+// With a table, the tiles of long blocks by the experts' counts: TM rows each, an
+// expert's last one of up to SHORT rows apart (`part` of the workgroups that share
+// it).  The whole tiles are dealt to the XCDs evenly, as above, but by their number
+// alone: a short tile counted as a whole one gives some XCDs more whole ones than
+// others, which is a round more where there are few.
+template <int TM, int SHORT>
+MOE_DEVICE bool table_tile(const MmArgs& g, int64_t& pos0, int64_t& j, int& e, int& nvalid, int& part) {
+  constexpr int kGroup = 4;
+  const int lane = threadIdx.x & 63, E1 = g.E + 1, n_jt = (int)g.n_jt;
+  const int32_t* cnt = g.table + E1 + 1;
+  const bool last = SHORT && (int64_t)blockIdx.x >= g.shorts;
+  int c, n, incl;  // of the lane's expert: slots, row tiles, and those up to it among these 64
+  auto look = [&](int i) {
+    c = i < E1 ? cnt[i] : 0;
+    const int rest = c % TM;
+    const bool is_short = rest > 0 && rest <= SHORT && i < g.E;
+    n = last ? (is_short ? 1 : 0) : c / TM + (rest > 0 && !is_short ? 1 : 0);
+    incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(incl, o);
+      if (lane >= o) incl += y;
+    }
+  };
+  int rows = 0;
+  for (int i0 = 0; i0 < E1; i0 += 64) {
+    look(i0 + lane);
+    rows += __builtin_amdgcn_readlane(incl, 63);
+  }
+  const int each = last ? n_jt * g.short_parts : n_jt, total = rows * each;
+  int t;
+  if (last) {
+    t = (int)((int64_t)blockIdx.x - g.shorts);
+  } else {
+    const int per = (total + 7) / 8, l = (int)(blockIdx.x / 8);
+    if (l >= per) return false;
+    t = (int)(blockIdx.x % 8) * per + l;
+  }
+  if (t >= total) return false;
+  const int at = t / each;  // the row tile among all experts'
+  int before = 0;
+  for (int i0 = 0;; i0 += 64) {
+    if (E1 > 64) look(i0 + lane);
+    const uint64_t hit = __ballot(before + incl > at);
+    if (hit) {
+      const int src = __ffsll((unsigned long long)hit) - 1;
+      e = i0 + src;
+      n = __builtin_amdgcn_readlane(n, src);
+      c = __builtin_amdgcn_readlane(c, src);
+      before += __builtin_amdgcn_readlane(incl, src) - n;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  int u;
+  if (last) {
+    u = c / TM;
+    part = t % each % g.short_parts;
+    j = t % each / g.short_parts;
+  } else {
+    const int in = t - before * n_jt, g0 = in / (kGroup * n) * kGroup, w = n_jt - g0 < kGroup ? n_jt - g0 : kGroup;
+    part = 0;
+    j = g0 + (in - g0 * n) % w;
+    u = (in - g0 * n) / w;
+  }
+  pos0 = g.table[e] + (int64_t)u * TM;
+  nvalid = c - u * TM < TM ? c - u * TM : TM;
+  return true;
+}
+
 // One tile: rows [i0, i0 + nvalid) of the output, or the nvalid slots of the
-// table, by columns j0 on, over `length` of the contraction.  K: the tile of the
-// launch, which T is or is shorter than.
+// table, by columns j0 on (col0 on of the columns' table), over `length` of the
+// contraction.  K: the tile of the launch, which T is or is a part of.
 template <class OP, bool FP16, int FORM, class K, class T>
-MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int e, int nvalid,
-                        int64_t length) {
+MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int col0, int e,
+                        int nvalid, int64_t length) {
   constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS, SB = T::SB;
   constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
   constexpr int STEP = SB / EB;  // contraction elements of a step
@@ -182,7 +252,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
   const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
   const float* smW = reinterpret_cast<const float*>(smem) + 2 * K::TM;
-  const float* smSb = reinterpret_cast<const float*>(smem) + 3 * K::TM;
+  const float* smSb = reinterpret_cast<const float*>(smem) + 3 * K::TM + col0;
   const float* smBias = smSb + K::TN;
   uint8_t* const ring = smem + K::TABLE;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)ring;
@@ -492,16 +562,28 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     const int64_t w = nt - ig < kGroup ? nt - ig : kGroup, at = in - ig * g.n_jt;
     const int64_t i0 = (ig + at % w) * TM, j0 = at / w * TN;
     const Run r = run_of(g, e);
-    mm_tile<OP, FP16, FORM, T, T>(g, smem, r.pos0, i0, j0, e, (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM), r.count);
+    mm_tile<OP, FP16, FORM, T, T>(g, smem, r.pos0, i0, j0, 0, e, (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM), r.count);
   } else {
-    int64_t b, j;
-    constexpr bool GROUPED = TM == 256;
-    if (!rows_tile<GROUPED>(g, b, j)) return;
-    const int64_t j0 = j * TN, pos0 = b * TM;
-    const int rows = !g.eids && pos0 + TM > g.S ? (int)(g.S - pos0) : TM;
-    const int e = g.eids ? g.eids[b] : 0;
-    // the rows' slots, their scales and factors, for their addresses and the results
+    // An expert's last block of up to kShort rows takes a shorter tile with a deeper
+    // ring; alone on its CU it waits for its weights (50-60 GB/s) as long as a whole
+    // tile takes, so that several workgroups share it where the launch has few rounds.
+    constexpr int kShort = TM == 256 && TN == 256 ? 64 : 0;
     int32_t* smSlot = reinterpret_cast<int32_t*>(smem);
+    int64_t pos0, j;
+    int e, nvalid = 0, part = 0;
+    const bool planned = TM == 256 && g.table;
+    if (planned) {
+      if constexpr (TM == 256)
+        if (!table_tile<TM, kShort>(g, pos0, j, e, nvalid, part)) return;
+    } else {
+      int64_t b;
+      if (!rows_tile<TM == 256>(g, b, j)) return;
+      pos0 = b * TM;
+      e = g.eids ? g.eids[b] : 0;
+    }
+    const int64_t j0 = j * TN;
+    const int rows = planned ? nvalid : !g.eids && pos0 + TM > g.S ? (int)(g.S - pos0) : TM;
+    // the rows' slots, their scales and factors, for their addresses and the results
     bool valid = false;
     static_assert(TM <= T::THREADS, "a thread a row");
     if (tid < TM) {
@@ -521,7 +603,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
         cols[TN + c] = g.bias ? from16<FP16>(g.bias[jj]) : 0.0f;
       }
     }
-    const int nvalid = __syncthreads_count(valid);
+    nvalid = __syncthreads_count(valid);
     if (nvalid == 0) return;
     if (e < 0 || e >= g.E) {  // no expert: zero rows
       for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
@@ -531,14 +613,18 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
       }
       return;
     }
-    // An expert's last rows: a tile that they fill, whose ring is deeper.
-    if constexpr (TM == 256 && TN == 256) {
-      if (nvalid <= 64) {
-        mm_tile<OP, FP16, FORM, T, MmTile<64, 256, 8, 1, 3, 1>>(g, smem, pos0, 0, j0, e, nvalid, g.Cn);
+    if constexpr (kShort > 0) {
+      if (nvalid <= kShort) {
+        if (planned && g.short_parts == 4) {
+          if (j0 + part * 64 < g.J)
+            mm_tile<OP, FP16, FORM, T, MmTile<64, 64, 8, 4, 6, 1>>(g, smem, pos0, 0, j0 + part * 64, part * 64, e, nvalid, g.Cn);
+        } else {
+          mm_tile<OP, FP16, FORM, T, MmTile<64, 256, 8, 1, 3, 1>>(g, smem, pos0, 0, j0, 0, e, nvalid, g.Cn);
+        }
         return;
       }
     }
-    mm_tile<OP, FP16, FORM, T, T>(g, smem, pos0, 0, j0, e, nvalid, g.Cn);
+    mm_tile<OP, FP16, FORM, T, T>(g, smem, pos0, 0, j0, 0, e, nvalid, g.Cn);
   }
 }
 

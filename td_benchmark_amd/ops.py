@@ -1368,16 +1368,17 @@ class ExpertSlots:
         _need_here("topk_ids", topk_ids)
         self.device = topk_ids.device
         # slot ids, sorted ids, block experts, the positions' count and align's workspace in one allocation
-        self.max_padded, blocks, self._sizes = _slots_layout(self.S, self.E, self.block_size_m)
+        self.max_padded, table, self._sizes = _slots_layout(self.S, self.E, self.block_size_m)
         self._buf = torch.empty(sum(self._sizes), dtype=torch.int32, device=self.device)
         ids = topk_ids.contiguous()
         at = self._buf.data_ptr()
         at_sorted = at + 4 * self._sizes[0]
         at_eids = at_sorted + 4 * self._sizes[1]
         at_ntpp = at_eids + 4 * self._sizes[2]
-        self._at = (at_sorted, at_eids, at_ntpp)
+        at_work = at_ntpp + 4 * self._sizes[3]
+        self._at = (at_sorted, at_eids, at_ntpp, at_work + table)
         check(lib().moe_expert_slots(ids.data_ptr(), ids.element_size(), self.S, self.E, self.block_size_m, at,
-                                     at_sorted, at_eids, at_ntpp, self.max_padded, at_ntpp + 4 * self._sizes[3],
+                                     at_sorted, at_eids, at_ntpp, self.max_padded, at_work,
                                      _stream_handle()), "moe_expert_slots")
 
     def _part(self, i: int, n: int) -> torch.Tensor:
@@ -1402,11 +1403,13 @@ class ExpertSlots:
 
 @functools.lru_cache(maxsize=256)
 def _slots_layout(S: int, E: int, block_m: int) -> tuple[int, int, tuple[int, ...]]:
-    """-> sorted positions, blocks, and the int32 words of ExpertSlots' parts (whole 16 bytes each)."""
+    """-> sorted positions, where the experts' table lies in the workspace, and the int32 words of ExpertSlots' parts
+    (whole 16 bytes each)."""
     mp = align_max_padded(S, E + 1, block_m)
     blocks = (mp + block_m - 1) // block_m
     work = align_workspace_bytes(S, E + 1)
-    return mp, blocks, tuple(max(n + 3, 4) // 4 * 4 for n in (S, mp, blocks, 1, (work + 3) // 4))
+    table = int(lib().moe_expert_slots_table(S, E))
+    return mp, table, tuple(max(n + 3, 4) // 4 * 4 for n in (S, mp, blocks, 1, (work + 3) // 4))
 
 
 def slots_block_m(num_slots: int, num_experts: int) -> int:

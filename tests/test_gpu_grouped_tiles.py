@@ -117,3 +117,45 @@ def test_int8_forms_give_equal_bits():
     outs.append(y)
     for y in outs[1:]:
         assert torch.equal(y, outs[0])
+
+
+@pytest.mark.parametrize("K,N,counts", [
+    (1288, 520, (800, 1030, 768 + 64, 1024, 1)),     # tiles dealt by the experts' counts, short ones whole
+    (520, 4104, (769, 1100, 900, 2000, 0, 513)),     # and in quarters (a contraction of 64 steps)
+])
+def test_few_long_experts(K, N, counts):
+    from td_benchmark_amd import ops
+    E = len(counts)
+    ids = torch.cat([torch.full((c,), e) for e, c in enumerate(counts)] + [torch.full((37,), -1)])
+    ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(6))].view(-1, 1).cuda()
+    x, w, _, dy = make(ids.numel(), 1, E, K, N, BF16)
+    slots = ops.ExpertSlots(ids, E)
+    (y, dx, dw), (my, mx, mw) = products64(x, w, ids, dy)
+    assert off(ops.grouped_mm(x, w, slots), y, my, K) <= 0
+    assert off(ops.grouped_mm_dgrad(dy, w, slots), dx, mx, N) <= 0
+    assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, max(counts)) <= 0
+
+
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (5, 3, 7), (1000, 2, 5), (8192, 2, 3), (16384, 1, 9), (8193, 2, 9), (9000, 8, 60),
+                                   (300, 8, 1023), (16000, 1, 1000)])
+def test_slot_table(T, k, E):
+    """The experts' first positions and counts that the products deal tiles by,
+    against the ids, for the one-launch and the three-launch align."""
+    from td_benchmark_amd import _lib, ops
+    g = torch.Generator().manual_seed(T + E)
+    ids = torch.randint(-1, E + 1, (T, k), generator=g)
+    L = _lib.lib()
+    for bm, dtype in ((16, torch.int32), (256, torch.int64)):
+        dev = ids.to(dtype).cuda()
+        slots = ops.ExpertSlots(dev, E, bm)
+        at = L.moe_expert_slots_table(T * k, E)
+        off_words = (slots._at[3] - slots._buf.data_ptr()) // 4
+        assert slots._at[3] - (slots._at[2] + 16) == at
+        table = slots._buf[off_words: off_words + 2 * E + 3].cpu()
+        flat = ids.view(-1)
+        flat = torch.where((flat < 0) | (flat >= E), E, flat)
+        cnt = torch.bincount(flat, minlength=E + 1)
+        padded = (cnt + bm - 1) // bm * bm
+        assert torch.equal(table[E + 2:].long(), cnt)
+        assert torch.equal(table[1: E + 2].long(), padded.cumsum(0)) and table[0] == 0
+        assert int(slots.ntpp.item()) == int(padded.sum())

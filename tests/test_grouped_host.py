@@ -105,18 +105,18 @@ def test_c_entries_refuse(L):
                                                       "MOE_ERR_BAD_TOPK", "MOE_ERR_BAD_EXPERTS"))
     ok = E["MOE_OK"]
     mm = lambda x=p, ldx=16, w=p, srt=p, S=8, k=2, N=24, K=16, e=3, bm=16, mp=48, dt=0, y=p: L.moe_grouped_mm(  # noqa: E731
-        x, ldx, w, srt, p, p, S, k, N, K, e, bm, mp, dt, y, None)
+        x, ldx, w, srt, p, p, None, S, k, N, K, e, bm, mp, dt, y, None)
     for want, kw in ((null, dict(x=None)), (null, dict(w=None)), (null, dict(srt=None)), (null, dict(y=None)), (bad, dict(ldx=15)),
                      (bad, dict(S=-1)), (bad, dict(N=-1)), (bad, dict(K=-1)), (bad, dict(dt=2)), (bad, dict(mp=-1)), (bad, dict(x=odd)),
                      (topk, dict(k=0)), (experts, dict(e=0)), (block, dict(bm=48)), (ok, dict(S=0)), (ok, dict(N=0))):
         assert mm(**kw) == want, kw
     dg = lambda dy=p, w=p, S=8, N=24, K=16, e=3, bm=16, mp=48, dt=0, dx=p: L.moe_grouped_mm_dgrad(  # noqa: E731
-        dy, w, p, p, p, S, N, K, e, bm, mp, dt, dx, None)
+        dy, w, p, p, p, None, S, N, K, e, bm, mp, dt, dx, None)
     for want, kw in ((null, dict(dy=None)), (null, dict(w=None)), (null, dict(dx=None)), (bad, dict(N=-1)), (bad, dict(dt=7)),
                      (bad, dict(dx=odd)), (experts, dict(e=-1)), (block, dict(bm=0)), (ok, dict(S=0)), (ok, dict(K=0))):
         assert dg(**kw) == want, kw
     wg = lambda dy=p, x=p, ldx=16, S=8, k=2, N=24, K=16, e=3, bm=16, mp=48, dt=0, dw=p: L.moe_grouped_mm_wgrad(  # noqa: E731
-        dy, x, ldx, p, p, p, S, k, N, K, e, bm, mp, dt, dw, None)
+        dy, x, ldx, p, p, p, None, S, k, N, K, e, bm, mp, dt, dw, None)
     for want, kw in ((null, dict(dy=None)), (null, dict(x=None)), (null, dict(dw=None)), (bad, dict(ldx=8)), (bad, dict(dt=-1)),
                      (bad, dict(dw=odd)), (topk, dict(k=-1)), (experts, dict(e=0)), (block, dict(bm=512)), (ok, dict(N=0))):
         assert wg(**kw) == want, kw
