@@ -400,10 +400,12 @@ int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const int32_t* sor
                    int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
 
 /* Its gradient by the rows, one for each slot: dx[s, k] = sum_n dy[s, n] *
- * w[e(s), n, k].  dy [S, N], dx [S, K]. */
+ * w[e(s), n, k].  dy [S, N], dx [S, K] of dtype, or of fp32 with rows_f32 (for
+ * moe_slot_sum). */
 int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_ids, const int32_t* expert_ids,
                          const int32_t* ntpp, const int32_t* expert_table, int64_t S, int64_t N, int64_t K, int32_t E,
-                         int32_t block_size_m, int64_t max_padded, int32_t dtype, void* dx, void* stream);
+                         int32_t block_size_m, int64_t max_padded, int32_t dtype, int32_t rows_f32, void* dx,
+                         void* stream);
 
 /* Its gradient by the weights: dw[e, n, k] = sum over the slots s of e of
  * dy[s, n] * x[s / top_k, k]; zeros for experts without slots.  expert_ids must
@@ -414,8 +416,8 @@ int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, const int32
                          int32_t dtype, void* dw, void* stream);
 
 /* The sum of each token's slot rows: y[t] = sum_i d[t * top_k + i].  d
- * [T * top_k, H], y [T, H]. */
-int moe_slot_sum(const void* d, int64_t T, int32_t top_k, int64_t H, int32_t dtype, void* y, void* stream);
+ * [T * top_k, H] fp32, y [T, H] of dtype. */
+int moe_slot_sum(const float* d, int64_t T, int32_t top_k, int64_t H, int32_t dtype, void* y, void* stream);
 
 /* Dynamic int8 quant with a scale a row: s = max(amax / 127, 1e-12), q =
  * clamp(rint(x / s), +-127).  A row that holds an infinity or a NaN gets it as

@@ -96,7 +96,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moe_expert_slots_table": (ctypes.c_int64, [_i64, _i32]),
     "moe_grouped_mm": (ctypes.c_int, [_P, _i64, _P, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32, _P,
                                       _P]),
-    "moe_grouped_mm_dgrad": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _P, _P]),
+    "moe_grouped_mm_dgrad": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _i32, _P,
+                                            _P]),
     "moe_grouped_mm_wgrad": (ctypes.c_int, [_P, _P, _i64, _P, _P, _P, _P, _i64, _i32, _i64, _i64, _i32, _i32, _i64, _i32,
                                             _P, _P]),
     "moe_slot_sum": (ctypes.c_int, [_P, _i64, _i32, _i64, _i32, _P, _P]),

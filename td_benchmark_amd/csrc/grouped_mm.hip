@@ -137,7 +137,8 @@ __global__ __launch_bounds__(256) void any_mm_kernel(MmArgs g) {
         } else {
           f = acc[r][c][v];
         }
-        reinterpret_cast<uint16_t*>(g.C)[orow * g.ldc + j] = (uint16_t)pack2<FP16>(f, 0.0f);
+        if (g.out32) reinterpret_cast<float*>(g.C)[orow * g.ldc + j] = f;
+        else reinterpret_cast<uint16_t*>(g.C)[orow * g.ldc + j] = (uint16_t)pack2<FP16>(f, 0.0f);
       }
   }
 }
@@ -412,13 +413,13 @@ extern "C" int moe_grouped_mm(const void* x, int64_t ldx, const void* w, const i
 extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_ids,
                                     const int32_t* expert_ids, const int32_t* ntpp, const int32_t* table, int64_t S,
                                     int64_t N, int64_t K, int32_t E, int32_t BM, int64_t max_padded, int32_t dtype,
-                                    void* dx, void* stream) {
+                                    int32_t rows_f32, void* dx, void* stream) {
   const int rc = slots_ok(sorted_ids, expert_ids, ntpp, S, E, BM, max_padded);
   if (rc != kOk) return rc;
   if (N < 0 || K < 0 || (dtype != kBf16 && dtype != kFp16)) return kErrBadShape;
   if (S == 0 || K == 0 || max_padded == 0) return kOk;
   if (!dx || (N > 0 && (!dy || !w))) return kErrNullPointer;
-  if (!aligned(dy, 2) || !aligned(w, 2) || !aligned(dx, 2)) return kErrBadShape;
+  if (!aligned(dy, 2) || !aligned(w, 2) || !aligned(dx, rows_f32 ? 4 : 2)) return kErrBadShape;
   MmArgs g{};
   g.A = (const uint8_t*)dy;
   g.B = (const uint8_t*)w;
@@ -438,6 +439,7 @@ extern "C" int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t
   g.n_blocks = max_padded / BM;
   g.bm = BM;
   set_top_k(g, 1);
+  g.out32 = rows_f32 ? 1 : 0;
   g.E = E;
   hipStream_t st = (hipStream_t)stream;
   if (N > 0 && chunks(dy, N, 2) && chunks(w, K, 2) && chunks(dx, K, 2))

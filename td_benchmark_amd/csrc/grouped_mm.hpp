@@ -100,6 +100,7 @@ struct MmArgs {
   const int32_t* table;
   int64_t shorts;       // rows form with a table: workgroups from this one on take the experts' short last tiles,
   int short_parts;      // so many of them each
+  int out32;            // kDgrad: rows of fp32, which are summed over a token's slots before they are rounded
   int bm, top_k, a_by_pos, E;
   // slot / top_k = slot * div_mul >> div_shift for slots below 2^31
   uint32_t div_mul;

@@ -510,6 +510,33 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   }
   mm_barrier();
 
+  if constexpr (FORM == kDgrad) {
+    // fp32 rows: 16 rows of the wave's columns a time through its own part of the
+    // ring, so that a row's columns leave as one run
+    if (g.out32) {
+      constexpr int CPR = 4 * T::CS;  // 16-byte chunks of a row
+      static_assert(T::NW * 16 * CPR * 16 <= KS * T::STAGE, "staging of fp32 rows");
+      v4f* part = reinterpret_cast<v4f*>(ring) + wave * 16 * CPR;
+#pragma unroll
+      for (int r = 0; r < T::RS; ++r) {
+        if (row_base + r * 16 >= nvalid) break;
+#pragma unroll
+        for (int c = 0; c < T::CS; ++c) part[fr * CPR + ((4 * c + kseg) ^ (fr & (CPR - 1) & 15))] = acc[r][c];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < CPR / 4; ++i) {
+          const int row = (i * 64 + lane) / CPR, cc = (i * 64 + lane) % CPR;
+          const int64_t jj = j0 + col_base + 4 * cc;
+          const v4f v = part[row * CPR + (cc ^ (row & (CPR - 1) & 15))];
+          if (row_base + r * 16 + row < nvalid && jj < g.J)
+            *reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + (int64_t)smSlot[row_base + r * 16 + row] * g.ldc + jj) = v;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      return;
+    }
+  }
+
   // ---- epilogue: rows of 16-bit outputs through LDS, chunks XOR the row ----
   uint16_t* out = reinterpret_cast<uint16_t*>(ring);
   constexpr int CH = TN / 8, ROT = CH < 16 ? CH - 1 : 15;
@@ -608,8 +635,14 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     if (e < 0 || e >= g.E) {  // no expert: zero rows
       for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
         const int64_t jj = j0 + c % (TN / 8) * 8;
-        if (jj < g.J)
-          *reinterpret_cast<v4i*>(g.C + ((int64_t)smSlot[c / (TN / 8)] * g.ldc + jj) * 2) = (v4i){0, 0, 0, 0};
+        if (jj >= g.J) continue;
+        const int64_t at = (int64_t)smSlot[c / (TN / 8)] * g.ldc + jj;
+        if (FORM == kDgrad && g.out32) {
+          v4f* to = reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + at);
+          to[0] = to[1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        } else {
+          *reinterpret_cast<v4i*>(g.C + at * 2) = (v4i){0, 0, 0, 0};
+        }
       }
       return;
     }

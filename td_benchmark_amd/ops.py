@@ -1458,10 +1458,12 @@ def _grouped_product(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> to
 def _dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool) -> torch.Tensor:
     E, N, K = w.shape
     dtype, stream = _DTYPE_CODE[dy.dtype], _stream_handle()
-    dx = torch.empty((slots.S, K), dtype=dy.dtype, device=dy.device)
+    summed = by_token and slots.top_k > 1
+    dx = torch.empty((slots.S, K), dtype=torch.float32 if summed else dy.dtype, device=dy.device)
     check(lib().moe_grouped_mm_dgrad(dy.data_ptr(), w.data_ptr(), *slots._at, slots.S, N, K, E, slots.block_size_m,
-                                     slots.max_padded, dtype, dx.data_ptr(), stream), "moe_grouped_mm_dgrad")
-    if not by_token or slots.top_k == 1:
+                                     slots.max_padded, dtype, 1 if summed else 0, dx.data_ptr(), stream),
+          "moe_grouped_mm_dgrad")
+    if not summed:
         return dx
     out = torch.empty((slots.T, K), dtype=dy.dtype, device=dy.device)
     check(lib().moe_slot_sum(dx.data_ptr(), slots.T, slots.top_k, K, dtype, out.data_ptr(), stream), "moe_slot_sum")
@@ -1480,8 +1482,7 @@ def _wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tenso
 
 def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool = False) -> torch.Tensor:
     """The gradient of ``grouped_mm`` by its rows: dx[s] = dy[s] @ w[e(s)], [S, K].
-    ``by_token``: summed over each token's slots (fp32, of the rows rounded to
-    dy's type), [T, K]."""
+    ``by_token``: summed over each token's slots in fp32 and rounded once, [T, K]."""
     if dy.dim() != 2 or w.dim() != 3:
         raise ValueError(f"dy must be [S, N] and w [E, N, K], got {tuple(dy.shape)} and {tuple(w.shape)}")
     if dy.dtype not in _DTYPE_CODE:

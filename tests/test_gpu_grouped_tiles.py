@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from grouped_cases import make, off, off_int8, products64  # noqa: E402
+from grouped_cases import by_token, make, off, off_int8, products64  # noqa: E402
 
 BF16, FP16 = torch.bfloat16, torch.float16
 
@@ -159,3 +159,20 @@ def test_slot_table(T, k, E):
         assert torch.equal(table[E + 2:].long(), cnt)
         assert torch.equal(table[1: E + 2].long(), padded.cumsum(0)) and table[0] == 0
         assert int(slots.ntpp.item()) == int(padded.sum())
+
+
+@pytest.mark.parametrize("T,k,E,K,N,block_m", [(37, 2, 5, 136, 72, None), (90, 3, 4, 33, 47, None), (60, 8, 40, 264, 520, 32),
+                                               (700, 2, 6, 1288, 200, 64), (500, 4, 6, 1032, 776, 128), (2000, 2, 5, 520, 264, 256),
+                                               (3300, 2, 8, 264, 4104, None), (20, 9, 12, 40, 24, 16)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gradient_by_tokens_rounds_once(T, k, E, K, N, block_m, dtype):
+    """The sum over a token's slots is held in fp32: one half step of the result, as
+    if each token had one sum of k N products."""
+    from td_benchmark_amd import ops
+    x, w, ids, dy = make(T, k, E, K, N, dtype, drop=0.1)
+    slots = ops.ExpertSlots(ids, E, block_m)
+    (_, dx, _), (_, mx, _) = products64(x, w, ids, dy)
+    got = ops.grouped_mm_dgrad(dy, w, slots, by_token=True)
+    assert got.dtype == dtype and off(got, by_token(dx, k), by_token(mx, k), N + k) <= 0
+    xg = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.grouped_mm(xg, w, slots), xg, dy)[0], got)

@@ -111,7 +111,7 @@ def test_c_entries_refuse(L):
                      (topk, dict(k=0)), (experts, dict(e=0)), (block, dict(bm=48)), (ok, dict(S=0)), (ok, dict(N=0))):
         assert mm(**kw) == want, kw
     dg = lambda dy=p, w=p, S=8, N=24, K=16, e=3, bm=16, mp=48, dt=0, dx=p: L.moe_grouped_mm_dgrad(  # noqa: E731
-        dy, w, p, p, p, None, S, N, K, e, bm, mp, dt, dx, None)
+        dy, w, p, p, p, None, S, N, K, e, bm, mp, dt, 0, dx, None)
     for want, kw in ((null, dict(dy=None)), (null, dict(w=None)), (null, dict(dx=None)), (bad, dict(N=-1)), (bad, dict(dt=7)),
                      (bad, dict(dx=odd)), (experts, dict(e=-1)), (block, dict(bm=0)), (ok, dict(S=0)), (ok, dict(K=0))):
         assert dg(**kw) == want, kw
