@@ -375,7 +375,8 @@ int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64_t R, int64
  * vLLM's fused_moe use_int8_w8a8 with per_channel_quant.  dtype: MOE_BF16 or
  * MOE_FP16.  Sums are fp32 (int8: exact in 32-bit integers) and rounded once, to
  * nearest even.  Any sizes; rows of whole 16-byte chunks (16-byte aligned bases,
- * widths and strides of whole chunks) take the faster kernels. */
+ * widths and strides of whole chunks) take the faster kernels.  sorted_ids: in each
+ * block the slots come before the padding (ids >= S), as align writes them. */
 #define MOE_BF16 0
 #define MOE_FP16 1
 

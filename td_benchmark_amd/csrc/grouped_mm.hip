@@ -264,6 +264,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) sum = sum + part[w][r][l];
     const int slot = smSlot[row];
+    if (slot < 0) return;  // padding before a slot, which align never writes
     float f[4];
     if constexpr (EB == 1) {
       const float sa = none ? 0.0f : g.As[g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot)];

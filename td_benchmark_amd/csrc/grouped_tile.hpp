@@ -1,19 +1,19 @@
 // The LDS-tiled kernel of the grouped products (grouped_mm.hip): operands whose
 // rows are whole, aligned 16-byte chunks.
 //
-// A workgroup computes TM x TN outputs.  An operand is staged by
-// rows, R rows of 128 bytes of the contraction, where it is contiguous along the
-// contraction (the product's x and w, the int8 operands, dy by rows), or by
-// columns, 64 contraction rows of R columns, where it is contiguous along the
-// output (w in the gradient by rows, dy and x in the gradient by weights).  Both
-// take R * 128 bytes of a stage and are filled by direct-to-LDS loads, 16 bytes a
-// lane from the lane's own address, so rows are gathered for nothing.  Fragments
-// of a row-staged operand are one ds_read_b128; of a column-staged one two
+// A workgroup computes TM x TN outputs.  An operand is staged by rows, R rows of
+// 128 bytes of the contraction, where it is contiguous along the contraction (the
+// product's x and w, the int8 operands, dy by rows), or by columns, 64 contraction
+// rows of R columns, where it is contiguous along the output (w in the gradient by
+// rows; dy and x in the gradient by weights, in steps of 32).  Both take R * 128
+// (64) bytes of a stage and are filled by direct-to-LDS loads, 16 bytes a lane from
+// the lane's own address, so rows are gathered for nothing.  Fragments of a
+// row-staged operand are one ds_read_b128; of a column-staged one two
 // ds_read_b64_tr_b16, which hand each lane four consecutive contraction values of
 // its column.
 //
 // LDS rows hold their 16-byte chunks at index XOR a function of the row
-// (slot_of; col_swz), applied on the global side, so that the lanes read
+// (row_place; col_swz), applied on the global side, so that the lanes read
 // together fall into distinct banks.
 #pragma once
 
@@ -528,8 +528,9 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
           const int row = (i * 64 + lane) / CPR, cc = (i * 64 + lane) % CPR;
           const int64_t jj = j0 + col_base + 4 * cc;
           const v4f v = part[row * CPR + (cc ^ (row & (CPR - 1) & 15))];
-          if (row_base + r * 16 + row < nvalid && jj < g.J)
-            *reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + (int64_t)smSlot[row_base + r * 16 + row] * g.ldc + jj) = v;
+          const int slot = row_base + r * 16 + row < nvalid ? smSlot[row_base + r * 16 + row] : -1;
+          if (slot >= 0 && jj < g.J)
+            *reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + (int64_t)slot * g.ldc + jj) = v;
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
@@ -562,6 +563,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     const int64_t j = j0 + cc * 8;
     if (j >= g.J) continue;
     const int64_t orow = FORM == kWgrad ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
+    if (FORM != kWgrad && orow < 0) continue;  // padding before a slot, which align never writes
     const v4i v = *reinterpret_cast<const v4i*>(out + row * TN + ((cc ^ (row & ROT)) << 3));
     v4i* const to = reinterpret_cast<v4i*>(g.C + (orow * g.ldc + j) * 2);
     // nothing reads the weights' gradient soon: past the L2 it takes 3-5 % less
@@ -635,8 +637,9 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     if (e < 0 || e >= g.E) {  // no expert: zero rows
       for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
         const int64_t jj = j0 + c % (TN / 8) * 8;
-        if (jj >= g.J) continue;
-        const int64_t at = (int64_t)smSlot[c / (TN / 8)] * g.ldc + jj;
+        const int slot = smSlot[c / (TN / 8)];
+        if (jj >= g.J || slot < 0) continue;
+        const int64_t at = (int64_t)slot * g.ldc + jj;
         if (FORM == kDgrad && g.out32) {
           v4f* to = reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + at);
           to[0] = to[1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
