@@ -285,16 +285,25 @@ __global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__
 template <bool FP16>
 static int slot_sum(const float* d, int64_t T, int32_t k, int64_t H, uint16_t* y, hipStream_t st) {
   const bool vec = H % 4 == 0 && aligned16(d) && ((uintptr_t)y & 7) == 0;
-  const int64_t blocks = (T * (vec ? H / 4 : H) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return kErrBadShape;
-  const dim3 grid((unsigned)blocks), threads(256);
-  if (!vec)
-    hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, d, T, (int)k, H, y);
-  else if (k <= 8)
-    hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, d, T, (int)k, H, y);
-  else
-    hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, d, T, (int)k, H, y);
-  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+  // a launch has fewer than 2^32 threads: the tokens in parts of up to 2^31 of them
+  const int64_t per_t = vec ? H / 4 : H;
+  if (per_t > 0x7FFFFFFF) return kErrBadShape;
+  const int64_t part = (((int64_t)1 << 31) - 1) / per_t;
+  const dim3 threads(256);
+  for (int64_t t = 0; t < T; t += part) {
+    const int64_t n = T - t < part ? T - t : part;
+    const dim3 grid((unsigned)((n * per_t + 255) / 256));
+    const float* dt = d + t * k * H;
+    uint16_t* yt = y + t * H;
+    if (!vec)
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+    else if (k <= 8)
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+    else
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+    if (hipGetLastError() != hipSuccess) return kErrLaunch;
+  }
+  return kOk;
 }
 
 }  // namespace moe

@@ -339,6 +339,15 @@ extern "C" int moe_quant_int8(const void* x, int64_t ldx, int64_t T, int64_t H, 
   if (!scales || (H > 0 && (!x || !q))) return kErrNullPointer;
   if (((uintptr_t)x & 1) != 0 || ((uintptr_t)scales & 3) != 0) return kErrBadShape;
   hipStream_t st = (hipStream_t)stream;
-  return dtype == MOE_FP16 ? quant_int8<true>((const uint16_t*)x, ldx, T, H, (uint8_t*)q, scales, st)
-                           : quant_int8<false>((const uint16_t*)x, ldx, T, H, (uint8_t*)q, scales, st);
+  // a launch has fewer than 2^32 threads, and a row takes up to 256
+  constexpr int64_t kRows = (int64_t)1 << 23;
+  int rc = kOk;
+  for (int64_t t = 0; t < T && rc == kOk; t += kRows) {
+    const int64_t n = T - t < kRows ? T - t : kRows;
+    const auto xt = (const uint16_t*)x + t * ldx;
+    const auto qt = (uint8_t*)q + t * H;
+    rc = dtype == MOE_FP16 ? quant_int8<true>(xt, ldx, n, H, qt, scales + t, st)
+                           : quant_int8<false>(xt, ldx, n, H, qt, scales + t, st);
+  }
+  return rc;
 }

@@ -34,3 +34,22 @@ def test_padding_before_a_slot_writes_nothing_else(BM, K, N, experts_here):
     assert (whole[:4] == 7).all() and (whole[4 + S:] == 7).all()
     want = (a[3:].double() @ b[1].double().t()).to(BF16)
     assert torch.equal(y[3:], want)
+
+
+def test_quant_of_more_rows_than_a_launch_has():
+    from td_benchmark_amd import ops
+    T, H = (1 << 24) + 5, 3
+    x = torch.empty((T, H), dtype=BF16, device="cuda").random_(-127, 128)
+    x[:, 1] = 127.0
+    q, s = ops.per_token_quant_int8(x)
+    assert bool((s == 1.0).all()) and torch.equal(q.to(BF16), x)
+
+
+def test_slot_sum_of_more_columns_than_a_launch_has():
+    from td_benchmark_amd import _lib
+    T, H = (1 << 31) // 5 + 11, 5
+    d = torch.empty((T, H), dtype=torch.float32, device="cuda").random_(-127, 128)
+    y = torch.full((T, H), 0.5, dtype=BF16, device="cuda")
+    assert _lib.lib().moe_slot_sum(d.data_ptr(), T, 1, H, 0, y.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    for t in range(0, T, 1 << 26):  # whole numbers below 2^8 are exact
+        assert torch.equal(y[t:t + (1 << 26)].float(), d[t:t + (1 << 26)])
