@@ -1545,7 +1545,11 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Te
     product) or [S, K] for each slot (the second); rows may be strided.  w [E, N,
     K] contiguous.  Slots without an expert get zero rows and add nothing to the
     gradients.  Equal inputs give equal bits.  The gradients are once
-    differentiable; see grouped_mm_dgrad and grouped_mm_wgrad."""
+    differentiable; see grouped_mm_dgrad and grouped_mm_wgrad, which are also what
+    to capture into a HIP graph (or torch.autograd.grad): a captured ``backward()``
+    ends in torch's own accumulation nodes, which wait for the stream they were
+    made on while an eager graph of the same leaves is alive, and that breaks the
+    capture."""
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMM.apply(x, w, slots)
     return _grouped_product(x, w, slots)
