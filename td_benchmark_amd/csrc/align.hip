@@ -252,9 +252,11 @@ MOE_DEVICE int32_t local_slots(const int32_t* ids, const int32_t* expert_map, in
 constexpr int kAlignThreads = 512;
 constexpr int kAlignWaves = kAlignThreads / 64;
 
-// IT: ids a lane holds (IT * 512 >= S).
-template <int IT>
-MOE_DEVICE void align_expert(const AlignArgs& a, int e) {
+// IT: ids a lane holds (IT * 512 >= S).  SLOTS: the ids are of type ID, those
+// outside [0, E - 1) belong to the last expert; slot_ids gets each slot's, and
+// table the experts' first positions and counts.
+template <int IT, class ID = int32_t, bool SLOTS = false>
+MOE_DEVICE void align_expert(const AlignArgs& a, int e, int32_t* slot_ids = nullptr, int32_t* table = nullptr) {
   constexpr int COPIES = IT > 2 ? 8 : 1;
   __shared__ __attribute__((aligned(16))) int32_t hist[kAlignMaxExperts * COPIES];
   auto count_of = [&](int x) {
@@ -275,7 +277,14 @@ MOE_DEVICE void align_expert(const AlignArgs& a, int e) {
   const int first = wave * IT * 64 + lane;
   int id[IT];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) id[i] = first + 64 * i < a.S ? a.ids[first + 64 * i] : -1;
+  for (int i = 0; i < IT; ++i) {
+    if constexpr (SLOTS) {
+      const ID x = first + 64 * i < a.S ? reinterpret_cast<const ID*>(a.ids)[first + 64 * i] : (ID)0;
+      id[i] = first + 64 * i >= a.S ? -1 : x >= 0 && x < a.E - 1 ? (int)x : a.E - 1;
+    } else {
+      id[i] = first + 64 * i < a.S ? a.ids[first + 64 * i] : -1;
+    }
+  }
   for (int i = tid; i < a.E * COPIES; i += kAlignThreads) hist[i] = 0;
   __syncthreads();
   int mine = 0;  // this wave's slots of expert e
@@ -338,7 +347,10 @@ MOE_DEVICE void align_expert(const AlignArgs& a, int e) {
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const uint64_t m = __ballot(id[i] == e);
-    if (id[i] == e) a.sorted[before + rank + __popcll(m & lt)] = first + 64 * i;
+    if (id[i] == e) {
+      a.sorted[before + rank + __popcll(m & lt)] = first + 64 * i;
+      if constexpr (SLOTS) slot_ids[first + 64 * i] = e;
+    }
     rank += __popcll(m);
   }
   for (int i = cnt + tid; i < padded; i += kAlignThreads) a.sorted[before + i] = a.S;
@@ -364,6 +376,13 @@ MOE_DEVICE void align_expert(const AlignArgs& a, int e) {
     reinterpret_cast<v4i*>(a.runs + 4)[place] = (v4i){before, cnt, local, padded};
   if (a.share && e == 0 && tid < kShareTiles) a.share[tid] = 0;
   if (a.share2 && e == 0 && tid < kShareTiles) a.share2[tid] = 0;
+  if constexpr (SLOTS) {
+    if (tid == 0) {
+      table[e] = before;
+      table[a.E + 1 + e] = cnt;
+      if (e == 0) table[a.E] = total;
+    }
+  }
   if (e == 0 && tid == 0) {
     *a.ntpp = total;
     if (a.local) *a.local = ltotal;
@@ -658,43 +677,12 @@ __global__ __launch_bounds__(256) void slot_ids_kernel(const ID* __restrict__ id
   out[s] = id >= 0 && id < E ? (int32_t)id : E;
 }
 
-// The same in one workgroup, which also counts: off [E + 2] the experts' first
-// sorted positions (runs padded to BM) and cnt [E + 1] their slots, where align's
-// three launches leave them too.  Up to 16384 slots, where align itself is one
-// launch that keeps no counts; a launch of its own for them would cost 2 us.
-template <class ID>
-__global__ __launch_bounds__(kAlignMaxExperts) void slot_ids_table_kernel(const ID* __restrict__ ids, int S, int E,
-                                                                          int BM, int32_t* __restrict__ out,
-                                                                          int32_t* __restrict__ off,
-                                                                          int32_t* __restrict__ cnt) {
-  __shared__ int32_t hist[kAlignMaxExperts];
-  __shared__ int32_t wave_tot[kAlignMaxExperts / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  hist[tid] = 0;
-  __syncthreads();
-  for (int s = tid; s < S; s += kAlignMaxExperts) {
-    const ID id = ids[s];
-    const int e = id >= 0 && id < E ? (int)id : E;
-    out[s] = e;
-    atomicAdd(&hist[e], 1);
-  }
-  __syncthreads();
-  const int c = hist[tid];
-  const int padded = (c + BM - 1) / BM * BM;
-  int incl = padded;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 63) wave_tot[wave] = incl;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) incl += wave_tot[w];
-  if (tid <= E) {
-    off[tid] = incl - padded;
-    cnt[tid] = c;
-  }
-  if (tid == E) off[E + 1] = incl;
+// Up to 16384 slots all of it in align's one launch (8 slots of 128 experts: 4.1 us,
+// 2.6 and 4.0 with a launch of its own before it).
+template <int IT, class ID>
+__global__ __launch_bounds__(kAlignThreads) void expert_slots_kernel(AlignArgs a, int32_t* __restrict__ slot_ids,
+                                                                     int32_t* __restrict__ table) {
+  align_expert<IT, ID, true>(a, blockIdx.x, slot_ids, table);
 }
 
 }  // namespace moe
@@ -717,23 +705,24 @@ extern "C" int moe_expert_slots(const void* topk_ids, int32_t id_bytes, int64_t 
   const int rc = align_args(slot_ids, S, E + 1, BM, sorted_ids, expert_ids, ntpp, max_padded, true, workspace);
   if (rc != kOk) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const auto ids64 = (const int64_t*)topk_ids;
-  const auto ids32 = (const int32_t*)topk_ids;
   if (align_one_launch(S, E + 1, nullptr)) {
-    int32_t* off = (int32_t*)workspace + slot_table_at(S, E);
-    int32_t* cnt = off + E + 2;
-    if (id_bytes == 8)
-      hipLaunchKernelGGL(slot_ids_table_kernel<int64_t>, dim3(1), dim3(kAlignMaxExperts), 0, st, ids64, (int)S, (int)E,
-                         (int)BM, slot_ids, off, cnt);
-    else
-      hipLaunchKernelGGL(slot_ids_table_kernel<int32_t>, dim3(1), dim3(kAlignMaxExperts), 0, st, ids32, (int)S, (int)E,
-                         (int)BM, slot_ids, off, cnt);
-  } else {
-    const dim3 grid((unsigned)((S + 255) / 256));
-    if (id_bytes == 8)
-      hipLaunchKernelGGL(slot_ids_kernel<int64_t>, grid, dim3(256), 0, st, ids64, S, (int)E, slot_ids);
-    else
-      hipLaunchKernelGGL(slot_ids_kernel<int32_t>, grid, dim3(256), 0, st, ids32, S, (int)E, slot_ids);
+    const AlignArgs a{(const int32_t*)topk_ids, nullptr, sorted_ids, expert_ids, ntpp, nullptr, nullptr, nullptr, nullptr,
+                      (int)max_padded, (int)S, 1, (uint16_t)(E + 1), (uint16_t)BM};
+    int32_t* table = (int32_t*)workspace + slot_table_at(S, E);
+    by_slots(S, [&](auto it) {
+      constexpr int IT = decltype(it)::value;
+      const dim3 grid((unsigned)E + 1), threads(kAlignThreads);
+      if (id_bytes == 8)
+        hipLaunchKernelGGL((expert_slots_kernel<IT, int64_t>), grid, threads, 0, st, a, slot_ids, table);
+      else
+        hipLaunchKernelGGL((expert_slots_kernel<IT, int32_t>), grid, threads, 0, st, a, slot_ids, table);
+    });
+    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
   }
+  const dim3 grid((unsigned)((S + 255) / 256));
+  if (id_bytes == 8)
+    hipLaunchKernelGGL(slot_ids_kernel<int64_t>, grid, dim3(256), 0, st, (const int64_t*)topk_ids, S, (int)E, slot_ids);
+  else
+    hipLaunchKernelGGL(slot_ids_kernel<int32_t>, grid, dim3(256), 0, st, (const int32_t*)topk_ids, S, (int)E, slot_ids);
   return align_impl(slot_ids, S, E + 1, BM, nullptr, sorted_ids, expert_ids, ntpp, max_padded, workspace, stream);
 }
