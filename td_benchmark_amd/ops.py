@@ -1312,12 +1312,13 @@ def _need_here(names: str, *tensors: torch.Tensor | None) -> None:
     """The tensors (``names`` by spaces) are on the current device, whose current
     stream the launch goes to: a pointer of another device would be read through
     the wrong one."""
-    here = tensors[0].get_device()  # -1: not a GPU tensor
+    here = _current_device() if tensors[0].is_cuda else -1
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            here = -1
-    if here >= 0 and here == _current_device():
-        return
+        if t is not None and t.get_device() != here:  # -1: not a GPU tensor
+            break
+    else:
+        if here >= 0:
+            return
     for name, t in zip(names.split(), tensors):
         if t is not None and not t.is_cuda:
             raise ValueError(f"{name} must be a GPU tensor")
@@ -1328,9 +1329,9 @@ def _need_here(names: str, *tensors: torch.Tensor | None) -> None:
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous."""
-    rows, cols = t.shape
     if t.is_contiguous():
-        return cols
+        return t.size(1)
+    rows, cols = t.shape
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     if rows <= 1 or cols == 0:
@@ -1448,7 +1449,7 @@ def _grouped_operands(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> i
 def _grouped_product(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
     k = _grouped_operands(x, w, slots)
     E, N, K = w.shape
-    y = torch.empty((slots.S, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((slots.S, N))
     check(lib().moe_grouped_mm(x.data_ptr(), _row_stride(x, "x"), w.data_ptr(), *slots._at, slots.S, k, N, K, E,
                                slots.block_size_m, slots.max_padded, _DTYPE_CODE[x.dtype], y.data_ptr(),
                                _stream_handle()), "moe_grouped_mm")
@@ -1572,13 +1573,20 @@ def per_token_quant_int8(x: torch.Tensor, out_q: torch.Tensor | None = None,
         raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
     if x.dtype not in _DTYPE_CODE:
         raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _need_here("x out_q out_s", x, out_q, out_s)
     T, H = x.shape
-    q = torch.empty((T, H), dtype=torch.int8, device=x.device) if out_q is None else out_q
-    s = torch.empty((T, 1), dtype=torch.float32, device=x.device) if out_s is None else out_s
-    if out_q is not None:
+    if out_q is None and out_s is None:
+        _need_here("x", x)
+    else:
+        _need_here("x out_q out_s", x, out_q, out_s)
+    if out_q is None:
+        q = x.new_empty((T, H), dtype=torch.int8)
+    else:
+        q = out_q
         _need(q, "out_q", torch.int8, (T, H), anywhere=True)
-    if out_s is not None:
+    if out_s is None:
+        s = x.new_empty((T, 1), dtype=torch.float32)
+    else:
+        s = out_s
         _need(s, "out_s", torch.float32, (T, 1), anywhere=True)
     check(lib().moe_quant_int8(x.data_ptr(), _row_stride(x, "x"), T, H, _DTYPE_CODE[x.dtype], q.data_ptr(),
                                s.data_ptr(), _stream_handle()), "moe_quant_int8")
@@ -1586,9 +1594,10 @@ def per_token_quant_int8(x: torch.Tensor, out_q: torch.Tensor | None = None,
 
 
 def _need_scales(t: torch.Tensor, name: str, n: int) -> None:
+    if t.dtype == torch.float32 and t.numel() == n and t.is_contiguous():
+        return
     _need(t, name, torch.float32, anywhere=True)
-    if t.numel() != n:
-        raise ValueError(f"{name} must hold {n} scales, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must hold {n} scales, got {tuple(t.shape)}")
 
 
 def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
@@ -1599,13 +1608,12 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
     ([M] or [M, 1] fp32) and each row of b ([N] or [N, 1]).  The integer sums are
     exact (K <= 131071), the rest is fp32, rounded once.  Rows of a, b and ``out``
     may be strided; bias [N] in out_dtype."""
-    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+    if a.dim() != 2 or b.dim() != 2 or a.size(1) != b.size(1):
         raise ValueError(f"a must be [M, K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
-    for t, name in ((a, "a"), (b, "b")):
-        if t.dtype != torch.int8:
-            raise TypeError(f"{name} must be torch.int8, got {t.dtype}")
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise TypeError(f"a and b must be torch.int8, got {a.dtype} and {b.dtype}")
     M, K = a.shape
-    N = b.shape[0]
+    N = b.size(0)
     if K > INT8_MAX_K:
         raise ValueError(f"K must be at most {INT8_MAX_K}, got {K}")
     out_dtype = out.dtype if out is not None else out_dtype
@@ -1615,14 +1623,17 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
     _need_scales(b_scale, "b_scale", N)
     if bias is not None:
         _need(bias, "bias", out_dtype, (N,), anywhere=True)
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-    elif tuple(out.shape) != (M, N):
+    if out is not None and tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
     _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
+    if out is None:
+        out = a.new_empty((M, N), dtype=out_dtype)
+        ldy = N
+    else:
+        ldy = _row_stride(out, "out")
     check(lib().moe_int8_scaled_mm(a.data_ptr(), _row_stride(a, "a"), a_scale.data_ptr(), b.data_ptr(),
                                    _row_stride(b, "b"), b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                                   M, N, K, _DTYPE_CODE[out_dtype], out.data_ptr(), _row_stride(out, "out"),
+                                   M, N, K, _DTYPE_CODE[out_dtype], out.data_ptr(), ldy,
                                    _stream_handle()), "moe_int8_scaled_mm")
     return out
 
