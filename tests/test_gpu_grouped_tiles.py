@@ -91,6 +91,23 @@ def test_int8_tiles(M, N, K):
     assert off_int8(ops.int8_scaled_mm(a, b, sa, sb, bias), want, bias.double().abs()) <= 0
 
 
+@pytest.mark.parametrize("M,N,K", [(100, 408, 2064), (100, 408, 592), (511, 520, 656), (513, 512, 656), (1463, 168, 1072),
+                                   (255, 4104, 272), (256, 4096, 272), (200, 8200, 144), (1025, 1016, 144), (33, 72, 144),
+                                   (4097, 8, 48)])
+def test_int8_rows_of_a_tile(M, N, K):
+    """Dense products whose tiles have fewer rows than there are."""
+    from td_benchmark_amd import ops
+    g = torch.Generator().manual_seed(M * N + K)
+    a = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8).cuda()
+    b = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8).cuda()
+    sa, sb = (torch.rand(M, generator=g) * 1e-2).cuda(), (torch.rand(N, generator=g) * 1e-2).cuda()
+    want = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double()
+    y = torch.full((M + 2, N), 7.0, dtype=BF16, device="cuda")
+    ops.int8_scaled_mm(a, b, sa, sb, out=y[1:-1])
+    assert off_int8(y[1:-1], want) <= 0
+    assert (y[0] == 7).all() and (y[-1] == 7).all()
+
+
 def test_int8_forms_give_equal_bits():
     """The sums are exact and every form rounds alike: the result depends on neither
     the block size nor the alignment."""
