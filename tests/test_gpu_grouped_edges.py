@@ -53,3 +53,71 @@ def test_slot_sum_of_more_columns_than_a_launch_has():
     assert _lib.lib().moe_slot_sum(d.data_ptr(), T, 1, H, 0, y.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
     for t in range(0, T, 1 << 26):  # whole numbers below 2^8 are exact
         assert torch.equal(y[t:t + (1 << 26)].float(), d[t:t + (1 << 26)])
+
+
+@pytest.mark.parametrize("S,E", [(1, 1), (7, 3), (1024, 9), (1025, 2), (4096, 64), (8192, 5), (8193, 7), (16384, 40), (16385, 40)])
+def test_slots_in_order(S, E):
+    """The sorted positions are each expert's slots in ascending order, then padding;
+    ids outside the experts come last, those past 32 bits among them."""
+    from td_benchmark_amd import ops
+    g = torch.Generator().manual_seed(S)
+    ids = torch.randint(-1, E + 1, (S, 1), generator=g)
+    ids[::5] += 1 << 32
+    ids[1::11] -= 1 << 33
+    slots = ops.ExpertSlots(ids.cuda(), E, 64)
+    want = []
+    for e in range(E + 1):
+        at = ((ids.view(-1) == e) if e < E else (ids.view(-1) < 0) | (ids.view(-1) >= E)).nonzero().view(-1).tolist()
+        want += at + [S] * (-len(at) % 64)
+    n = int(slots.ntpp.item())
+    assert n == len(want) and slots.sorted_ids[:n].tolist() == want
+    assert slots._part(0, S).tolist() == [i if 0 <= i < E else E for i in ids.view(-1).tolist()]
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_ids_by_columns_and_an_expert_twice(dtype):
+    from grouped_cases import make, off, products64
+    from td_benchmark_amd import ops
+    T, k, E, K, N = 150, 3, 4, 264, 136
+    x, w, ids, dy = make(T, k, E, K, N, BF16)
+    ids[:, 2] = ids[:, 0]  # a token twice on one expert
+    by_column = torch.empty((k, T), dtype=dtype, device="cuda").t()
+    by_column.copy_(ids)
+    assert not by_column.is_contiguous()
+    slots = ops.ExpertSlots(by_column, E)
+    (y, dx, dw), (my, mx, mw) = products64(x, w, ids, dy)
+    assert off(ops.grouped_mm(x, w, slots), y, my, K) <= 0
+    assert off(ops.grouped_mm_dgrad(dy, w, slots), dx, mx, N) <= 0
+    assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, T * k) <= 0
+    assert off(ops.grouped_mm_dgrad(dy, w, slots, by_token=True), dx.view(T, k, K).sum(1), mx.view(T, k, K).sum(1),
+               N + k) <= 0
+
+
+def test_two_captured_graphs_in_turn():
+    """Two graphs of one process share no workspace: each replay gives its own inputs' result."""
+    from grouped_cases import make
+    from td_benchmark_amd import ops
+    E, K, N = 6, 136, 264
+    cases, graphs = [], []
+    for i, T in enumerate((70, 190)):
+        x, w, ids, dy = make(T, 2, E, K, N, BF16, seed=i)
+
+        def step(x=x, w=w, ids=ids, dy=dy):
+            slots = ops.ExpertSlots(ids, E)
+            return ops.grouped_mm(x, w, slots), ops.grouped_mm_dgrad(dy, w, slots, by_token=True), ops.grouped_mm_wgrad(dy, x, slots)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        cases.append((step, ids, out))
+        graphs.append(graph)
+    for r in range(3):
+        for i in (0, 1):
+            cases[i][1].copy_(cases[i][1].roll(1 + r, 0))
+            graphs[i].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for step, _, out in cases:
+            for a, b in zip(out, step()):
+                assert torch.equal(a, b)
