@@ -480,10 +480,24 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
   hipStream_t st = (hipStream_t)stream;
   if (S > 0 && chunks(dy, N, 2) && chunks(x, ldx, 2) && chunks(dw, K, 2) &&
       N < (1 << 30) && ldx < (1 << 30)) {
-    // Steps of 32 slots in a ring of four: rows of a column-staged step are whole
-    // lines at any length, so the finer ring costs nothing (256 slots an expert of
-    // 128: 381 us, 403 with steps of 64 in a ring of two; 1024 of 8 even).  The rows
+    // Steps of 32 slots in rings of three or four: rows of a column-staged step are
+    // whole lines at any length, so the finer ring costs nothing (256 slots an expert
+    // of 128: 381 us, 403 with steps of 64 in a ring of two; 1024 of 8 even).  The rows
     // forms lose with it, whose row-staged lines it reads in halves.
+    //
+    // Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
+    // sums, where runs are short and most of the time is the gradient's own bytes, or
+    // fill a chip that the square tiles leave half empty.  They read half as much
+    // again: longer runs lose, with many experts sooner, whose operands few tiles share
+    // (us, 256 and 128 rows; 8 experts of 14336 x 4096: 16 slots 183 and 161; 16 of 1536
+    // x 2048: 100 slots 39 and 37, 1000 slots 113 and 124; 128 of 2048 x 1536: 16 slots
+    // 193 and 177, 96 slots 261 and 286; 8 of 256 x 1024, 32 square tiles: 1000 slots 37
+    // and 31).
+    const int64_t square = E * ((N + 255) / 256) * ((K + 255) / 256);
+    if (S <= (E <= 32 ? 100 : 32) * (int64_t)E || square <= 128) {
+      using T = MmTile<128, 256, 4, 2, 3, 2, 64>;
+      return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
+    }
     using T = MmTile<256, 256, 8, 4, 4, 1, 64>;
     return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
   }

@@ -247,7 +247,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
   constexpr int STEP = SB / EB;  // contraction elements of a step
   static_assert(EB == 2 || FORM == kProduct, "transposing reads are of 16-bit values");
-  static_assert(FORM != kWgrad || (KS <= 4 && TM == TN && 8 * STEP * 4 <= K::TABLE), "the ring of slots");
+  static_assert(FORM != kWgrad || (KS <= 4 && 8 * STEP * 4 <= K::TABLE), "the ring of slots");
   static_assert(T::THREADS == K::THREADS && T::LDS_BYTES <= K::LDS_BYTES && T::TABLE <= K::TABLE, "a part of the launch's tile");
   const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
   const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
@@ -300,12 +300,16 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
   const int a_rows = KS == 2 ? (nvalid + 15) / 16 * 16 : TM;
 
-  // kWgrad: the slots of this lane's rows of a step, read ahead of its loads
-  uint32_t slot_r[T::NA_W];
+  // kWgrad: the slots of this lane's rows of a step, read ahead of its loads; square
+  // tiles place both operands alike
+  uint32_t slot_a[T::NA_W], slot_b[T::NB_W];
   auto read_slots = [&](int kk) {
 #pragma unroll
     for (int i = 0; i < T::NA_W; ++i)
-      slot_r[i] = (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, ACPR)];
+      slot_a[i] = (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, ACPR)];
+#pragma unroll
+    for (int i = 0; i < T::NB_W; ++i)
+      slot_b[i] = TM == TN ? slot_a[i < T::NA_W ? i : 0] : (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, BCPR)];
   };
 
   // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
@@ -324,8 +328,8 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     const int gi = wave + T::NW * i;
     if constexpr (FORM == kWgrad) {
       const uint8_t* p;
-      if constexpr (is_b) p = b_ptr[i] + (uint64_t)slot_row(g, slot_r[i]) * (uint32_t)(g.sbc * EB);
-      else p = a_ptr[i] + (uint64_t)slot_r[i] * (uint32_t)(g.lda * EB);
+      if constexpr (is_b) p = b_ptr[i] + (uint64_t)slot_row(g, slot_b[i]) * (uint32_t)(g.sbc * EB);
+      else p = a_ptr[i] + (uint64_t)slot_a[i] * (uint32_t)(g.lda * EB);
       if constexpr (first) p = col_row(gi, is_b ? BCPR : ACPR) < left ? p : zeros;
       if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
         lds_load16(p, dst + (is_b ? T::A_BYTES : 0) + gi * 1024);

@@ -71,6 +71,20 @@ def test_weights_gradient_lengths(rows):
         assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, rows) <= 0
 
 
+@pytest.mark.parametrize("rows", [1, 31, 33, 64, 97, 128, 129, 225, 300])
+def test_weights_gradient_lengths_among_many_long_experts(rows):
+    """The same where the tiles are square: more than 32 experts of more than 32 slots on average."""
+    from td_benchmark_amd import ops
+    K, N, E, S = 264, 280, 33, 1100 + rows
+    x, w, _, dy = make(S, 1, E, K, N, BF16)
+    ids = torch.full((S, 1), 5, dtype=torch.int64, device="cuda")
+    ids[torch.randperm(S, generator=torch.Generator().manual_seed(rows))[:rows]] = 7
+    for block_m in (16, 256):
+        slots = ops.ExpertSlots(ids, E, block_m)
+        (_, _, dw), (_, _, mw) = products64(x, w, ids, dy)
+        assert off(ops.grouped_mm_wgrad(dy, x, slots), dw, mw, S) <= 0
+
+
 @pytest.mark.parametrize("K", [8, 56, 64, 72, 120, 128, 136, 192, 200, 256, 264, 320, 392, 456, 520])
 @pytest.mark.parametrize("block_m", [16, 32, 64, 128, 256])
 def test_contraction_lengths(K, block_m):

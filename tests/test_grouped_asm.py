@@ -66,3 +66,11 @@ def test_tall_tiles_run_two_waves_a_simd(asm):
     assert len(tall) >= 8
     for name, body in tall:
         assert int(re.search(r"next_free_vgpr (\d+)", body).group(1)) <= 256, name
+
+
+def test_two_workgroups_of_the_weights_gradient_share_a_cu(asm):
+    found = [(n, b) for n, b in re.findall(r"\.amdhsa_kernel (\S+)(.*?)\.end_amdhsa_kernel", asm, flags=re.S)
+             if "tile_mm_kernel" in n and "ILi128ELi256ELi4E" in n]
+    assert len(found) == 2
+    for name, body in found:
+        assert int(re.search(r"next_free_vgpr (\d+)", body).group(1)) <= 256, name
