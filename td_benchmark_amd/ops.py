@@ -14,6 +14,7 @@ import functools
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import MoeLayer, check, lib
 
@@ -1327,6 +1328,15 @@ def _need_here(names: str, *tensors: torch.Tensor | None) -> None:
             raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
 
 
+def _no_tangent(a: torch.Tensor, b: torch.Tensor) -> None:
+    """Forward-mode derivatives are not implemented: a result without a tangent
+    would count as one with a derivative of zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open: no tensor has one (0.1 us, 0.6 by unpacking)
+        return
+    if forward_ad.unpack_dual(a).tangent is not None or forward_ad.unpack_dual(b).tangent is not None:
+        raise NotImplementedError("the grouped products have no forward-mode derivative")
+
+
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous."""
     if t.is_contiguous():
@@ -1483,7 +1493,9 @@ def _wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tenso
 
 def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_token: bool = False) -> torch.Tensor:
     """The gradient of ``grouped_mm`` by its rows: dx[s] = dy[s] @ w[e(s)], [S, K].
-    ``by_token``: summed over each token's slots in fp32 and rounded once, [T, K]."""
+    ``by_token``: summed over each token's slots in fp32 and rounded once, [T, K].
+    The call itself is not differentiable."""
+    _no_tangent(dy, w)
     if dy.dim() != 2 or w.dim() != 3:
         raise ValueError(f"dy must be [S, N] and w [E, N, K], got {tuple(dy.shape)} and {tuple(w.shape)}")
     if dy.dtype not in _DTYPE_CODE:
@@ -1501,7 +1513,8 @@ def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> t
     """The gradient of ``grouped_mm`` by its weights: dw[e] = sum over the slots s
     of e of dy[s]^T x[row(s)], [E, N, K] in dy's type; zeros for experts without
     slots.  Each value is one fp32 sum in slot order, so equal inputs give equal
-    bits."""
+    bits.  The call itself is not differentiable."""
+    _no_tangent(dy, x)
     if dy.dim() != 2 or x.dim() != 2:
         raise ValueError(f"dy must be [S, N] and x [rows, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
     if dy.dtype not in _DTYPE_CODE:
@@ -1529,6 +1542,7 @@ class _GroupedMM(torch.autograd.Function):
     def backward(ctx: Any, dy: torch.Tensor):
         x, w = ctx.saved_tensors
         slots = ctx.slots
+        _no_tangent(dy, dy)
         dy = dy.contiguous()  # a sum's gradient comes with stride 0
         dx = dw = None
         if ctx.needs_input_grad[0]:
@@ -1550,7 +1564,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Te
     to capture into a HIP graph (or torch.autograd.grad): a captured ``backward()``
     ends in torch's own accumulation nodes, which wait for the stream they were
     made on while an eager graph of the same leaves is alive, and that breaks the
-    capture."""
+    capture.  An operand with a forward-mode tangent raises NotImplementedError."""
+    _no_tangent(x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMM.apply(x, w, slots)
     return _grouped_product(x, w, slots)
