@@ -1377,20 +1377,30 @@ class ExpertSlots:
         if self.block_size_m not in SUPPORTED_BLOCK_M:
             raise ValueError(f"block_size_m must be one of {SUPPORTED_BLOCK_M}")
         _need_here("topk_ids", topk_ids)
-        self.device = topk_ids.device
         # slot ids, sorted ids, block experts, the positions' count and align's workspace in one allocation
         self.max_padded, table, self._sizes = _slots_layout(self.S, self.E, self.block_size_m)
-        self._buf = torch.empty(sum(self._sizes), dtype=torch.int32, device=self.device)
+        self._buf = torch.empty(sum(self._sizes), dtype=torch.int32, device=topk_ids.device)
         ids = topk_ids.contiguous()
-        at = self._buf.data_ptr()
-        at_sorted = at + 4 * self._sizes[0]
+        at_sorted = 4 * self._sizes[0]
         at_eids = at_sorted + 4 * self._sizes[1]
         at_ntpp = at_eids + 4 * self._sizes[2]
         at_work = at_ntpp + 4 * self._sizes[3]
-        self._at = (at_sorted, at_eids, at_ntpp, at_work + table)
+        self._offsets = (at_sorted, at_eids, at_ntpp, at_work + table)
+        at = self._buf.data_ptr()
         check(lib().moe_expert_slots(ids.data_ptr(), ids.element_size(), self.S, self.E, self.block_size_m, at,
-                                     at_sorted, at_eids, at_ntpp, self.max_padded, at_work,
+                                     at + at_sorted, at + at_eids, at + at_ntpp, self.max_padded, at + at_work,
                                      _stream_handle()), "moe_expert_slots")
+
+    @property
+    def _at(self) -> tuple[int, int, int, int]:
+        """Addresses of the sorted ids, the block experts, their count and the experts' table: always in the buffer
+        that this object has, so that a copy or an unpickled one reads its own."""
+        p, (a, b, c, d) = self._buf.data_ptr(), self._offsets
+        return p + a, p + b, p + c, p + d
+
+    @property
+    def device(self) -> torch.device:
+        return self._buf.device
 
     def _part(self, i: int, n: int) -> torch.Tensor:
         start = sum(self._sizes[:i])

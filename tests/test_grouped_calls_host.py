@@ -69,3 +69,48 @@ def test_plain_inputs_inside_a_dual_level(calls):
         assert ops.grouped_mm_dgrad(dy, w, Slots()).shape == (8, 16)
         assert ops.grouped_mm_wgrad(dy, x, Slots()).shape == (3, 24, 16)
     assert calls == ["moe_grouped_mm", "moe_grouped_mm_dgrad", "moe_grouped_mm_wgrad"]
+
+
+# ---------------------------------------------------------------- copies of the slots
+
+@pytest.fixture
+def native(monkeypatch):
+    """The arguments of the native calls that launch, none of which runs; sizes come from the library."""
+    from td_benchmark_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("native library not built")
+    real, seen = _lib.lib(), []
+
+    class Stub:
+        def __getattr__(self, name):
+            if name.endswith(("_bytes", "_table", "_max_padded")):
+                return getattr(real, name)
+            return lambda *args: seen.append((name, args)) or 0
+
+    monkeypatch.setattr(ops, "lib", Stub)
+    monkeypatch.setattr(ops, "_need_here", lambda *args: None)
+    monkeypatch.setattr(ops, "_stream_handle", lambda: 0)
+    return seen
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "copy"])
+def test_a_copy_reads_its_own_memory(native, how):
+    """Sorted ids, block experts, their count and the table come from the copy's buffer."""
+    import copy
+    import pickle
+    slots = ops.ExpertSlots(torch.tensor([[0, 2], [1, 0], [2, -1], [1, 2]], dtype=torch.int32), 3)
+    x, w, dy = _operands()
+    ops.grouped_mm(x, w, slots)
+    first = native[-1][1][3:7]
+    start = slots._buf.data_ptr()
+    new = {"deepcopy": copy.deepcopy, "pickle": lambda s: pickle.loads(pickle.dumps(s)), "copy": copy.copy}[how](slots)
+    assert (new._buf.data_ptr() == start) == (how == "copy")
+    assert (new.T, new.S, new.E, new.device) == (slots.T, slots.S, slots.E, slots.device)
+    del slots
+    for call, args, at in ((ops.grouped_mm, (x, w), 3), (ops.grouped_mm_dgrad, (dy, w), 2), (ops.grouped_mm_wgrad, (dy, x), 3)):
+        call(*args, new)
+        assert [p - new._buf.data_ptr() for p in native[-1][1][at:at + 4]] == [p - start for p in first], native[-1][0]
+    inside = range(new._buf.data_ptr(), new._buf.data_ptr() + 4 * new._buf.numel())
+    assert all(p in inside for p in native[-1][1][3:7])
+    assert new.sorted_ids.data_ptr() == native[-1][1][3] and new.expert_ids.data_ptr() == native[-1][1][4]
+    assert new.ntpp.data_ptr() == native[-1][1][5]
