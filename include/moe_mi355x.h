@@ -375,8 +375,9 @@ int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64_t R, int64
  * vLLM's fused_moe use_int8_w8a8 with per_channel_quant.  dtype: MOE_BF16 or
  * MOE_FP16.  Sums are fp32 (int8: exact in 32-bit integers) and rounded once, to
  * nearest even.  Any sizes; rows of whole 16-byte chunks (16-byte aligned bases,
- * widths and strides of whole chunks) take the faster kernels.  sorted_ids: in each
- * block the slots come before the padding (ids >= S), as align writes them. */
+ * widths and strides of whole chunks) take the faster kernels.  The products and the
+ * gradient by rows write the row of every slot that sorted_ids lists, wherever
+ * padding (ids >= S) stands in a block. */
 #define MOE_BF16 0
 #define MOE_FP16 1
 
@@ -410,7 +411,8 @@ int moe_grouped_mm_dgrad(const void* dy, const void* w, const int32_t* sorted_id
 
 /* Its gradient by the weights: dw[e, n, k] = sum over the slots s of e of
  * dy[s, n] * x[s / top_k, k]; zeros for experts without slots.  expert_ids must
- * ascend over the blocks, as align without an expert map writes them. */
+ * ascend over the blocks and an expert's slots come before its padding, as align
+ * without an expert map writes them. */
 int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, const int32_t* sorted_ids,
                          const int32_t* expert_ids, const int32_t* ntpp, const int32_t* expert_table, int64_t S,
                          int32_t top_k, int64_t N, int64_t K, int32_t E, int32_t block_size_m, int64_t max_padded,

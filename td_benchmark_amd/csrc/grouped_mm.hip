@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
     valid = slot < g.S;
     smSlot[tid] = valid ? (int)slot : -1;
   }
-  const int nvalid = __syncthreads_count(valid);
+  const int nvalid = end_of<TM>(valid);  // rows up to the last slot
   if (nvalid == 0) return;
   const bool none = e < 0 || e >= g.E;
   const uint8_t* a_row[RT];
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) sum = sum + part[w][r][l];
     const int slot = smSlot[row];
-    if (slot < 0) return;  // padding before a slot, which align never writes
+    if (slot < 0) return;  // padding before a slot
     float f[4];
     if constexpr (EB == 1) {
       const float sa = none ? 0.0f : g.As[g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot)];

@@ -128,6 +128,23 @@ MOE_DEVICE int64_t live_blocks(const MmArgs& g) {
   return n < 0 ? 0 : (n < g.n_blocks ? n : g.n_blocks);
 }
 
+// One past the last of the workgroup's first N threads with `on`; a barrier.  Rows of
+// a block up to its last slot count, for padding may stand between them in sorted
+// ids that align did not write.
+template <int N>
+MOE_DEVICE int end_of(bool on) {
+  constexpr int WAVES = (N + 63) / 64;
+  __shared__ int ends[WAVES];
+  const int wave = threadIdx.x >> 6;
+  const uint64_t m = __ballot(on);
+  if (wave < WAVES && (threadIdx.x & 63) == 0) ends[wave] = m ? 64 * wave + 64 - __clzll((long long)m) : 0;
+  __syncthreads();
+  int end = ends[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) end = ends[w] > end ? ends[w] : end;
+  return __builtin_amdgcn_readfirstlane(end);
+}
+
 // One round of a search in ascending words by the calling wave: [lo, hi] holds the
 // place of the first word that is at least v; 64 probes narrow it to a 64th.
 MOE_DEVICE void narrow(const int32_t* a, int32_t v, int64_t& lo, int64_t& hi) {

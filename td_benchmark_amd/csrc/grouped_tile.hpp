@@ -237,8 +237,8 @@ MOE_DEVICE bool table_tile(const MmArgs& g, int64_t& pos0, int64_t& j, int& e, i
   return true;
 }
 
-// One tile: rows [i0, i0 + nvalid) of the output, or the nvalid slots of the
-// table, by columns j0 on (col0 on of the columns' table), over `length` of the
+// One tile: rows [i0, i0 + nvalid) of the output, or the slots of the table's first
+// nvalid rows, by columns j0 on (col0 on of the columns' table), over `length` of the
 // contraction.  K: the tile of the launch, which T is or is a part of.
 template <class OP, bool FP16, int FORM, class K, class T>
 MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int col0, int e,
@@ -567,7 +567,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     const int64_t j = j0 + cc * 8;
     if (j >= g.J) continue;
     const int64_t orow = FORM == kWgrad ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
-    if (FORM != kWgrad && orow < 0) continue;  // padding before a slot, which align never writes
+    if (FORM != kWgrad && orow < 0) continue;  // padding before a slot
     const v4i v = *reinterpret_cast<const v4i*>(out + row * TN + ((cc ^ (row & ROT)) << 3));
     v4i* const to = reinterpret_cast<v4i*>(g.C + (orow * g.ldc + j) * 2);
     // nothing reads the weights' gradient soon: past the L2 it takes 3-5 % less
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
         cols[TN + c] = g.bias ? from16<FP16>(g.bias[jj]) : 0.0f;
       }
     }
-    nvalid = __syncthreads_count(valid);
+    nvalid = end_of<TM>(valid);
     if (nvalid == 0) return;
     if (e < 0 || e >= g.E) {  // no expert: zero rows
       for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {

@@ -1,0 +1,76 @@
+"""GPU: rows and sizes of the grouped and int8 products that align's own output
+does not have: slots behind padding."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+BF16 = torch.bfloat16
+
+
+def _holes(BM, slots, S):
+    """Sorted positions of one block: the given slots at its first, some inner and its last places, else padding."""
+    places = [0, BM - 1, 1, BM // 2 + 1, BM // 2 - 1][:len(slots)]
+    ids = torch.full((BM,), S, dtype=torch.int32)
+    ids[torch.tensor(places)] = torch.tensor(slots, dtype=torch.int32)
+    return ids
+
+
+@pytest.mark.parametrize("a_by_pos", [False, True])
+@pytest.mark.parametrize("BM,K,N", [(16, 2048, 64), (32, 4096, 64), (16, 160, 200), (32, 160, 200), (64, 160, 200), (128, 160, 264),
+                                    (256, 160, 264), (64, 33, 50), (256, 33, 50)])
+def test_int8_slots_behind_padding(BM, K, N, a_by_pos):
+    """Every listed slot gets its row wherever it stands in its block, as in the FP8 form of the same call."""
+    from td_benchmark_amd import ops
+    S = 13
+    g = torch.Generator(device="cuda").manual_seed(BM + K)
+    blocks = [_holes(BM, [2], S), _holes(BM, [7, 0, 3, 9, 11], S), _holes(BM, [1, 4], S), torch.full((BM,), S, dtype=torch.int32),
+              _holes(BM, [5, 12, 8], S).flip(0)]
+    experts = [0, 1, 1, 0, -1]  # the last one's rows are zeros
+    ids = torch.cat(blocks).cuda()
+    a = torch.randint(-127, 128, (ids.numel() if a_by_pos else S, K), generator=g, device="cuda").to(torch.int8)
+    b = torch.randint(-127, 128, (2, N, K), generator=g, device="cuda").to(torch.int8)
+    sa, sb = torch.ones(a.shape[0], device="cuda"), torch.ones((2, N), device="cuda")
+    y = torch.full((S, 1, N), 7.0, dtype=BF16, device="cuda")
+    ops.dispatch_fused_moe_kernel(a, b, y, sa, sb, None, None, ids, torch.tensor(experts, dtype=torch.int32, device="cuda"),
+                                  torch.tensor([ids.numel()], dtype=torch.int32, device="cuda"), False, 1, {"BLOCK_SIZE_M": BM},
+                                  use_fp8_w8a8=False, use_int8_w8a8=True, per_channel_quant=True, a_by_pos=a_by_pos)
+    want = torch.full((S, N), 7.0, dtype=BF16, device="cuda")
+    for p, s in enumerate(ids.tolist()):
+        if s < S:  # whole sums below 2^24 are exact in fp32, then rounded once
+            e = experts[p // BM]
+            want[s] = (a[p if a_by_pos else s].double() @ b[e].double().t()).float().to(BF16) if e >= 0 else 0.0
+    assert (y.view(S, N) == want).all(1).tolist() == [True] * S
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("BM,K,N", [(16, 2048, 64), (32, 160, 200), (64, 160, 200), (128, 160, 264), (256, 160, 264), (256, 33, 50)])
+def test_16_bit_slots_behind_padding(BM, K, N, dtype):
+    """The same of the C entries of the 16-bit product and its gradient by rows, in both types of its rows."""
+    from td_benchmark_amd import _lib
+    S, E = 9, 2
+    code = {torch.bfloat16: 0, torch.float16: 1}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(BM + K)
+    ids = torch.cat([_holes(BM, [2, 8, 0], S), _holes(BM, [7, 3], S).flip(0), _holes(BM, [6, 1, 4, 5], S)]).cuda()
+    experts = [0, 1, -1]
+    eids = torch.tensor(experts, dtype=torch.int32, device="cuda")
+    ntpp = torch.tensor([ids.numel()], dtype=torch.int32, device="cuda")
+    # small whole numbers: every sum is exact in fp32
+    x, dy = (torch.randint(-3, 4, (S, n), generator=g, device="cuda").to(dtype) for n in (K, N))
+    w = torch.randint(-3, 4, (E, N, K), generator=g, device="cuda").to(dtype)
+    y, dx = (torch.full((S, n), 7.5, dtype=dtype, device="cuda") for n in (N, K))
+    dx32 = torch.full((S, K), 7.5, dtype=torch.float32, device="cuda")
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    at = (ids.data_ptr(), eids.data_ptr(), ntpp.data_ptr(), None)
+    assert L.moe_grouped_mm(x.data_ptr(), K, w.data_ptr(), *at, S, 1, N, K, E, BM, ids.numel(), code, y.data_ptr(), st) == 0
+    for f32, out in ((0, dx), (1, dx32)):
+        assert L.moe_grouped_mm_dgrad(dy.data_ptr(), w.data_ptr(), *at, S, N, K, E, BM, ids.numel(), code, f32, out.data_ptr(), st) == 0
+    for p, s in enumerate(ids.tolist()):
+        if s >= S:
+            continue
+        e = experts[p // BM]
+        wy, wx = (x[s].double() @ w[e].double().t(), dy[s].double() @ w[e].double()) if e >= 0 else (y.new_zeros(N), y.new_zeros(K))
+        assert torch.equal(y[s], wy.to(dtype)) and torch.equal(dx[s], wx.to(dtype)), (p, s)
+        assert torch.equal(dx32[s], wx.float()), (p, s)
