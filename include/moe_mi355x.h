@@ -374,8 +374,9 @@ int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64_t R, int64
  * integers.  No counterpart in the reference's FP8 layer; the int8 forms are
  * vLLM's fused_moe use_int8_w8a8 with per_channel_quant.  dtype: MOE_BF16 or
  * MOE_FP16.  Sums are fp32 (int8: exact in 32-bit integers) and rounded once, to
- * nearest even.  Any sizes; rows of whole 16-byte chunks (16-byte aligned bases,
- * widths and strides of whole chunks) take the faster kernels.  The products and the
+ * nearest even.  Any widths; rows of whole 16-byte chunks (16-byte aligned bases,
+ * widths and strides of whole chunks) take the faster kernels.  A grouped product
+ * whose tiles need more than one launch's 2^32 threads is MOE_ERR_BAD_SHAPE.  The products and the
  * gradient by rows write the row of every slot that sorted_ids lists, wherever
  * padding (ids >= S) stands in a block. */
 #define MOE_BF16 0

@@ -13,6 +13,9 @@
 
 namespace moe {
 
+// A launch has fewer than 2^32 threads.
+static bool fits_launch(int64_t workgroups, int threads) { return workgroups <= 0xFFFFFFFFll / threads; }
+
 // ---- any sizes, strides and alignment --------------------------------------
 // 64 x 64 tiles in four waves of 32 x 32; a step of 64 bytes of the contraction
 // is staged through registers one element at a time.  Bound by those loads; it
@@ -149,7 +152,7 @@ static int launch_any(MmArgs g, hipStream_t st) {
   const int64_t rows = WEIGHTS ? g.E * ((g.Cn + kAnyTile - 1) / kAnyTile)
                                : g.n_blocks * ((g.bm + kAnyTile - 1) / kAnyTile);
   const int64_t grid = rows * g.n_jt;
-  if (grid > 0x7FFFFFFF) return kErrBadShape;
+  if (!fits_launch(grid, 256)) return kErrBadShape;
   hipLaunchKernelGGL((any_mm_kernel<OP, FP16, WEIGHTS>), dim3((unsigned)grid), dim3(256), 0, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
@@ -157,10 +160,6 @@ static int launch_any(MmArgs g, hipStream_t st) {
 // ---- whole, aligned chunks ---------------------------------------------------
 template <class OP, bool FP16, int FORM, class T>
 static int launch_tile(MmArgs g, hipStream_t st) {
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)tile_mm_kernel<OP, FP16, FORM, T>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          T::LDS_BYTES);
-  if (attr != hipSuccess) return kErrLaunch;
   g.n_jt = (g.J + T::TN - 1) / T::TN;
   int64_t tiles = (FORM == kWgrad ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt, more = 0;
   if (FORM != kWgrad) {
@@ -183,7 +182,11 @@ static int launch_tile(MmArgs g, hipStream_t st) {
   const int64_t deal = FORM == kWgrad ? 8 * kWgradChunk : 8;
   g.shorts = (tiles + deal - 1) / deal * deal;
   const int64_t grid = g.shorts + more;
-  if (grid > 0x7FFFFFFF) return kErrBadShape;
+  if (!fits_launch(grid, T::THREADS)) return kErrBadShape;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)tile_mm_kernel<OP, FP16, FORM, T>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          T::LDS_BYTES);
+  if (attr != hipSuccess) return kErrLaunch;
   hipLaunchKernelGGL((tile_mm_kernel<OP, FP16, FORM, T>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
@@ -287,7 +290,7 @@ template <class OP, bool FP16, int RT>
 static int launch_few(MmArgs g, hipStream_t st) {
   g.n_jt = (g.J + 15) / 16;
   const int64_t grid = (g.n_blocks * g.n_jt + 7) / 8 * 8;
-  if (grid > 0x7FFFFFFF) return kErrBadShape;
+  if (!fits_launch(grid, 64 * kFewWaves)) return kErrBadShape;
   hipLaunchKernelGGL((few_mm_kernel<OP, FP16, RT>), dim3((unsigned)grid), dim3(64 * kFewWaves), 0, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
@@ -560,14 +563,6 @@ extern "C" int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_sca
   if (!y || !a_scale || !b_scale || (K > 0 && (!a || !b))) return kErrNullPointer;
   if (!aligned(y, 2) || !aligned(bias, 2) || !aligned(a_scale, 4) || !aligned(b_scale, 4)) return kErrBadShape;
   MmArgs g{};
-  g.A = (const uint8_t*)a;
-  g.B = (const uint8_t*)b;
-  g.C = (uint8_t*)y;
-  g.As = a_scale;
-  g.Bs = b_scale;
-  g.bias = (const uint16_t*)bias;
-  g.S = M;
-  g.J = N;
   g.Cn = K;
   g.lda = lda;
   g.sbj = ldb;
@@ -579,8 +574,27 @@ extern "C" int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_sca
   // 7168 to 512 18, 23, 21, 24, 33; 200 x 1024 to 8192 26, 16, 11, 8.7, 9.9).
   g.bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
   while (M > 32 && g.bm > 16 && (M + g.bm / 2 - 1) / (g.bm / 2) * ((N + 63) / 64) <= 256) g.bm /= 2;
-  g.n_blocks = (M + g.bm - 1) / g.bm;
   set_top_k(g, 1);
   g.E = 1;
-  return int8_product(g, dtype, (hipStream_t)stream);
+  // In parts that one launch has the threads for, up to 512 of them for 16 columns of a
+  // block of up to 32 rows or 64 x 64 of another: up to 2^26 columns, and whole blocks.
+  const int64_t cols = N < (1 << 26) ? N : 1 << 26;
+  const int64_t tiles = g.bm <= 32 ? (cols + 15) / 16 : g.bm / 64 * ((cols + 63) / 64);
+  const int64_t rows = (0xFFFFFFFFll / 512 - 8) / tiles * g.bm;
+  for (int64_t m = 0; m < M; m += rows) {
+    for (int64_t n = 0; n < N; n += cols) {
+      g.A = (const uint8_t*)a + m * lda;
+      g.As = a_scale + m;
+      g.B = (const uint8_t*)b + n * ldb;
+      g.Bs = b_scale + n;
+      g.bias = bias ? (const uint16_t*)bias + n : nullptr;
+      g.C = (uint8_t*)y + 2 * (m * ldy + n);
+      g.S = M - m < rows ? M - m : rows;
+      g.J = N - n < cols ? N - n : cols;
+      g.n_blocks = (g.S + g.bm - 1) / g.bm;
+      const int rc = int8_product(g, dtype, (hipStream_t)stream);
+      if (rc != kOk) return rc;
+    }
+  }
+  return kOk;
 }

@@ -74,3 +74,23 @@ def test_16_bit_slots_behind_padding(BM, K, N, dtype):
         wy, wx = (x[s].double() @ w[e].double().t(), dy[s].double() @ w[e].double()) if e >= 0 else (y.new_zeros(N), y.new_zeros(K))
         assert torch.equal(y[s], wy.to(dtype)) and torch.equal(dx[s], wx.to(dtype)), (p, s)
         assert torch.equal(dx32[s], wx.float()), (p, s)
+
+
+@pytest.mark.parametrize("M,N", [((1 << 30) + 5, 1), (3, (1 << 30) // 3 + 71), (1, (1 << 26) + 64 * 9 + 8)])
+def test_int8_product_past_one_launch(M, N):
+    """More rows or columns than one launch's threads take: parts, each with its own scales and bias."""
+    from td_benchmark_amd import ops
+    K = 16 if N == (1 << 26) + 64 * 9 + 8 else 1  # the last: whole chunks
+    a = torch.randint(-9, 10, (M, K), device="cuda", dtype=torch.int8)
+    b = torch.randint(-9, 10, (N, K), device="cuda", dtype=torch.int8)
+    # scales of 1 and 2 and a bias of whole numbers: every step is exact in fp32, and rounded once
+    sa, sb = (1.0 + torch.arange(n, device="cuda").remainder(5).eq(0).float() for n in (M, N))
+    a, b = (a.remainder(3), b.remainder(3)) if K > 1 else (a.remainder(8), b.remainder(8))
+    bias = torch.arange(N, device="cuda").remainder(7).to(BF16)
+    y = ops.int8_scaled_mm(a, b, sa, sb, bias=bias)
+    step = 1 << 26
+    for m in range(0, M, step):
+        for n in range(0, N, step):
+            am, bn = a[m:m + step], b[n:n + step]
+            want = sum(am[:, k:k + 1].float() * bn[:, k] for k in range(K)) * sa[m:m + step, None] * sb[n:n + step] + bias[n:n + step].float()
+            assert torch.equal(y[m:m + step, n:n + step], want.to(BF16)), (m, n)

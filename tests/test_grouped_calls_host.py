@@ -114,3 +114,29 @@ def test_a_copy_reads_its_own_memory(native, how):
     assert all(p in inside for p in native[-1][1][3:7])
     assert new.sorted_ids.data_ptr() == native[-1][1][3] and new.expert_ids.data_ptr() == native[-1][1][4]
     assert new.ntpp.data_ptr() == native[-1][1][5]
+
+
+# ---------------------------------------------------------------- more workgroups than a launch has
+
+def test_grouped_products_past_one_launch():
+    """A launch has fewer than 2^32 threads: a grouped product that needs more is a bad shape, found before the launch."""
+    import ctypes
+    from td_benchmark_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("native library not built")
+    L = _lib.lib()
+    bad = next(code for code, name in _lib.STATUS.items() if name == "MOE_ERR_BAD_SHAPE")
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not rejected would launch on host memory")
+    buf = (ctypes.c_int32 * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    # (S, N, K, BM, max_padded): the kernel of any widths, of few rows, of rows of whole chunks
+    for S, N, K, BM, mp in ((1 << 28, 1, 1, 16, 1 << 28), (8, 8, 1024, 16, 1 << 27), (1 << 28, 8, 8, 16, 1 << 29),
+                            (1 << 30, 256, 8, 32, 1 << 30)):
+        for dtype in (0, 1):
+            assert L.moe_grouped_mm(p, K, p, p, p, p, None, S, 1, N, K, 3, BM, mp, dtype, p, None) == bad
+            if N != 8 or K != 1024:
+                assert L.moe_grouped_mm_dgrad(p, p, p, p, p, None, S, K, N, 3, BM, mp, dtype, 0, p, None) == bad
+        assert L.moe_grouped_gemm_int8(p, p, p, p, p, p, p, None, S, 1, 0, N, 2 * K, 3, BM, mp, 0, p, None) == bad
+    for E, N, K in ((1 << 24, 1, 1), (1 << 24, 8, 8), (1 << 23, 8, 520), (1 << 24, 8, 9)):
+        assert L.moe_grouped_mm_wgrad(p, p, K, p, p, p, None, 8, 1, N, K, E, 16, 64, 0, p, None) == bad
