@@ -490,14 +490,18 @@ extern "C" int moe_grouped_mm_wgrad(const void* dy, const void* x, int64_t ldx, 
     //
     // Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
     // sums, where runs are short and most of the time is the gradient's own bytes, or
-    // fill a chip that the square tiles leave half empty.  They read half as much
-    // again: longer runs lose, with many experts sooner, whose operands few tiles share
-    // (us, 256 and 128 rows; 8 experts of 14336 x 4096: 16 slots 183 and 161; 16 of 1536
-    // x 2048: 100 slots 39 and 37, 1000 slots 113 and 124; 128 of 2048 x 1536: 16 slots
-    // 193 and 177, 96 slots 261 and 286; 8 of 256 x 1024, 32 square tiles: 1000 slots 37
-    // and 31).
-    const int64_t square = E * ((N + 255) / 256) * ((K + 255) / 256);
-    if (S <= (E <= 32 ? 100 : 32) * (int64_t)E || square <= 128) {
+    // where square tiles would take more rounds (never fewer) or leave CUs idle in one.
+    // They read half as much again, which long runs lose.  Over 1471 calls of 16 shapes
+    // (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
+    // 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
+    // the others only; limits of 192 to 640 slots are alike within 0.3 %.  By rounds, 128
+    // and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
+    // 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
+    // 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
+    // slots 2039 and 1988.
+    const int64_t cols = (K + 255) / 256;
+    const int64_t half = (E * ((N + 127) / 128) * cols + 511) / 512, square = (E * ((N + 255) / 256) * cols + 255) / 256;
+    if (half < square || half == 1 || S <= 224 * (int64_t)E) {
       using T = MmTile<128, 256, 4, 2, 3, 2, 64>;
       return dtype == kFp16 ? launch_tile<Fp16, true, kWgrad, T>(g, st) : launch_tile<Bf16, false, kWgrad, T>(g, st);
     }

@@ -94,3 +94,25 @@ def test_int8_product_past_one_launch(M, N):
             am, bn = a[m:m + step], b[n:n + step]
             want = sum(am[:, k:k + 1].float() * bn[:, k] for k in range(K)) * sa[m:m + step, None] * sb[n:n + step] + bias[n:n + step].float()
             assert torch.equal(y[m:m + step, n:n + step], want.to(BF16)), (m, n)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 31, 32, 33, 64, 97, 128, 129, 160, 225, 257, 300])
+@pytest.mark.parametrize("over", [0, 1])
+def test_weights_gradient_of_long_runs_in_two_rounds(over, rows):
+    """64 experts of 224 slots on average and of one more in all, in two rounds of tiles of either kind; one expert
+    around the lengths of a step and of the ring, and one with no slot."""
+    from grouped_cases import make, off, products64
+    from td_benchmark_amd import ops
+    E, K, N = 64, 520, 504
+    S = 224 * E + over
+    x, w, _, dy = make(S, 1, E, K, N, BF16 if rows % 2 else torch.float16)
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randint(2, E, (S,), generator=g)
+    ids[ids == 7] = 9
+    ids[torch.randperm(S, generator=g)[:rows]] = 7
+    ids = ids.view(-1, 1).cuda()
+    (_, _, dw), (_, _, mw) = products64(x, w, ids, dy)
+    for block_m in (16, 256):
+        got = ops.grouped_mm_wgrad(dy, x, ops.ExpertSlots(ids, E, block_m))
+        assert off(got, dw, mw, S) <= 0
+        assert not got[:2].any() and (rows > 0 or not got[7].any())
