@@ -116,3 +116,19 @@ def test_weights_gradient_of_long_runs_in_two_rounds(over, rows):
         got = ops.grouped_mm_wgrad(dy, x, ops.ExpertSlots(ids, E, block_m))
         assert off(got, dw, mw, S) <= 0
         assert not got[:2].any() and (rows > 0 or not got[7].any())
+
+
+@pytest.mark.parametrize("K,N", [(1, 1), (8, 8), (7, 5), (33, 47), (64, 64), (72, 136), (128, 256), (200, 264), (256, 128), (136, 520),
+                                 (520, 72), (1000, 24), (130, 258)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autograd_by_tokens_rounds_once(K, N, dtype):
+    """The gradient by the tokens is one fp32 sum of k N products, rounded once, at every width and block size."""
+    from grouped_cases import by_token, make, off, products64
+    from td_benchmark_amd import ops
+    for T, k, E, block_m, how in ((37, 2, 5, None, {}), (129, 4, 6, 16, dict(skew=True, drop=0.05)), (129, 4, 6, 64, dict(drop=0.05)),
+                                  (515, 3, 6, 256, dict(skew=True))):
+        x, w, ids, dy = make(T, k, E, K, N, dtype, **how)
+        (_, dx, _), (_, mx, _) = products64(x, w, ids, dy)
+        x.requires_grad_()
+        got = torch.autograd.grad(ops.grouped_mm(x, w, ops.ExpertSlots(ids, E, block_m)), x, dy)[0]
+        assert off(got, by_token(dx, k), by_token(mx, k), N + k) <= 0
