@@ -236,8 +236,9 @@ extern "C" int moe_fp8_dequant_sum(const void* q_fp8, const float* scales, int64
 // The sum of a token's slot rows (the gradient by the tokens of a grouped
 // product): fp32 rows in ascending slots, rounded once to a 16-bit type.  Rows of
 // 16 bits would halve the bytes, but round each slot's part by itself: 1.4-1.5
-// times the error of one rounding.  HBM-bound: 4 k H bytes read and 2 H written
-// per token.
+// times the error of one rounding.  4 k H bytes are read and 2 H written per token,
+// at 3.1 TB/s (4096 tokens of 8, 2048 columns: 90 us) to 2.8 (of 2, 4096: 60), of the
+// 4.9 of a large copy; what holds it there is not established.
 
 namespace moe {
 

@@ -1360,7 +1360,7 @@ class ExpertSlots:
     device) have no expert, and the products give them zero rows.
     num_experts <= 1023.  ``block_size_m``: the align block size, by default from
     the average slots of an expert.  The ids are copied, so ``topk_ids`` may
-    change afterwards."""
+    change afterwards; a deep copy or an unpickled object has a buffer of its own."""
 
     def __init__(self, topk_ids: torch.Tensor, num_experts: int, block_size_m: int | None = None):
         if topk_ids.dim() != 2:
@@ -1522,8 +1522,10 @@ def grouped_mm_dgrad(dy: torch.Tensor, w: torch.Tensor, slots: ExpertSlots, by_t
 def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, slots: ExpertSlots) -> torch.Tensor:
     """The gradient of ``grouped_mm`` by its weights: dw[e] = sum over the slots s
     of e of dy[s]^T x[row(s)], [E, N, K] in dy's type; zeros for experts without
-    slots.  Each value is one fp32 sum in slot order, so equal inputs give equal
-    bits.  The call itself is not differentiable."""
+    slots.  Each value is one fp32 sum, whose order follows from the run's length
+    and the kernel that widths and alignment select (it is not that of the slots),
+    so that the same call on equal inputs gives equal bits.  The call itself is not
+    differentiable."""
     _no_tangent(dy, x)
     if dy.dim() != 2 or x.dim() != 2:
         raise ValueError(f"dy must be [S, N] and x [rows, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
@@ -1569,8 +1571,9 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, slots: ExpertSlots) -> torch.Te
     x [T, K] has a row for each token (its slots share it: a layer's first
     product) or [S, K] for each slot (the second); rows may be strided.  w [E, N,
     K] contiguous.  Slots without an expert get zero rows and add nothing to the
-    gradients.  Equal inputs give equal bits.  The gradients are once
-    differentiable; see grouped_mm_dgrad and grouped_mm_wgrad, which are also what
+    gradients.  The same call on equal inputs (alike in sizes and alignment, by which
+    a kernel and with it the order of a sum is chosen) gives equal bits.  The
+    gradients are once differentiable; see grouped_mm_dgrad and grouped_mm_wgrad, which are also what
     to capture into a HIP graph (or torch.autograd.grad): a captured ``backward()``
     ends in torch's own accumulation nodes, which wait for the stream they were
     made on while an eager graph of the same leaves is alive, and that breaks the
