@@ -1,5 +1,6 @@
-"""GPU: rows and sizes of the grouped and int8 products that align's own output
-does not have: slots behind padding."""
+"""GPU: rows and sizes of the grouped and int8 products: slots behind padding, more
+workgroups than a launch has, both tiles of the gradient by weights, and the one
+rounding of the gradient by tokens."""
 from __future__ import annotations
 
 import pytest

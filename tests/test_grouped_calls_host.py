@@ -1,5 +1,6 @@
-"""CPU: calls of the grouped products that no refusal of shapes or types covers,
-with the native library replaced by a stub: inputs with a forward-mode tangent."""
+"""CPU: calls of the grouped products that no refusal of shapes or types covers:
+inputs with a forward-mode tangent and copies of the slots, with the native calls
+replaced by a stub, and sizes past the threads of one launch."""
 from __future__ import annotations
 
 import pytest
