@@ -446,6 +446,49 @@ int moe_grouped_gemm_int8(const void* a, const float* a_scale, const void* b, co
                           const float* topk_weights, int64_t S, int32_t top_k, int32_t a_by_pos, int64_t N, int64_t K,
                           int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The gated feed-forward block in 16-bit floats with its gradients, dense or by
+ * experts (no counterpart in the reference's FP8 layer).  Slot s belongs to token
+ * t = s / top_k and to the expert e of its block:
+ *   h_s = topk_weights[s] * silu(x_t Wg_e^T) * (x_t Wu_e^T),  w13_e = [Wg_e; Wu_e]
+ *   y_t = sum_s h_s w2_e^T
+ * Sums are fp32; h and the gradient of [Wg Wu]'s outputs are rounded to dtype, y
+ * and the gradients once from their fp32 sums (a token's over its slots' fp32
+ * rows).  Slots without an expert add nothing.  Any H and I >= 1: widths, strides
+ * and addresses that are not of whole 16-byte chunks go through copies in the
+ * workspace.
+ *
+ * With sorted_ids, expert_ids and ntpp NULL the block is dense: E = 1, top_k = 1,
+ * every row through the one expert. */
+typedef struct moe_ffn {
+  int64_t T, H, I;
+  int64_t ldx;                 /* row stride of x, elements */
+  int64_t max_padded;          /* as for the grouped products; dense: 0 */
+  int32_t top_k, E;
+  int32_t block_size_m;        /* dense: any */
+  int32_t dtype;               /* MOE_BF16 or MOE_FP16 */
+  const void* x;               /* [T, H] */
+  const void* w13;             /* [E, 2 I, H] */
+  const void* w2;              /* [E, H, I] */
+  const float* topk_weights;   /* [T * top_k], or NULL: ones */
+  const int32_t* sorted_ids;   /* as moe_expert_slots writes them */
+  const int32_t* expert_ids;
+  const int32_t* ntpp;
+  const int32_t* expert_table; /* or NULL */
+  void* h;                     /* [T * top_k, Ip] dtype, Ip = I up to a multiple of 8; written by the forward pass, read by the backward */
+  float* gu;                   /* [T * top_k, 2 Ip] fp32, likewise */
+  void* workspace;             /* of moe_ffn_workspace_bytes, 16-byte aligned; only within a call */
+} moe_ffn;
+/* The workspace of a pass; negative: a status code. */
+int64_t moe_ffn_workspace_bytes(const moe_ffn* ffn, int32_t backward);
+/* y [T, H] of dtype. */
+int moe_ffn_forward(const moe_ffn* ffn, void* y, void* stream);
+/* From dy [T, H] the gradients dx [T, H], dw13, dw2 (of dtype) and dtopk_weights
+ * [T * top_k] (fp32), each where not NULL.  h and gu are the forward pass's, and
+ * expert_ids ascend over the blocks as for moe_grouped_mm_wgrad. */
+int moe_ffn_backward(const moe_ffn* ffn, const void* dy, void* dx, void* dw13, void* dw2, float* dtopk_weights,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

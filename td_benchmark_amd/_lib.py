@@ -42,7 +42,16 @@ class MoeLayer(ctypes.Structure):
                                      "share", "hq", "hs", "D")])
 
 
+class MoeFfn(ctypes.Structure):
+    """struct moe_ffn of include/moe_mi355x.h."""
+    _fields_ = ([(n, _i64) for n in ("T", "H", "I", "ldx", "max_padded")]
+                + [(n, _i32) for n in ("top_k", "E", "block_size_m", "dtype")]
+                + [(n, _P) for n in ("x", "w13", "w2", "topk_weights", "sorted_ids", "expert_ids", "ntpp",
+                                     "expert_table", "h", "gu", "workspace")])
+
+
 _LAYER = ctypes.POINTER(MoeLayer)
+_FFN = ctypes.POINTER(MoeFfn)
 
 # name -> (restype, argtypes); must match include/moe_mi355x.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -105,6 +114,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moe_int8_scaled_mm": (ctypes.c_int, [_P, _i64, _P, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _P, _i64, _P]),
     "moe_grouped_gemm_int8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _i64, _i32, _i32, _i64, _i64, _i32, _i32,
                                              _i64, _i32, _P, _P]),
+    "moe_ffn_workspace_bytes": (ctypes.c_int64, [_FFN, _i32]),
+    "moe_ffn_forward": (ctypes.c_int, [_FFN, _P, _P]),
+    "moe_ffn_backward": (ctypes.c_int, [_FFN, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -116,7 +128,7 @@ class MoeKernelError(RuntimeError):
 
 def build(force: bool = True) -> Path:
     """Compile libmoe_mi355x.so for gfx950 with hipcc (no GPU needed)."""
-    args = ["make", "-s", "-C", str(CSRC_DIR)]
+    args = ["make", "-s", "-j8", "-C", str(CSRC_DIR)]
     if force:
         args.insert(1, "-B")
     subprocess.run(args, check=True)

@@ -253,39 +253,39 @@ MOE_DEVICE uint32_t slot_pair(float a, float b) {
 // VEC: a thread has 4 columns of a token, and KMAX > 0 keeps its rows' loads in
 // flight together; else one column.
 template <bool FP16, bool VEC, int KMAX>
-__global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ d, int64_t T, int k, int64_t H,
-                                                       uint16_t* __restrict__ y) {
+__global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ d, int64_t ldd, int64_t T, int k,
+                                                       int64_t H, uint16_t* __restrict__ y) {
   constexpr int W = VEC ? 4 : 1;
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t cpr = H / W;
   if (idx >= T * cpr) return;
   const int64_t t = idx / cpr, c = (idx - t * cpr) * W;
-  const float* src = d + t * k * H + c;
+  const float* src = d + t * k * ldd + c;
   if constexpr (VEC) {
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (KMAX > 0) {
       v4f rows[KMAX];
 #pragma unroll
       for (int i = 0; i < KMAX; ++i)
-        if (i < k) rows[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + i * H));
+        if (i < k) rows[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + i * ldd));
 #pragma unroll
       for (int i = 0; i < KMAX; ++i)
         if (i < k) acc = acc + rows[i];
     } else {
-      for (int i = 0; i < k; ++i) acc = acc + *reinterpret_cast<const v4f*>(src + i * H);
+      for (int i = 0; i < k; ++i) acc = acc + *reinterpret_cast<const v4f*>(src + i * ldd);
     }
     const v2u out = {slot_pair<FP16>(acc[0], acc[1]), slot_pair<FP16>(acc[2], acc[3])};
     *reinterpret_cast<v2u*>(y + t * H + c) = out;
   } else {
     float acc = 0.0f;
-    for (int i = 0; i < k; ++i) acc += src[i * H];
+    for (int i = 0; i < k; ++i) acc += src[i * ldd];
     y[t * H + c] = (uint16_t)slot_pair<FP16>(acc, 0.0f);
   }
 }
 
 template <bool FP16>
-static int slot_sum(const float* d, int64_t T, int32_t k, int64_t H, uint16_t* y, hipStream_t st) {
-  const bool vec = H % 4 == 0 && aligned16(d) && ((uintptr_t)y & 7) == 0;
+static int slot_sum(const float* d, int64_t ldd, int64_t T, int32_t k, int64_t H, uint16_t* y, hipStream_t st) {
+  const bool vec = H % 4 == 0 && ldd % 4 == 0 && aligned16(d) && ((uintptr_t)y & 7) == 0;
   // a launch has fewer than 2^32 threads: the tokens in parts of up to 2^31 of them
   const int64_t per_t = vec ? H / 4 : H;
   if (per_t > 0x7FFFFFFF) return kErrBadShape;
@@ -294,17 +294,22 @@ static int slot_sum(const float* d, int64_t T, int32_t k, int64_t H, uint16_t* y
   for (int64_t t = 0; t < T; t += part) {
     const int64_t n = T - t < part ? T - t : part;
     const dim3 grid((unsigned)((n * per_t + 255) / 256));
-    const float* dt = d + t * k * H;
+    const float* dt = d + t * k * ldd;
     uint16_t* yt = y + t * H;
     if (!vec)
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
     else if (k <= 8)
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
     else
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, dt, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
   }
   return kOk;
+}
+
+int slot_sum_rows(const float* d, int64_t ldd, int64_t T, int32_t k, int64_t H, int32_t dtype, void* y, hipStream_t st) {
+  return dtype == MOE_FP16 ? slot_sum<true>(d, ldd, T, k, H, (uint16_t*)y, st)
+                           : slot_sum<false>(d, ldd, T, k, H, (uint16_t*)y, st);
 }
 
 }  // namespace moe
@@ -316,6 +321,5 @@ extern "C" int moe_slot_sum(const float* d, int64_t T, int32_t top_k, int64_t H,
   if (!d || !y) return kErrNullPointer;
   if (((uintptr_t)d & 3) != 0 || ((uintptr_t)y & 1) != 0) return kErrBadShape;
   hipStream_t st = (hipStream_t)stream;
-  return dtype == MOE_FP16 ? slot_sum<true>(d, T, top_k, H, (uint16_t*)y, st)
-                           : slot_sum<false>(d, T, top_k, H, (uint16_t*)y, st);
+  return slot_sum_rows(d, H, T, top_k, H, dtype, y, st);
 }

@@ -1,0 +1,404 @@
+// The gated feed-forward block in 16-bit floats with its gradients, dense or by
+// experts.  Slot s of token t(s) = s / top_k, expert e(s), router's weight w_s (1
+// without):
+//   G = x_t Wg_e^T, U = x_t Wu_e^T           w13_e = [Wg; Wu], fp32 sums, kept in fp32
+//   h_s = round16(w_s silu(G) U)             silu(z) = z s(z), s(z) = 1 / (1 + exp(-z))
+//   y_t = round16(sum_s h_s W2_e^T)          fp32 rows, fp32 sum
+// and with D_s = dy_t W2_e (fp32):
+//   dw_s = sum_i D silu(G) U,  dU = w_s D silu(G),  dG = w_s D U (s + silu(G) (1 - s))
+//   dx_t = round16(sum_s [dG dU]_s W13_e)    [dG dU] rounded to 16 bits
+//   dW13_e = sum_s [dG dU]_s^T x_t,  dW2_e = sum_s dy_t^T h_s
+// The router's weight goes into h, where there is a rounding anyway: no slot's
+// output row is kept for its gradient.  h and [dG dU] are rounded because the
+// matrix instructions take 16 bits; G and U are kept in fp32, which costs 8 I bytes
+// more a slot than in 16 bits (3 % of a training step) and leaves the gradient of
+// the router's weights, an fp32 value, as exact as its sums.
+#include "grouped_launch.hpp"
+
+namespace moe {
+
+static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+static int64_t up_to_256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// ---- activation ---------------------------------------------------------------
+MOE_DEVICE float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+
+// h of 4 columns a thread: reads 32 bytes of fp32 and writes 8.
+template <bool FP16>
+__global__ __launch_bounds__(256) void act_kernel(const float* __restrict__ gu, const float* __restrict__ weight, int64_t S,
+                                                  int64_t I, uint16_t* __restrict__ h) {
+  const int64_t cpr = I / 4, n = S * cpr;
+  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
+    const int64_t s = idx / cpr, c = (idx - s * cpr) * 4;
+    const v4f g = *reinterpret_cast<const v4f*>(gu + s * 2 * I + c), u = *reinterpret_cast<const v4f*>(gu + s * 2 * I + I + c);
+    const float w = weight ? weight[s] : 1.0f;
+    float f[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) f[v] = g[v] * sigmoid(g[v]) * u[v] * w;
+    *reinterpret_cast<v2u*>(h + s * I + c) = (v2u){pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
+  }
+}
+
+// [dG dU] and the router's weight's gradient of one slot a workgroup.
+template <bool FP16>
+__global__ __launch_bounds__(256) void act_grad_kernel(const float* __restrict__ d, const float* __restrict__ gu,
+                                                       const float* __restrict__ weight, int64_t S, int64_t I,
+                                                       uint16_t* __restrict__ dgu, float* __restrict__ dweight) {
+  __shared__ float part[4];
+  for (int64_t s = blockIdx.x; s < S; s += gridDim.x) {
+    const float w = weight ? weight[s] : 1.0f;
+    float sum = 0.0f;
+    for (int64_t c = threadIdx.x * 4; c < I; c += 1024) {
+      const v4f dv = *reinterpret_cast<const v4f*>(d + s * I + c);
+      const v4f g = *reinterpret_cast<const v4f*>(gu + s * 2 * I + c), u = *reinterpret_cast<const v4f*>(gu + s * 2 * I + I + c);
+      float dg[4], du[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float sg = sigmoid(g[v]), a = g[v] * sg;
+        sum += dv[v] * a * u[v];
+        du[v] = dv[v] * w * a;
+        dg[v] = dv[v] * w * u[v] * (sg + a * (1.0f - sg));
+      }
+      *reinterpret_cast<v2u*>(dgu + s * 2 * I + c) = (v2u){pack2<FP16>(dg[0], dg[1]), pack2<FP16>(dg[2], dg[3])};
+      *reinterpret_cast<v2u*>(dgu + s * 2 * I + I + c) = (v2u){pack2<FP16>(du[0], du[1]), pack2<FP16>(du[2], du[3])};
+    }
+    if (!dweight) continue;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) dweight[s] = part[0] + part[1] + part[2] + part[3];
+  }
+}
+
+// ---- rows that are not whole 16-byte chunks --------------------------------------
+// dst [B][rows_d][cols_d] = src [B][rows_s][cols_s] with zeros past its ends, or its
+// first rows and columns: widths that the products cannot take are copied to whole
+// chunks and their results back.  8 columns a thread, one by one on the odd side.
+struct Copy {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t B, rows_s, cols_s, ld_s, batch_s, rows_d, cols_d, ld_d, batch_d;
+};
+__global__ __launch_bounds__(256) void copy_kernel(Copy c) {
+  const int64_t cpr = (c.cols_d + 7) / 8, n = c.B * c.rows_d * cpr;
+  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
+    const int64_t r = idx / cpr, col = (idx - r * cpr) * 8, b = r / c.rows_d, row = r - b * c.rows_d;
+    const uint16_t* src = c.src + b * c.batch_s + row * c.ld_s + col;
+    uint16_t* dst = c.dst + b * c.batch_d + row * c.ld_d + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < c.cols_d) dst[i] = row < c.rows_s && col + i < c.cols_s ? src[i] : (uint16_t)0;
+  }
+}
+static unsigned grid_for(int64_t threads) {
+  const int64_t g = (threads + 255) / 256;
+  return (unsigned)(g < 8192 ? g : 8192);
+}
+static int launch_copy(const Copy& c, hipStream_t st) {
+  const int64_t n = c.B * c.rows_d * ((c.cols_d + 7) / 8);
+  if (n == 0) return kOk;
+  hipLaunchKernelGGL(copy_kernel, dim3(grid_for(n)), dim3(256), 0, st, c);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+// ---- the block ---------------------------------------------------------------------
+// Rows of a dense product's tile: as many as there are up to 256, or fewer where
+// tiles of 64 columns do not fill the 256 CUs.
+static int dense_rows(int64_t M, int64_t N) {
+  int bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  while (M > 32 && bm > 16 && (M + bm / 2 - 1) / (bm / 2) * ((N + 63) / 64) <= 256) bm /= 2;
+  return bm;
+}
+
+static int check_ffn(const moe_ffn& f) {
+  if (f.T < 0 || f.H < 1 || f.I < 1 || f.H > (1 << 29) || f.I > (1 << 28) || f.ldx < f.H || f.ldx > (1 << 29)) return kErrBadShape;
+  if (f.dtype != kBf16 && f.dtype != kFp16) return kErrBadShape;
+  if (f.top_k < 1) return kErrBadTopK;
+  if (f.E < 1) return kErrBadExperts;
+  if (f.T * f.top_k > 0x7FFFFFFE || f.max_padded < 0 || f.max_padded > 0x7FFFFFFF) return kErrBadShape;
+  if (!f.sorted_ids && !f.expert_ids && !f.ntpp) {
+    if (f.E != 1 || f.top_k != 1) return kErrBadExperts;
+  } else {
+    if (!f.sorted_ids || !f.expert_ids || !f.ntpp) return kErrNullPointer;
+    if (!block_m_ok(f.block_size_m)) return kErrBadBlockSize;
+  }
+  return kOk;
+}
+
+// Sizes and places of one pass.
+struct Ffn {
+  const moe_ffn& f;
+  int64_t S, Hp, Ip;
+  bool dense, odd;  // odd: widths that are padded
+  hipStream_t st;
+  explicit Ffn(const moe_ffn& l, void* stream = nullptr)
+      : f(l), S(l.T * l.top_k), Hp(up8(l.H)), Ip(up8(l.I)), dense(!l.sorted_ids), odd(Hp != l.H || Ip != l.I),
+        st((hipStream_t)stream) {}
+  bool copy_x() const { return Hp != f.H || !chunks(f.x, f.ldx, 2); }
+  bool copy_w(const void* w) const { return odd || !aligned(w, 16); }
+  int64_t x_bytes() const { return up_to_256(2 * f.T * Hp); }
+  int64_t w13_bytes() const { return up_to_256(4 * f.E * Ip * Hp); }
+  int64_t w2_bytes() const { return up_to_256(2 * f.E * Ip * Hp); }
+  int64_t rows_bytes() const { return f.top_k > 1 ? up_to_256(4 * S * Hp) : 0; }
+
+  int pad_rows(const void* x, int64_t ldx, void* to) const {
+    return launch_copy({(const uint16_t*)x, (uint16_t*)to, 1, f.T, f.H, ldx, 0, f.T, Hp, Hp, 0}, st);
+  }
+  int pad_w13(const void* w, void* to) const {
+    return launch_copy({(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, f.H, f.I * f.H, Ip, Hp, Hp, Ip * Hp}, st);
+  }
+  int pad_w2(const void* w, void* to) const {
+    return launch_copy({(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, f.I, f.H * f.I, Hp, Ip, Ip, Hp * Ip}, st);
+  }
+  int crop_rows(const void* y, void* to) const {
+    return launch_copy({(const uint16_t*)y, (uint16_t*)to, 1, f.T, f.H, Hp, 0, f.T, f.H, f.H, 0}, st);
+  }
+  int crop_w13(const void* w, void* to) const {
+    return launch_copy({(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, Hp, Ip * Hp, f.I, f.H, f.H, f.I * f.H}, st);
+  }
+  int crop_w2(const void* w, void* to) const {
+    return launch_copy({(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, Ip, Hp * Ip, f.H, f.I, f.I, f.H * f.I}, st);
+  }
+
+  // A product over the slots, of J columns.
+  MmArgs args(int64_t J) const {
+    MmArgs g{};
+    g.S = S;
+    g.J = J;
+    g.E = f.E;
+    if (dense) {
+      g.bm = dense_rows(S, J);
+      g.n_blocks = (S + g.bm - 1) / g.bm;
+    } else {
+      const bool any = f.max_padded > 0;
+      g.sorted = f.sorted_ids;
+      g.eids = f.expert_ids;
+      g.ntpp = any ? f.ntpp : nullptr;
+      g.table = any ? f.expert_table : nullptr;
+      g.bm = f.block_size_m;
+      g.n_blocks = f.max_padded / f.block_size_m;
+    }
+    return g;
+  }
+  template <int FORM>
+  int rows(const MmArgs& g) const {
+    return f.dtype == kFp16 ? launch_rows<Fp16, true, FORM>(g, st) : launch_rows<Bf16, false, FORM>(g, st);
+  }
+  // out rows [S] = A's rows (a row for each `per` slots) times B [E][J][Cn] along its rows, or with `columns` [E][Cn][J]
+  // along its columns; fp32 rows with out32.
+  int product(const void* A, int64_t lda, int per, const void* B, int64_t J, int64_t Cn, bool columns, bool out32, void* out) const {
+    MmArgs g = args(J);
+    g.A = (const uint8_t*)A;
+    g.B = (const uint8_t*)B;
+    g.C = (uint8_t*)out;
+    g.Cn = Cn;
+    g.lda = lda;
+    g.sbj = columns ? 1 : Cn;
+    g.sbc = columns ? J : 1;
+    g.b_es = J * Cn;
+    g.ldc = J;
+    set_top_k(g, per);
+    g.out32 = out32 ? 1 : 0;
+    if (columns) return tile_dgrad(g, f.dtype, st);
+    return out32 ? rows<kRows32>(g) : tile_product(g, f.dtype, st);
+  }
+  // dw [E][N][J] = A^T B over each expert's slots; by_token: A has the token's row and B the slot's, else the other way.
+  int weights(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t N, int64_t J, bool by_token, void* dw) const {
+    MmArgs g = args(J);
+    g.A = (const uint8_t*)A;
+    g.B = (const uint8_t*)B;
+    g.C = (uint8_t*)dw;
+    g.Cn = N;
+    g.lda = lda;
+    g.sbc = ldb;
+    g.ldc = J;
+    set_top_k(g, f.top_k);
+    if (dense) return launch_weights<kWgradDense>(g, f.dtype, st);
+    return by_token ? launch_weights<kWgradTok>(g, f.dtype, st) : tile_wgrad(g, f.dtype, st);
+  }
+  // Rows of the tokens from rows of the slots.
+  int token_rows(const float* rows32, void* out) const { return slot_sum_rows(rows32, Hp, f.T, f.top_k, f.H, f.dtype, out, st); }
+};
+
+// Parts of a workspace in order.
+struct Parts {
+  uint8_t* base;
+  int64_t at = 0;
+  void* take(int64_t bytes, bool on = true) {
+    if (!on) return nullptr;
+    uint8_t* p = base ? base + at : nullptr;
+    at += up_to_256(bytes);
+    return p;
+  }
+};
+
+struct Forward {
+  void *x, *w13, *w2, *rows, *y;
+  Forward(const Ffn& b, Parts& p) {
+    x = p.take(b.x_bytes(), b.copy_x());
+    w13 = p.take(b.w13_bytes(), b.copy_w(b.f.w13));
+    w2 = p.take(b.w2_bytes(), b.copy_w(b.f.w2));
+    rows = p.take(b.rows_bytes(), b.f.top_k > 1);
+    y = p.take(b.x_bytes(), b.f.top_k == 1);  // for an output that is not of whole chunks
+  }
+};
+struct Backward {
+  void *x, *dy, *w13, *w2, *d, *dgu, *rows, *dx, *dw13, *dw2;
+  Backward(const Ffn& b, Parts& p) {
+    x = p.take(b.x_bytes(), b.copy_x());
+    dy = p.take(b.x_bytes());
+    w13 = p.take(b.w13_bytes(), b.copy_w(b.f.w13));
+    w2 = p.take(b.w2_bytes(), b.copy_w(b.f.w2));
+    d = p.take(4 * b.S * b.Ip);
+    dgu = p.take(4 * b.S * b.Ip);
+    rows = p.take(b.rows_bytes(), b.f.top_k > 1);
+    dx = p.take(b.x_bytes(), b.f.top_k == 1);
+    dw13 = p.take(b.w13_bytes(), b.odd);
+    dw2 = p.take(b.w2_bytes(), b.odd);
+  }
+};
+
+#define MOE_TRY(call)              \
+  do {                             \
+    const int rc_ = (call);        \
+    if (rc_ != kOk) return rc_;    \
+  } while (0)
+
+static int ffn_forward(const Ffn& b, void* y) {
+  const moe_ffn& f = b.f;
+  Parts parts{(uint8_t*)f.workspace};
+  const Forward ws(b, parts);
+  const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
+  int64_t ldx = f.ldx;
+  if (ws.x) {
+    MOE_TRY(b.pad_rows(x, ldx, ws.x));
+    x = ws.x;
+    ldx = b.Hp;
+  }
+  if (ws.w13) {
+    MOE_TRY(b.pad_w13(w13, ws.w13));
+    w13 = ws.w13;
+  }
+  if (ws.w2) {
+    MOE_TRY(b.pad_w2(w2, ws.w2));
+    w2 = ws.w2;
+  }
+  MOE_TRY(b.product(x, ldx, f.top_k, w13, 2 * b.Ip, b.Hp, false, true, f.gu));
+  const dim3 grid(grid_for(b.S * b.Ip / 4));
+  if (f.dtype == kFp16) hipLaunchKernelGGL(act_kernel<true>, grid, dim3(256), 0, b.st, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)f.h);
+  else hipLaunchKernelGGL(act_kernel<false>, grid, dim3(256), 0, b.st, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)f.h);
+  if (hipGetLastError() != hipSuccess) return kErrLaunch;
+  if (f.top_k > 1) {
+    MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, true, ws.rows));
+    return b.token_rows((const float*)ws.rows, y);
+  }
+  const bool direct = b.Hp == f.H && aligned(y, 16);
+  MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, false, direct ? y : ws.y));
+  return direct ? kOk : b.crop_rows(ws.y, y);
+}
+
+static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void* dw2, float* dweight) {
+  const moe_ffn& f = b.f;
+  Parts parts{(uint8_t*)f.workspace};
+  const Backward ws(b, parts);
+  const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
+  int64_t ldx = f.ldx;
+  if (b.Hp != f.H || !aligned(dy, 16)) {
+    MOE_TRY(b.pad_rows(dy, f.H, ws.dy));
+    dy = ws.dy;
+  }
+  if (ws.x && dw13) {
+    MOE_TRY(b.pad_rows(x, ldx, ws.x));
+    x = ws.x;
+    ldx = b.Hp;
+  }
+  if (dx || dw13 || dweight) {
+    if (ws.w2) {
+      MOE_TRY(b.pad_w2(w2, ws.w2));
+      w2 = ws.w2;
+    }
+    if (b.S > 0) {
+      MOE_TRY(b.product(dy, b.Hp, f.top_k, w2, b.Ip, b.Hp, true, true, ws.d));
+      const dim3 grid(b.S < 16384 ? (unsigned)b.S : 16384u);
+      if (f.dtype == kFp16)
+        hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, b.st, (const float*)ws.d, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)ws.dgu, dweight);
+      else
+        hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, b.st, (const float*)ws.d, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)ws.dgu, dweight);
+      if (hipGetLastError() != hipSuccess) return kErrLaunch;
+    }
+  }
+  if (dx && b.S > 0) {
+    if (ws.w13) {
+      MOE_TRY(b.pad_w13(w13, ws.w13));
+      w13 = ws.w13;
+    }
+    if (f.top_k > 1) {
+      MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, true, ws.rows));
+      MOE_TRY(b.token_rows((const float*)ws.rows, dx));
+    } else {
+      const bool direct = b.Hp == f.H && aligned(dx, 16);
+      MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, false, direct ? dx : ws.dx));
+      if (!direct) MOE_TRY(b.crop_rows(ws.dx, dx));
+    }
+  }
+  if (dw13) {
+    const bool direct = !b.odd && aligned(dw13, 16);
+    if (!direct && !ws.dw13) return kErrBadShape;
+    MOE_TRY(b.weights(ws.dgu, 2 * b.Ip, x, ldx, 2 * b.Ip, b.Hp, false, direct ? dw13 : ws.dw13));
+    if (!direct) MOE_TRY(b.crop_w13(ws.dw13, dw13));
+  }
+  if (dw2) {
+    const bool direct = !b.odd && aligned(dw2, 16);
+    if (!direct && !ws.dw2) return kErrBadShape;
+    MOE_TRY(b.weights(dy, b.Hp, f.h, b.Ip, b.Hp, b.Ip, true, direct ? dw2 : ws.dw2));
+    if (!direct) MOE_TRY(b.crop_w2(ws.dw2, dw2));
+  }
+  return kOk;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t backward) {
+  if (!f) return kErrNullPointer;
+  const int rc = check_ffn(*f);
+  if (rc != kOk) return rc;
+  Parts p{nullptr};
+  const Ffn b(*f);
+  if (backward) Backward(b, p);
+  else Forward(b, p);
+  return p.at;
+}
+
+static int check_pointers(const moe_ffn& f, bool backward) {
+  if (f.T == 0 && !backward) return kOk;
+  if ((f.T > 0 && (!f.x || !f.h || !f.gu)) || !f.w13 || !f.w2) return kErrNullPointer;
+  if (!aligned(f.x, 2) || !aligned(f.w13, 2) || !aligned(f.w2, 2) || !aligned(f.topk_weights, 4) || !aligned(f.h, 16) ||
+      !aligned(f.gu, 16) || !aligned(f.workspace, 16))
+    return kErrBadShape;
+  if (!f.workspace && moe_ffn_workspace_bytes(&f, backward) > 0) return kErrNullPointer;
+  return kOk;
+}
+
+extern "C" int moe_ffn_forward(const moe_ffn* f, void* y, void* stream) {
+  if (!f) return kErrNullPointer;
+  MOE_TRY(check_ffn(*f));
+  MOE_TRY(check_pointers(*f, false));
+  if (f->T == 0) return kOk;
+  if (!y) return kErrNullPointer;
+  if (!aligned(y, 2)) return kErrBadShape;
+  return ffn_forward(Ffn(*f, stream), y);
+}
+
+extern "C" int moe_ffn_backward(const moe_ffn* f, const void* dy, void* dx, void* dw13, void* dw2, float* dtopk_weights,
+                                void* stream) {
+  if (!f) return kErrNullPointer;
+  MOE_TRY(check_ffn(*f));
+  MOE_TRY(check_pointers(*f, true));
+  if (f->T > 0 && !dy) return kErrNullPointer;
+  if (!aligned(dy, 2) || !aligned(dx, 2) || !aligned(dw13, 2) || !aligned(dw2, 2) || !aligned(dtopk_weights, 4)) return kErrBadShape;
+  return ffn_backward(Ffn(*f, stream), dy, dx, dw13, dw2, dtopk_weights);
+}

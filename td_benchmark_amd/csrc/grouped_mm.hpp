@@ -185,4 +185,9 @@ MOE_DEVICE Run run_of(const MmArgs& g, int e) {
   return r;
 }
 
+// Products of rows of whole, aligned 16-byte chunks (grouped_mm.hip).
+int tile_product(const MmArgs& g, int32_t dtype, hipStream_t st);
+int tile_dgrad(const MmArgs& g, int32_t dtype, hipStream_t st);
+int tile_wgrad(const MmArgs& g, int32_t dtype, hipStream_t st);
+
 }  // namespace moe

@@ -21,7 +21,13 @@
 
 namespace moe {
 
-enum Form { kProduct, kDgrad, kWgrad };
+// The product and its two gradients; then, for the feed-forward block (gated.hip),
+// the product into fp32 rows, and the gradient by weights with a row of A for each
+// token and of B for each slot, or of S rows of one expert without a list of slots.
+enum Form { kProduct, kDgrad, kWgrad, kRows32, kWgradTok, kWgradDense };
+constexpr bool by_weights(int form) { return form == kWgrad || form == kWgradTok || form == kWgradDense; }
+// Whether the rows form reads B along its columns.
+constexpr bool by_columns(int form) { return form == kDgrad; }
 
 // Tiles of the weights' gradient that go to an XCD together.  Zipf routing (4093
 // tokens, 64 experts): 1573 us with an even contiguous range of the experts a XCD,
@@ -244,10 +250,11 @@ template <class OP, bool FP16, int FORM, class K, class T>
 MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0, int64_t j0, int col0, int e,
                         int nvalid, int64_t length) {
   constexpr int EB = OP::BYTES, TM = T::TM, TN = T::TN, KS = T::KS, SB = T::SB;
-  constexpr bool A_COLS = FORM == kWgrad, B_COLS = FORM != kProduct;
+  constexpr bool WEIGHTS = by_weights(FORM), COLUMNS = by_columns(FORM);
+  constexpr bool A_COLS = WEIGHTS, B_COLS = WEIGHTS || COLUMNS;
   constexpr int STEP = SB / EB;  // contraction elements of a step
   static_assert(EB == 2 || FORM == kProduct, "transposing reads are of 16-bit values");
-  static_assert(FORM != kWgrad || (KS <= 4 && 8 * STEP * 4 <= K::TABLE), "the ring of slots");
+  static_assert(!WEIGHTS || (KS <= 4 && 8 * STEP * 4 <= K::TABLE), "the ring of slots");
   static_assert(T::THREADS == K::THREADS && T::LDS_BYTES <= K::LDS_BYTES && T::TABLE <= K::TABLE, "a part of the launch's tile");
   const int32_t* smSlot = reinterpret_cast<const int32_t*>(smem);
   const float* smSa = reinterpret_cast<const float*>(smem) + K::TM;
@@ -265,7 +272,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   const uint8_t* a_ptr[T::NA_W];
   const uint8_t* b_ptr[T::NB_W];
   constexpr int ACPR = TM / 8, BCPR = TN / 8;  // chunks of a column-staged row
-  const uint8_t* b_base = g.B + (FORM == kWgrad ? 0 : (int64_t)e * g.b_es * EB);
+  const uint8_t* b_base = g.B + (WEIGHTS ? 0 : (int64_t)e * g.b_es * EB);
   const uint8_t* zeros = reinterpret_cast<const uint8_t*>(&kZeroChunk);
   constexpr int LPR = SB / 16, RPI = 64 / LPR;  // lanes of a row, rows of a load
   auto row_chunk = [&](int gi) { return row_place<SB>(lane % LPR, RPI * gi + lane / LPR); };
@@ -291,7 +298,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     if constexpr (B_COLS) {
       const int64_t c = j0 + col_of(gi, BCPR);
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
-      if constexpr (FORM == kDgrad) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
+      if constexpr (COLUMNS) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
     } else {
       const int64_t j = j0 + RPI * gi + lane / LPR;
       b_ptr[i] = b_base + (j < g.J ? j : g.J - 1) * g.sbj * EB + row_chunk(gi) * 16;
@@ -304,6 +311,15 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // tiles place both operands alike
   uint32_t slot_a[T::NA_W], slot_b[T::NB_W];
   auto read_slots = [&](int kk) {
+    if constexpr (FORM == kWgradDense) {  // row c of the contraction is slot c
+      const uint32_t c0 = (uint32_t)((kk == 0 ? KB - 1 : kk - 1) * STEP), end = (uint32_t)length - 1;
+      auto at = [&](int row) { return c0 + row < end ? c0 + row : end; };
+#pragma unroll
+      for (int i = 0; i < T::NA_W; ++i) slot_a[i] = at(col_row(wave + T::NW * i, ACPR));
+#pragma unroll
+      for (int i = 0; i < T::NB_W; ++i) slot_b[i] = TM == TN ? slot_a[i < T::NA_W ? i : 0] : at(col_row(wave + T::NW * i, BCPR));
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < T::NA_W; ++i)
       slot_a[i] = (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, ACPR)];
@@ -316,7 +332,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // partial run of the contraction, so that no other step has to look for its
   // end; the addresses of the others advance from load to load.
   const int tail = (int)(length - (int64_t)(KB - 1) * STEP);  // elements of step 0
-  const int64_t b_step = FORM == kDgrad ? STEP * g.sbc * EB : SB;
+  const int64_t b_step = COLUMNS ? STEP * g.sbc * EB : SB;
   constexpr int ND = T::NA_W + T::NB_W;
   auto load = [&](int kk, int stage, auto dc, auto first_c) {
     constexpr int d = decltype(dc)::value;
@@ -326,10 +342,10 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     constexpr bool is_b = d < T::NB_W;
     constexpr int i = is_b ? d : d - T::NB_W;
     const int gi = wave + T::NW * i;
-    if constexpr (FORM == kWgrad) {
+    if constexpr (WEIGHTS) {
       const uint8_t* p;
-      if constexpr (is_b) p = b_ptr[i] + (uint64_t)slot_row(g, slot_b[i]) * (uint32_t)(g.sbc * EB);
-      else p = a_ptr[i] + (uint64_t)slot_a[i] * (uint32_t)(g.lda * EB);
+      if constexpr (is_b) p = b_ptr[i] + (uint64_t)(FORM == kWgrad ? slot_row(g, slot_b[i]) : slot_b[i]) * (uint32_t)(g.sbc * EB);
+      else p = a_ptr[i] + (uint64_t)(FORM == kWgradTok ? slot_row(g, slot_a[i]) : slot_a[i]) * (uint32_t)(g.lda * EB);
       if constexpr (first) p = col_row(gi, is_b ? BCPR : ACPR) < left ? p : zeros;
       if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
         lds_load16(p, dst + (is_b ? T::A_BYTES : 0) + gi * 1024);
@@ -337,7 +353,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       const uint8_t* p = b_ptr[i];
       if constexpr (first) {
         p += (KB - 1) * b_step;
-        const bool in = FORM == kDgrad ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
+        const bool in = COLUMNS ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
         p = in ? p : zeros;
       } else {
         b_ptr[i] += b_step;
@@ -388,7 +404,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   int ra = (nvalid - row_base + 15) / 16;
   ra = ra < 0 ? 0 : (ra > T::RS ? T::RS : ra);
 
-  if constexpr (FORM == kWgrad) {
+  if constexpr (WEIGHTS && FORM != kWgradDense) {
     if (KB > 0) {
       for (int s = 0; s < KS + kAhead; ++s) issue_ids(s);
       mm_wait<0>();
@@ -397,11 +413,11 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   }
   const std::integral_constant<int, 0> none;
   const std::integral_constant<int, ND> all;
-  if constexpr (FORM == kWgrad) read_slots(0);
+  if constexpr (WEIGHTS) read_slots(0);
   if (KB > 0) loads(0, 0, none, all, std::true_type{});
 #pragma unroll
   for (int s = 1; s < KS; ++s) {
-    if constexpr (FORM == kWgrad) read_slots(s);
+    if constexpr (WEIGHTS) read_slots(s);
     if (s < KB) loads(s, s, none, all, std::false_type{});
   }
 
@@ -454,10 +470,10 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
               read_b(next, 0);
               read_b(next, 1);
             }
-            if constexpr (FORM == kWgrad) {
+            if constexpr (WEIGHTS) {
               if (kk + KS < KB) {
                 read_slots(kk + KS);
-                issue_ids(kk + KS + kAhead);
+                if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
               }
             }
           }
@@ -514,10 +530,10 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   }
   mm_barrier();
 
-  if constexpr (FORM == kDgrad) {
+  if constexpr (FORM == kDgrad || FORM == kRows32) {
     // fp32 rows: 16 rows of the wave's columns a time through its own part of the
     // ring, so that a row's columns leave as one run
-    if (g.out32) {
+    if (FORM == kRows32 || g.out32) {
       constexpr int CPR = 4 * T::CS;  // 16-byte chunks of a row
       static_assert(T::NW * 16 * CPR * 16 <= KS * T::STAGE, "staging of fp32 rows");
       v4f* part = reinterpret_cast<v4f*>(ring) + wave * 16 * CPR;
@@ -566,12 +582,12 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     const int row = c / CH, cc = c % CH;
     const int64_t j = j0 + cc * 8;
     if (j >= g.J) continue;
-    const int64_t orow = FORM == kWgrad ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
-    if (FORM != kWgrad && orow < 0) continue;  // padding before a slot
+    const int64_t orow = WEIGHTS ? (int64_t)e * g.Cn + i0 + row : (int64_t)smSlot[row];
+    if (!WEIGHTS && orow < 0) continue;  // padding before a slot
     const v4i v = *reinterpret_cast<const v4i*>(out + row * TN + ((cc ^ (row & ROT)) << 3));
     v4i* const to = reinterpret_cast<v4i*>(g.C + (orow * g.ldc + j) * 2);
     // nothing reads the weights' gradient soon: past the L2 it takes 3-5 % less
-    if constexpr (FORM == kWgrad) __builtin_nontemporal_store(v, to);
+    if constexpr (WEIGHTS) __builtin_nontemporal_store(v, to);
     else *to = v;
   }
 }
@@ -581,7 +597,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   constexpr int TM = T::TM, TN = T::TN;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x;
-  if constexpr (FORM == kWgrad) {
+  if constexpr (by_weights(FORM)) {
     // The experts' tiles go in groups of four row tiles with all column tiles, and
     // in chunks to the XCDs in turn: a chunk's tiles share an L2, and an expert with
     // many slots, whose tiles are the long ones, is spread over the chip.
@@ -594,7 +610,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     const int64_t in = t % per_e, ig = in / (kGroup * g.n_jt) * kGroup;
     const int64_t w = nt - ig < kGroup ? nt - ig : kGroup, at = in - ig * g.n_jt;
     const int64_t i0 = (ig + at % w) * TM, j0 = at / w * TN;
-    const Run r = run_of(g, e);
+    const Run r = FORM == kWgradDense ? Run{0, g.S} : run_of(g, e);
     mm_tile<OP, FP16, FORM, T, T>(g, smem, r.pos0, i0, j0, 0, e, (int)(g.Cn - i0 < TM ? g.Cn - i0 : TM), r.count);
   } else {
     // An expert's last block of up to kShort rows takes a shorter tile with a deeper
@@ -644,7 +660,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
         const int slot = smSlot[c / (TN / 8)];
         if (jj >= g.J || slot < 0) continue;
         const int64_t at = (int64_t)slot * g.ldc + jj;
-        if (FORM == kDgrad && g.out32) {
+        if (FORM == kRows32 || (FORM == kDgrad && g.out32)) {
           v4f* to = reinterpret_cast<v4f*>(reinterpret_cast<float*>(g.C) + at);
           to[0] = to[1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
         } else {

@@ -87,4 +87,7 @@ int quant_align(const void* x, int64_t T, int64_t H, void* q, int64_t ldq, float
 int reduce_topk(const void* D, int64_t ldd, const void* addend, int64_t lda, int64_t T, int32_t top_k, int64_t H,
                 const int32_t* mask, void* y, void* stream);
 
+// y[t] = the sum of rows t k to t k + k - 1 of d (row stride ldd), H columns in dtype.
+int slot_sum_rows(const float* d, int64_t ldd, int64_t T, int32_t k, int64_t H, int32_t dtype, void* y, hipStream_t st);
+
 }  // namespace moe

@@ -16,7 +16,7 @@ from typing import Any
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import MoeLayer, check, lib
+from ._lib import MoeFfn, MoeLayer, check, lib
 
 FP8 = torch.float8_e4m3fn
 BLOCK_SHAPE = [128, 128]
@@ -1717,3 +1717,139 @@ def _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_i
                                       num_tokens_post_padded.data_ptr(), None if w is None else w.data_ptr(), S, top_k,
                                       1 if a_by_pos else 0, N, K, E, BM, sorted_token_ids.numel(),
                                       _DTYPE_CODE[C.dtype], C.data_ptr(), _stream_handle()), "moe_grouped_gemm_int8")
+
+
+# ---------------------------------------------------------------------------
+# The gated feed-forward block in 16-bit floats, with its gradients
+# ---------------------------------------------------------------------------
+
+def _ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, slots: ExpertSlots | None,
+         topk_weights: torch.Tensor | None) -> MoeFfn:
+    """The checked operands as the native block's, without buffers."""
+    dims = 2 if slots is None else 3
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
+    if w13.dtype != x.dtype or w2.dtype != x.dtype:
+        raise TypeError(f"w13 and w2 must be {x.dtype} as x, got {w13.dtype} and {w2.dtype}")
+    lead = () if slots is None else (slots.E,)
+    if w13.dim() != dims or w2.dim() != dims or w13.shape[-2] % 2:
+        raise ValueError(f"w13 must be [{'' if slots is None else 'E, '}2 I, H] and w2 [{'' if slots is None else 'E, '}H, I], "
+                         f"got {tuple(w13.shape)} and {tuple(w2.shape)}")
+    I = w13.shape[-2] // 2  # noqa: E741
+    if tuple(w13.shape) != (*lead, 2 * I, H) or tuple(w2.shape) != (*lead, H, I):
+        raise ValueError(f"w13 must be {(*lead, 2 * I, H)} and w2 {(*lead, H, I)}, got {tuple(w13.shape)} and {tuple(w2.shape)}")
+    if H < 1 or I < 1:
+        raise ValueError("hidden and intermediate size must be at least 1")
+    if not w13.is_contiguous() or not w2.is_contiguous():
+        raise ValueError("w13 and w2 must be contiguous")
+    f = MoeFfn(T=T, H=H, I=I, ldx=_row_stride(x, "x"), top_k=1, E=1, block_size_m=16, dtype=_DTYPE_CODE[x.dtype],
+               x=x.data_ptr(), w13=w13.data_ptr(), w2=w2.data_ptr())
+    if slots is None:
+        _need_here("x w13 w2", x, w13, w2)
+        return f
+    if T != slots.T:
+        raise ValueError(f"x has {T} rows, the slots are of {slots.T} tokens")
+    if topk_weights is not None:
+        _need(topk_weights, "topk_weights", torch.float32, (T, slots.top_k), anywhere=True)
+        f.topk_weights = topk_weights.data_ptr()
+    _need_here("x w13 w2 slots topk_weights", x, w13, w2, slots._buf, topk_weights)
+    f.top_k, f.E, f.block_size_m, f.max_padded = slots.top_k, slots.E, slots.block_size_m, slots.max_padded
+    f.sorted_ids, f.expert_ids, f.ntpp, f.expert_table = slots._at
+    return f
+
+
+def _ffn_saved_bytes(f: MoeFfn) -> tuple[int, int]:
+    """Bytes of the saved gate and up products (fp32) and of the saved h."""
+    n = f.T * f.top_k * ((f.I + 7) // 8 * 8)
+    return 8 * n, 2 * n
+
+
+def _ffn_workspace(f: MoeFfn, backward: int) -> int:
+    n = int(lib().moe_ffn_workspace_bytes(f, backward))
+    if n < 0:
+        check(n, "moe_ffn_workspace_bytes")
+    return n
+
+
+def _ffn_forward(f: MoeFfn, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> y and the buffer of gu and h."""
+    gu, h = _ffn_saved_bytes(f)
+    y = x.new_empty((f.T, f.H))
+    saved = torch.empty(gu + h, dtype=torch.uint8, device=x.device)
+    work = torch.empty(_ffn_workspace(f, 0), dtype=torch.uint8, device=x.device)
+    f.gu, f.h, f.workspace = saved.data_ptr(), saved.data_ptr() + gu, work.data_ptr()
+    check(lib().moe_ffn_forward(f, y.data_ptr(), _stream_handle()), "moe_ffn_forward")
+    return y, saved
+
+
+class _FfnFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor | None,
+                slots: ExpertSlots | None) -> torch.Tensor:
+        y, saved = _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x)
+        ctx.save_for_backward(x, w13, w2, topk_weights, saved)
+        ctx.slots = slots
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, dy: torch.Tensor):
+        x, w13, w2, topk_weights, saved = ctx.saved_tensors
+        _no_tangent(dy, dy)
+        dy = dy.contiguous()  # a sum's gradient comes with stride 0
+        f = _ffn(x, w13, w2, ctx.slots, topk_weights)
+        need = ctx.needs_input_grad
+        dx = x.new_empty(x.shape) if need[0] else None
+        dw13 = torch.empty_like(w13) if need[1] else None
+        dw2 = torch.empty_like(w2) if need[2] else None
+        dweights = torch.empty_like(topk_weights) if need[3] else None
+        work = torch.empty(_ffn_workspace(f, 1), dtype=torch.uint8, device=x.device)
+        f.gu, f.h, f.workspace = saved.data_ptr(), saved.data_ptr() + _ffn_saved_bytes(f)[0], work.data_ptr()
+        at = [None if t is None else t.data_ptr() for t in (dx, dw13, dw2, dweights)]
+        check(lib().moe_ffn_backward(f, dy.data_ptr(), *at, _stream_handle()), "moe_ffn_backward")
+        return dx, dw13, dw2, dweights, None
+
+
+def _run_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor | None,
+             slots: ExpertSlots | None) -> torch.Tensor:
+    _no_tangent(x, w13)
+    _no_tangent(w2, w2 if topk_weights is None else topk_weights)
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
+                                    or (topk_weights is not None and topk_weights.requires_grad)):
+        return _FfnFunction.apply(x, w13, w2, topk_weights, slots)
+    return _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x)[0]
+
+
+def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
+    """The gated feed-forward block of a dense layer or a shared expert in bf16 or
+    fp16: y = (silu(x @ wg^T) * (x @ wu^T)) @ w2^T, [T, H], differentiable in x and
+    both weights.  x [T, H], rows may be strided; w13 [2 I, H] = [wg; wu] and w2
+    [H, I] contiguous; any H and I >= 1 (multiples of 8 at 16-byte aligned
+    addresses are taken as they are, others are copied in the call).
+
+    Sums are fp32; the intermediate rows are rounded to 16 bits once, y once from
+    its fp32 sum, in the backward pass the gradient of the two projections once and
+    each gradient once.  What the backward pass needs is kept from the forward one:
+    the projections in fp32 and the intermediate rows, 10 I bytes a token.  The same
+    call on equal inputs (alike in sizes and alignment) gives equal bits.  Once
+    differentiable; for capture into a HIP graph as grouped_mm: torch.autograd.grad
+    rather than ``backward()``.  An operand with a forward-mode tangent raises
+    NotImplementedError."""
+    return _run_ffn(x, w13, w2, None, None)
+
+
+def experts_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, slots: ExpertSlots,
+                topk_weights: torch.Tensor | None = None) -> torch.Tensor:
+    """The gated feed-forward block by experts, y[t] = sum over the slots s of token
+    t of topk_weights[s] * ((silu(x[t] @ wg[e]^T) * (x[t] @ wu[e]^T)) @ w2[e]^T), e
+    the slot's expert, [T, H]; differentiable in x, both weights and topk_weights.
+
+    x [T, H] bf16 or fp16, w13 [E, 2 I, H] = [wg; wu], w2 [E, H, I], topk_weights
+    [T, top_k] fp32 (None: ones).  Slots without an expert add nothing, and their
+    weights' gradients are zero.  The router's weight multiplies the intermediate
+    row before its rounding; a token's sum is over fp32 rows of its slots, in
+    ascending slots.  Otherwise as gated_ffn, with 10 I bytes kept a slot."""
+    return _run_ffn(x, w13, w2, topk_weights, slots)
