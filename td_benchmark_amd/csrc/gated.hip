@@ -20,56 +20,16 @@ namespace moe {
 static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 static int64_t up_to_256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// ---- activation ---------------------------------------------------------------
-MOE_DEVICE float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
-
-// h of 4 columns a thread: reads 32 bytes of fp32 and writes 8.
-template <bool FP16>
-__global__ __launch_bounds__(256) void act_kernel(const float* __restrict__ gu, const float* __restrict__ weight, int64_t S,
-                                                  int64_t I, uint16_t* __restrict__ h) {
-  const int64_t cpr = I / 4, n = S * cpr;
-  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
-    const int64_t s = idx / cpr, c = (idx - s * cpr) * 4;
-    const v4f g = *reinterpret_cast<const v4f*>(gu + s * 2 * I + c), u = *reinterpret_cast<const v4f*>(gu + s * 2 * I + I + c);
-    const float w = weight ? weight[s] : 1.0f;
-    float f[4];
+// ---- the gradient of the router's weights -------------------------------------------
+// dweight[s] = the sum of the slot's n parts: a wave a slot, lanes in order.
+__global__ __launch_bounds__(256) void part_sum_kernel(const float* __restrict__ parts, int64_t S, int64_t n, float* __restrict__ dweight) {
+  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (s >= S) return;
+  float sum = 0.0f;
+  for (int64_t i = threadIdx.x & 63; i < n; i += 64) sum += parts[s * n + i];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) f[v] = g[v] * sigmoid(g[v]) * u[v] * w;
-    *reinterpret_cast<v2u*>(h + s * I + c) = (v2u){pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
-  }
-}
-
-// [dG dU] and the router's weight's gradient of one slot a workgroup.
-template <bool FP16>
-__global__ __launch_bounds__(256) void act_grad_kernel(const float* __restrict__ d, const float* __restrict__ gu,
-                                                       const float* __restrict__ weight, int64_t S, int64_t I,
-                                                       uint16_t* __restrict__ dgu, float* __restrict__ dweight) {
-  __shared__ float part[4];
-  for (int64_t s = blockIdx.x; s < S; s += gridDim.x) {
-    const float w = weight ? weight[s] : 1.0f;
-    float sum = 0.0f;
-    for (int64_t c = threadIdx.x * 4; c < I; c += 1024) {
-      const v4f dv = *reinterpret_cast<const v4f*>(d + s * I + c);
-      const v4f g = *reinterpret_cast<const v4f*>(gu + s * 2 * I + c), u = *reinterpret_cast<const v4f*>(gu + s * 2 * I + I + c);
-      float dg[4], du[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float sg = sigmoid(g[v]), a = g[v] * sg;
-        sum += dv[v] * a * u[v];
-        du[v] = dv[v] * w * a;
-        dg[v] = dv[v] * w * u[v] * (sg + a * (1.0f - sg));
-      }
-      *reinterpret_cast<v2u*>(dgu + s * 2 * I + c) = (v2u){pack2<FP16>(dg[0], dg[1]), pack2<FP16>(dg[2], dg[3])};
-      *reinterpret_cast<v2u*>(dgu + s * 2 * I + I + c) = (v2u){pack2<FP16>(du[0], du[1]), pack2<FP16>(du[2], du[3])};
-    }
-    if (!dweight) continue;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) dweight[s] = part[0] + part[1] + part[2] + part[3];
-  }
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) == 0) dweight[s] = sum;
 }
 
 // ---- rows that are not whole 16-byte chunks --------------------------------------
@@ -245,13 +205,13 @@ struct Forward {
   }
 };
 struct Backward {
-  void *x, *dy, *w13, *w2, *d, *dgu, *rows, *dx, *dw13, *dw2;
+  void *x, *dy, *w13, *w2, *parts, *dgu, *rows, *dx, *dw13, *dw2;
   Backward(const Ffn& b, Parts& p) {
     x = p.take(b.x_bytes(), b.copy_x());
     dy = p.take(b.x_bytes());
     w13 = p.take(b.w13_bytes(), b.copy_w(b.f.w13));
     w2 = p.take(b.w2_bytes(), b.copy_w(b.f.w2));
-    d = p.take(4 * b.S * b.Ip);
+    parts = p.take(4 * b.S * ((b.Ip + 31) / 32), b.f.topk_weights);
     dgu = p.take(4 * b.S * b.Ip);
     rows = p.take(b.rows_bytes(), b.f.top_k > 1);
     dx = p.take(b.x_bytes(), b.f.top_k == 1);
@@ -285,11 +245,20 @@ static int ffn_forward(const Ffn& b, void* y) {
     MOE_TRY(b.pad_w2(w2, ws.w2));
     w2 = ws.w2;
   }
-  MOE_TRY(b.product(x, ldx, f.top_k, w13, 2 * b.Ip, b.Hp, false, true, f.gu));
-  const dim3 grid(grid_for(b.S * b.Ip / 4));
-  if (f.dtype == kFp16) hipLaunchKernelGGL(act_kernel<true>, grid, dim3(256), 0, b.st, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)f.h);
-  else hipLaunchKernelGGL(act_kernel<false>, grid, dim3(256), 0, b.st, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)f.h);
-  if (hipGetLastError() != hipSuccess) return kErrLaunch;
+  MmArgs g = b.args(b.Ip);
+  g.A = (const uint8_t*)x;
+  g.B = (const uint8_t*)w13;
+  g.C = (uint8_t*)f.h;
+  g.gu = f.gu;
+  g.topk_w = f.topk_weights;
+  g.Cn = b.Hp;
+  g.lda = ldx;
+  g.sbj = b.Hp;
+  g.sbc = 1;
+  g.b_es = 2 * b.Ip * b.Hp;
+  g.ldc = b.Ip;
+  set_top_k(g, f.top_k);
+  MOE_TRY(b.rows<kGated>(g));
   if (f.top_k > 1) {
     MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, true, ws.rows));
     return b.token_rows((const float*)ws.rows, y);
@@ -320,13 +289,25 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
       w2 = ws.w2;
     }
     if (b.S > 0) {
-      MOE_TRY(b.product(dy, b.Hp, f.top_k, w2, b.Ip, b.Hp, true, true, ws.d));
-      const dim3 grid(b.S < 16384 ? (unsigned)b.S : 16384u);
-      if (f.dtype == kFp16)
-        hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, b.st, (const float*)ws.d, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)ws.dgu, dweight);
-      else
-        hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, b.st, (const float*)ws.d, f.gu, f.topk_weights, b.S, b.Ip, (uint16_t*)ws.dgu, dweight);
-      if (hipGetLastError() != hipSuccess) return kErrLaunch;
+      MmArgs g = b.args(b.Ip);
+      g.A = (const uint8_t*)dy;
+      g.B = (const uint8_t*)w2;
+      g.C = (uint8_t*)ws.dgu;
+      g.gu = f.gu;
+      g.parts = dweight ? (float*)ws.parts : nullptr;
+      g.topk_w = f.topk_weights;
+      g.Cn = b.Hp;
+      g.lda = b.Hp;
+      g.sbj = 1;
+      g.sbc = b.Ip;
+      g.b_es = b.Hp * b.Ip;
+      g.ldc = 2 * b.Ip;
+      set_top_k(g, f.top_k);
+      MOE_TRY(b.rows<kActGrad>(g));
+      if (dweight) {
+        hipLaunchKernelGGL(part_sum_kernel, dim3((unsigned)((b.S + 3) / 4)), dim3(256), 0, b.st, (const float*)ws.parts, b.S, (b.Ip + 31) / 32, dweight);
+        if (hipGetLastError() != hipSuccess) return kErrLaunch;
+      }
     }
   }
   if (dx && b.S > 0) {
@@ -375,7 +356,7 @@ extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t backward) {
 
 static int check_pointers(const moe_ffn& f, bool backward) {
   if (f.T == 0 && !backward) return kOk;
-  if ((f.T > 0 && (!f.x || !f.h || !f.gu)) || !f.w13 || !f.w2) return kErrNullPointer;
+  if ((f.T > 0 && (!f.x || !f.h || (backward && !f.gu))) || !f.w13 || !f.w2) return kErrNullPointer;
   if (!aligned(f.x, 2) || !aligned(f.w13, 2) || !aligned(f.w2, 2) || !aligned(f.topk_weights, 4) || !aligned(f.h, 16) ||
       !aligned(f.gu, 16) || !aligned(f.workspace, 16))
     return kErrBadShape;
@@ -398,7 +379,7 @@ extern "C" int moe_ffn_backward(const moe_ffn* f, const void* dy, void* dx, void
   if (!f) return kErrNullPointer;
   MOE_TRY(check_ffn(*f));
   MOE_TRY(check_pointers(*f, true));
-  if (f->T > 0 && !dy) return kErrNullPointer;
+  if ((f->T > 0 && !dy) || (dtopk_weights && !f->topk_weights)) return kErrNullPointer;
   if (!aligned(dy, 2) || !aligned(dx, 2) || !aligned(dw13, 2) || !aligned(dw2, 2) || !aligned(dtopk_weights, 4)) return kErrBadShape;
   return ffn_backward(Ffn(*f, stream), dy, dx, dw13, dw2, dtopk_weights);
 }

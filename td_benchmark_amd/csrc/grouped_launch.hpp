@@ -12,7 +12,8 @@ static bool fits_launch(int64_t workgroups, int threads) { return workgroups <= 
 // ---- whole, aligned chunks ---------------------------------------------------
 template <class OP, bool FP16, int FORM, class T>
 static int launch_tile(MmArgs g, hipStream_t st) {
-  g.n_jt = (g.J + T::TN - 1) / T::TN;
+  constexpr int kColumns = out_columns(FORM, T::TN);
+  g.n_jt = (g.J + kColumns - 1) / kColumns;
   int64_t tiles = (by_weights(FORM) ? g.E * ((g.Cn + T::TM - 1) / T::TM) : g.n_blocks) * g.n_jt, more = 0;
   if (!by_weights(FORM)) {
     // The short last tiles apart from the whole ones: even rounds, but an expert's
@@ -52,7 +53,7 @@ static int launch_tile(MmArgs g, hipStream_t st) {
 // GB/s of data that is in no cache.
 constexpr int kFewWaves = 8;
 
-template <class OP, bool FP16, int RT, bool ROWS32>
+template <class OP, bool FP16, int RT, int FORM>
 __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
   constexpr int EB = OP::BYTES, TM = 16 * RT, U = 4;
   __shared__ typename OP::Acc part[kFewWaves][RT][64];
@@ -61,7 +62,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t b, j;
   if (!rows_tile<false>(g, b, j)) return;
-  const int64_t j0 = j * 16, pos0 = b * g.bm;
+  constexpr int kCols = out_columns(FORM, 16);
+  const int64_t j0 = j * kCols, pos0 = b * g.bm;
   const int e = g.eids ? g.eids[b] : 0;
   bool valid = false;
   if (tid < TM) {
@@ -79,7 +81,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
     const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + 16 * r + fr : (int64_t)slot_row(g, (uint32_t)slot);
     a_row[r] = g.A + ar * g.lda * EB + kseg * 32;
   }
-  const int64_t jb = j0 + fr < g.J ? j0 + fr : g.J - 1;
+  // kGated: rows of 8 gate and the 8 up columns
+  const int64_t jc = FORM == kGated ? j0 + (fr & 7) : j0 + fr;
+  const int64_t jb = (jc < g.J ? jc : g.J - 1) + (FORM == kGated && fr >= 8 ? g.J : 0);
   const uint8_t* b_row = g.B + ((int64_t)e * g.b_es + jb * g.sbj) * EB + kseg * 32;
   typename OP::Acc acc[RT] = {};
   const int64_t bytes = g.Cn * EB;
@@ -113,11 +117,26 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
   // a lane's four columns of one row again, 64 lanes a 16 x 16 part
   if (tid < RT * 64) {
     const int l = tid & 63, r = tid / 64, row = 16 * r + (l & 15);
-    const int64_t jj = j0 + 4 * (l >> 4);
+    const int64_t jj = j0 + (FORM == kGated ? 4 * (l >> 4 & 1) : 4 * (l >> 4));
     if (row >= nvalid || jj >= g.J) return;  // J is a multiple of 8
     typename OP::Acc sum = part[0][r][l];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) sum = sum + part[w][r][l];
+    if constexpr (FORM == kGated) {
+      // lanes 0 to 31 hold the gate's, 32 to 63 the up projection's four columns of the row
+      const int slot = smSlot[row];
+      if (slot < 0 || none) return;
+      if (g.gu) *reinterpret_cast<v4f*>(g.gu + (int64_t)slot * 2 * g.J + (l & 32 ? g.J : 0) + jj) = sum;
+      if (l & 32) return;
+      typename OP::Acc up = part[0][r][l + 32];
+#pragma unroll
+      for (int w = 1; w < kFewWaves; ++w) up = up + part[w][r][l + 32];
+      const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
+      const v2u pk = {pack2<FP16>(gated(sum[0], up[0], w), gated(sum[1], up[1], w)),
+                      pack2<FP16>(gated(sum[2], up[2], w), gated(sum[3], up[3], w))};
+      *reinterpret_cast<v2u*>(g.C + ((int64_t)slot * g.ldc + jj) * 2) = pk;
+      return;
+    }
     const int slot = smSlot[row];
     if (slot < 0) return;  // padding before a slot
     float f[4];
@@ -133,7 +152,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) f[v] = sum[v];
     }
-    if constexpr (ROWS32) {
+    if constexpr (FORM == kRows32) {
       *reinterpret_cast<v4f*>(g.C + ((int64_t)slot * g.ldc + jj) * 4) = (v4f){f[0], f[1], f[2], f[3]};
     } else {
       const v2u pk = {pack2<FP16>(f[0], f[1]), pack2<FP16>(f[2], f[3])};
@@ -142,12 +161,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
   }
 }
 
-template <class OP, bool FP16, int RT, bool ROWS32>
+template <class OP, bool FP16, int RT, int FORM>
 static int launch_few(MmArgs g, hipStream_t st) {
-  g.n_jt = (g.J + 15) / 16;
+  g.n_jt = (g.J + out_columns(FORM, 16) - 1) / out_columns(FORM, 16);
   const int64_t grid = (g.n_blocks * g.n_jt + 7) / 8 * 8;
   if (!fits_launch(grid, 64 * kFewWaves)) return kErrBadShape;
-  hipLaunchKernelGGL((few_mm_kernel<OP, FP16, RT, ROWS32>), dim3((unsigned)grid), dim3(64 * kFewWaves), 0, st, g);
+  hipLaunchKernelGGL((few_mm_kernel<OP, FP16, RT, FORM>), dim3((unsigned)grid), dim3(64 * kFewWaves), 0, st, g);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
@@ -178,15 +197,15 @@ static double live_blocks_guess(const MmArgs& g) {
 template <class OP, bool FP16, int FORM>
 static int launch_rows(const MmArgs& g, hipStream_t st) {
   const double blocks = live_blocks_guess(g);
-  const double wide = rounds(blocks, g.J, 256, 1.0), half = rounds(blocks, g.J, 128, 0.65),
-               slim = rounds(blocks, g.J, 64, 0.5);
+  const int64_t J = FORM == kGated ? 2 * g.J : g.J;  // columns of B
+  const double wide = rounds(blocks, J, 256, 1.0), half = rounds(blocks, J, 128, 0.65), slim = rounds(blocks, J, 64, 0.5);
   // Few rows on long rows of weights: few tiles, or one or two slots a block (more
   // rows make it draw as much of A as of the weights).  int8, one row, 7168 x 4096:
   // 16.3 us, staged 24.5; 16 tokens on 128 experts 126 and 148; 9 slots a block of
   // 14336 272 and 226; rows of 768 bytes 123 and 79.
-  if constexpr (FORM == kProduct || FORM == kRows32) {
-    if (g.bm <= 32 && g.Cn * OP::BYTES >= 2048 && (blocks * ((g.J + 63) / 64) <= 128.0 || g.S <= 2.0 * blocks))
-      return g.bm == 16 ? launch_few<OP, FP16, 1, FORM == kRows32>(g, st) : launch_few<OP, FP16, 2, FORM == kRows32>(g, st);
+  if constexpr (!by_columns(FORM)) {
+    if (g.bm <= 32 && g.Cn * OP::BYTES >= 2048 && (blocks * ((J + 63) / 64) <= 128.0 || g.S <= 2.0 * blocks))
+      return g.bm == 16 ? launch_few<OP, FP16, 1, FORM>(g, st) : launch_few<OP, FP16, 2, FORM>(g, st);
   }
   if (g.bm <= 32) {
     const bool stream = !by_columns(FORM) || wide <= 1.0;

@@ -66,6 +66,17 @@ MOE_DEVICE float int8_out(int acc, float sa, float sb, bool with_bias, float bia
   return f;
 }
 
+// The feed-forward block's activation, h = w silu(g) u with silu(z) = z s(z), and its
+// gradient by g and u from the gradient d of h; returns d's part of the gradient of w.
+MOE_DEVICE float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+MOE_DEVICE float gated(float g, float u, float w) { return g * sigmoid(g) * u * w; }
+MOE_DEVICE float gated_grad(float d, float g, float u, float w, float& dg, float& du) {
+  const float s = sigmoid(g), a = g * s;
+  dg = d * w * u * (s + a * (1.0f - s));
+  du = d * w * a;
+  return d * a * u;
+}
+
 // One launch of a product.  With sorted, eids and ntpp (as moe_align_block_size
 // writes them): position p of block p / bm belongs to expert eids[p / bm] and
 // slot sorted[p] (S or more: none).  Without: S rows of one expert, slot p.
@@ -100,6 +111,8 @@ struct MmArgs {
   const int32_t* table;
   int64_t shorts;       // rows form with a table: workgroups from this one on take the experts' short last tiles,
   int short_parts;      // so many of them each
+  float* gu;            // feed-forward block: gate and up products of each slot, [S, 2 J], or null
+  float* parts;         // kActGrad: parts of the gradient of topk_w, [S, (J + 31) / 32], or null
   int out32;            // kDgrad: rows of fp32, which are summed over a token's slots before they are rounded
   int bm, top_k, a_by_pos, E;
   // slot / top_k = slot * div_mul >> div_shift for slots below 2^31

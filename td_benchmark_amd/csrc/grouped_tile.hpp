@@ -22,12 +22,17 @@
 namespace moe {
 
 // The product and its two gradients; then, for the feed-forward block (gated.hip),
-// the product into fp32 rows, and the gradient by weights with a row of A for each
-// token and of B for each slot, or of S rows of one expert without a list of slots.
-enum Form { kProduct, kDgrad, kWgrad, kRows32, kWgradTok, kWgradDense };
+// the product into fp32 rows, the product of both projections with the activation,
+// the gradient by rows with the activation's gradient, and the gradient by weights
+// with a row of A for each token and of B for each slot, or of S rows of one expert
+// without a list of slots.
+enum Form { kProduct, kDgrad, kWgrad, kRows32, kGated, kActGrad, kWgradTok, kWgradDense };
 constexpr bool by_weights(int form) { return form == kWgrad || form == kWgradTok || form == kWgradDense; }
 // Whether the rows form reads B along its columns.
-constexpr bool by_columns(int form) { return form == kDgrad; }
+constexpr bool by_columns(int form) { return form == kDgrad || form == kActGrad; }
+// Output columns of a tile of TN columns of B: kGated pairs 16 of the gate with 16 of
+// the up projection, so that a lane holds both of an element.
+constexpr int out_columns(int form, int TN) { return form == kGated ? TN / 2 : TN; }
 
 // Tiles of the weights' gradient that go to an XCD together.  Zipf routing (4093
 // tokens, 64 experts): 1573 us with an even contiguous range of the experts a XCD,
@@ -300,8 +305,16 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
       if constexpr (COLUMNS) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
     } else {
-      const int64_t j = j0 + RPI * gi + lane / LPR;
-      b_ptr[i] = b_base + (j < g.J ? j : g.J - 1) * g.sbj * EB + row_chunk(gi) * 16;
+      const int row = RPI * gi + lane / LPR;
+      int64_t j;
+      if constexpr (FORM == kGated) {
+        j = j0 + (row >> 5) * 16 + (row & 15);
+        j = (j < g.J ? j : g.J - 1) + (row & 16 ? g.J : 0);
+      } else {
+        j = j0 + row;
+        j = j < g.J ? j : g.J - 1;
+      }
+      b_ptr[i] = b_base + j * g.sbj * EB + row_chunk(gi) * 16;
     }
   }
   // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
@@ -558,6 +571,103 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     }
   }
 
+  if constexpr (FORM == kGated || FORM == kActGrad) {
+    // As above: 16 rows of the wave's fp32 columns a time through its part of the
+    // ring, from where a lane takes 8 columns of a row.
+    constexpr int CPR = 4 * T::CS;
+    static_assert(T::NW * 16 * CPR * 16 <= KS * T::STAGE && T::CS % 2 == 0, "staging of fp32 rows");
+    v4f* part = reinterpret_cast<v4f*>(ring) + wave * 16 * CPR;
+    auto stage = [&](int r) {
+#pragma unroll
+      for (int c = 0; c < T::CS; ++c) part[fr * CPR + ((4 * c + kseg) ^ (fr & (CPR - 1) & 15))] = acc[r][c];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    auto chunk = [&](int row, int c) { return part[row * CPR + (c ^ (row & (CPR - 1) & 15))]; };
+    constexpr int UPR = FORM == kGated ? T::CS : 2 * T::CS;  // lanes of a row
+    constexpr int NI = (16 * UPR + 63) / 64;
+#pragma unroll
+    for (int r = 0; r < T::RS; ++r) {
+      if (row_base + r * 16 >= nvalid) break;
+      if constexpr (FORM == kGated) {
+        stage(r);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = (i * 64 + lane) / UPR, u = (i * 64 + lane) % UPR;
+          const int64_t jj = j0 + wn * T::CS * 8 + 8 * u;
+          const int slot = row < 16 && row_base + r * 16 + row < nvalid ? smSlot[row_base + r * 16 + row] : -1;
+          if (slot < 0 || jj >= g.J) continue;
+          const int c = 8 * (u >> 1) + 2 * (u & 1);  // of the gate; the up projection's 4 chunks on
+          const v4f gl = chunk(row, c), gh = chunk(row, c + 1), ul = chunk(row, c + 4), uh = chunk(row, c + 5);
+          if (g.gu) {
+            v4f* to = reinterpret_cast<v4f*>(g.gu + (int64_t)slot * 2 * g.J + jj);
+            to[0] = gl;
+            to[1] = gh;
+            to = reinterpret_cast<v4f*>(g.gu + (int64_t)slot * 2 * g.J + g.J + jj);
+            to[0] = ul;
+            to[1] = uh;
+          }
+          const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
+          v4i out;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            out[v] = (int)pack2<FP16>(gated(gl[2 * v], ul[2 * v], w), gated(gl[2 * v + 1], ul[2 * v + 1], w));
+            out[2 + v] = (int)pack2<FP16>(gated(gh[2 * v], uh[2 * v], w), gated(gh[2 * v + 1], uh[2 * v + 1], w));
+          }
+          *reinterpret_cast<v4i*>(g.C + ((int64_t)slot * g.ldc + jj) * 2) = out;
+        }
+      } else {
+        // the saved products of all of the lane's elements are on their way before the first is used
+        v4f gu[NI][4];
+        int slots[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = (i * 64 + lane) / UPR;
+          const int64_t jj = j0 + col_base + 8 * (lane % UPR);
+          slots[i] = row_base + r * 16 + row < nvalid && jj < g.J ? smSlot[row_base + r * 16 + row] : -1;
+          const v4f* from = reinterpret_cast<const v4f*>(g.gu + (int64_t)(slots[i] < 0 ? 0 : slots[i]) * 2 * g.J + (jj < g.J ? jj : 0));
+          const v4f* up = reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(from) + g.J);
+          gu[i][0] = from[0];
+          gu[i][1] = from[1];
+          gu[i][2] = up[0];
+          gu[i][3] = up[1];
+        }
+        stage(r);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = (i * 64 + lane) / UPR, u = lane % UPR, slot = slots[i];
+          const int64_t jj = j0 + col_base + 8 * u;
+          float sum = 0.0f;
+          if (slot >= 0) {
+            const v4f dl = chunk(row, 2 * u), dh = chunk(row, 2 * u + 1);
+            const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
+            v4i dg, du;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              float a[2], b[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int n = 2 * v + x;
+                sum += gated_grad(n < 4 ? dl[n & 3] : dh[n & 3], gu[i][n < 4 ? 0 : 1][n & 3], gu[i][n < 4 ? 2 : 3][n & 3], w, a[x], b[x]);
+              }
+              dg[v] = (int)pack2<FP16>(a[0], a[1]);
+              du[v] = (int)pack2<FP16>(b[0], b[1]);
+            }
+            uint8_t* to = g.C + ((int64_t)slot * g.ldc + jj) * 2;
+            *reinterpret_cast<v4i*>(to) = dg;
+            *reinterpret_cast<v4i*>(to + 2 * g.J) = du;
+          }
+          if (g.parts) {  // of 32 columns, whatever the tile
+            sum += __shfl_xor(sum, 1);
+            sum += __shfl_xor(sum, 2);
+            if (slot >= 0 && (u & 3) == 0) g.parts[(int64_t)slot * ((g.J + 31) / 32) + jj / 32] = sum;
+          }
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    return;
+  }
+
   // ---- epilogue: rows of 16-bit outputs through LDS, chunks XOR the row ----
   uint16_t* out = reinterpret_cast<uint16_t*>(ring);
   constexpr int CH = TN / 8, ROT = CH < 16 ? CH - 1 : 15;
@@ -630,7 +740,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
       pos0 = b * TM;
       e = g.eids ? g.eids[b] : 0;
     }
-    const int64_t j0 = j * TN;
+    const int64_t j0 = j * out_columns(FORM, TN);
     const int rows = planned ? nvalid : !g.eids && pos0 + TM > g.S ? (int)(g.S - pos0) : TM;
     // the rows' slots, their scales and factors, for their addresses and the results
     bool valid = false;
@@ -655,6 +765,18 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     nvalid = end_of<TM>(valid);
     if (nvalid == 0) return;
     if (e < 0 || e >= g.E) {  // no expert: zero rows
+      if constexpr (FORM == kGated) return;  // nothing reads the row
+      if constexpr (FORM == kActGrad) {      // but the sum over the parts
+        const int64_t n_parts = (g.J + 31) / 32;
+        if (g.parts) {
+          for (int c = tid; c < nvalid * (TN / 32); c += T::THREADS) {
+            const int64_t at = j0 / 32 + c % (TN / 32);
+            const int slot = smSlot[c / (TN / 32)];
+            if (slot >= 0 && at < n_parts) g.parts[(int64_t)slot * n_parts + at] = 0.0f;
+          }
+        }
+        return;
+      }
       for (int c = tid; c < nvalid * (TN / 8); c += T::THREADS) {
         const int64_t jj = j0 + c % (TN / 8) * 8;
         const int slot = smSlot[c / (TN / 8)];
@@ -672,8 +794,9 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     if constexpr (kShort > 0) {
       if (nvalid <= kShort) {
         if (planned && g.short_parts == 4) {
-          if (j0 + part * 64 < g.J)
-            mm_tile<OP, FP16, FORM, T, MmTile<64, 64, 8, 4, 6, 1>>(g, smem, pos0, 0, j0 + part * 64, part * 64, e, nvalid, g.Cn);
+          constexpr int kPart = out_columns(FORM, 64);
+          if (j0 + part * kPart < g.J)
+            mm_tile<OP, FP16, FORM, T, MmTile<64, 64, 8, 4, 6, 1>>(g, smem, pos0, 0, j0 + part * kPart, part * 64, e, nvalid, g.Cn);
         } else {
           mm_tile<OP, FP16, FORM, T, MmTile<64, 256, 8, 1, 3, 1>>(g, smem, pos0, 0, j0, 0, e, nvalid, g.Cn);
         }

@@ -1774,13 +1774,15 @@ def _ffn_workspace(f: MoeFfn, backward: int) -> int:
     return n
 
 
-def _ffn_forward(f: MoeFfn, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """-> y and the buffer of gu and h."""
+def _ffn_forward(f: MoeFfn, x: torch.Tensor, save: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> y and the buffer of gu and h (h alone without ``save``)."""
     gu, h = _ffn_saved_bytes(f)
+    if not save:
+        gu = 0
     y = x.new_empty((f.T, f.H))
     saved = torch.empty(gu + h, dtype=torch.uint8, device=x.device)
     work = torch.empty(_ffn_workspace(f, 0), dtype=torch.uint8, device=x.device)
-    f.gu, f.h, f.workspace = saved.data_ptr(), saved.data_ptr() + gu, work.data_ptr()
+    f.gu, f.h, f.workspace = saved.data_ptr() if save else None, saved.data_ptr() + gu, work.data_ptr()
     check(lib().moe_ffn_forward(f, y.data_ptr(), _stream_handle()), "moe_ffn_forward")
     return y, saved
 
@@ -1789,7 +1791,7 @@ class _FfnFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor | None,
                 slots: ExpertSlots | None) -> torch.Tensor:
-        y, saved = _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x)
+        y, saved = _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x, True)
         ctx.save_for_backward(x, w13, w2, topk_weights, saved)
         ctx.slots = slots
         return y
@@ -1820,7 +1822,7 @@ def _run_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights:
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
                                     or (topk_weights is not None and topk_weights.requires_grad)):
         return _FfnFunction.apply(x, w13, w2, topk_weights, slots)
-    return _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x)[0]
+    return _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x, False)[0]
 
 
 def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
