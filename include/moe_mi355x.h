@@ -446,6 +446,20 @@ int moe_grouped_gemm_int8(const void* a, const float* a_scale, const void* b, co
                           const float* topk_weights, int64_t S, int32_t top_k, int32_t a_by_pos, int64_t N, int64_t K,
                           int32_t E, int32_t block_size_m, int64_t max_padded, int32_t dtype, void* y, void* stream);
 
+/* The dense product in e4m3fn with a scale for each row and 128 columns of a and for
+ * each 128 x 128 block of b: y[m, n] = sum over blocks g of 128 columns of (sum of
+ * a[m, k] * b[n, k] over g) * a_scale[m, g] * b_scale[n / 128, g], + bias[n].  a [M, K],
+ * b [N, K] (row strides lda, ldb), a_scale [M, KB], b_scale [ceil(N / 128), KB], KB =
+ * ceil(K / 128), bias [N] of dtype or NULL, y [M, N] of dtype, row stride ldy.  A
+ * block's dot is the FP8 matrix instruction's, the blocks are added in fp32 and the
+ * sum is rounded once.  Any sizes with 1 <= K < 2^23 - 15; rows of a or b that are
+ * not whole 16-byte chunks at 16-byte aligned addresses are copied to the workspace. */
+int64_t moe_fp8_scaled_mm_workspace_bytes(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
+                                          int64_t K);
+int moe_fp8_scaled_mm(const void* a, int64_t lda, const float* a_scale, const void* b, int64_t ldb,
+                      const float* b_scale, const void* bias, int64_t M, int64_t N, int64_t K, int32_t dtype, void* y,
+                      int64_t ldy, void* workspace, void* stream);
+
 /* ---------------------------------------------------------------------------
  * The gated feed-forward block in 16-bit floats with its gradients, dense or by
  * experts (no counterpart in the reference's FP8 layer).  Slot s belongs to token

@@ -114,6 +114,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moe_int8_scaled_mm": (ctypes.c_int, [_P, _i64, _P, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _P, _i64, _P]),
     "moe_grouped_gemm_int8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _i64, _i32, _i32, _i64, _i64, _i32, _i32,
                                              _i64, _i32, _P, _P]),
+    "moe_fp8_scaled_mm_workspace_bytes": (ctypes.c_int64, [_P, _i64, _P, _i64, _i64, _i64, _i64]),
+    "moe_fp8_scaled_mm": (ctypes.c_int, [_P, _i64, _P, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _P, _i64, _P, _P]),
     "moe_ffn_workspace_bytes": (ctypes.c_int64, [_FFN, _i32]),
     "moe_ffn_forward": (ctypes.c_int, [_FFN, _P, _P]),
     "moe_ffn_backward": (ctypes.c_int, [_FFN, _P, _P, _P, _P, _P, _P]),

@@ -64,14 +64,6 @@ static int launch_copy(const Copy& c, hipStream_t st) {
 }
 
 // ---- the block ---------------------------------------------------------------------
-// Rows of a dense product's tile: as many as there are up to 256, or fewer where
-// tiles of 64 columns do not fill the 256 CUs.
-static int dense_rows(int64_t M, int64_t N) {
-  int bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  while (M > 32 && bm > 16 && (M + bm / 2 - 1) / (bm / 2) * ((N + 63) / 64) <= 256) bm /= 2;
-  return bm;
-}
-
 static int check_ffn(const moe_ffn& f) {
   if (f.T < 0 || f.H < 1 || f.I < 1 || f.H > (1 << 29) || f.I > (1 << 28) || f.ldx < f.H || f.ldx > (1 << 29)) return kErrBadShape;
   if (f.dtype != kBf16 && f.dtype != kFp16) return kErrBadShape;

@@ -232,6 +232,17 @@ static int launch_rows(const MmArgs& g, hipStream_t st) {
   return launch_tile<OP, FP16, FORM, MmTile<256, 256, 8, 4, 2, 1>>(g, st);
 }
 
+// The rows of a dense product's tile are free: as many as there are up to 256, or
+// fewer where tiles of 64 columns do not fill the 256 CUs (int8, us by 16, 32, 64,
+// 128, 256 rows: 1463 x 10640 to 168 columns 29, 23, 29, 39, 61; 256 x 7168 to 4096 66,
+// 37, 22, 24, 33; 512 x 7168 to 512 18, 23, 21, 24, 33; 200 x 1024 to 8192 26, 16, 11,
+// 8.7, 9.9).
+static int dense_rows(int64_t M, int64_t N) {
+  int bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  while (M > 32 && bm > 16 && (M + bm / 2 - 1) / (bm / 2) * ((N + 63) / 64) <= 256) bm /= 2;
+  return bm;
+}
+
 // The gradient by weights.
 template <int FORM>
 static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {

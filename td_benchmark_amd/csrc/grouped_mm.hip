@@ -347,12 +347,7 @@ extern "C" int moe_int8_scaled_mm(const void* a, int64_t lda, const float* a_sca
   g.sbj = ldb;
   g.sbc = 1;
   g.ldc = ldy;
-  // The rows of a tile are free here: as many as there are up to 256, or fewer where
-  // tiles of 64 columns do not fill the 256 CUs (us by 16, 32, 64, 128, 256 rows: 1463 x
-  // 10640 to 168 columns 29, 23, 29, 39, 61; 256 x 7168 to 4096 66, 37, 22, 24, 33; 512 x
-  // 7168 to 512 18, 23, 21, 24, 33; 200 x 1024 to 8192 26, 16, 11, 8.7, 9.9).
-  g.bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  while (M > 32 && g.bm > 16 && (M + g.bm / 2 - 1) / (g.bm / 2) * ((N + 63) / 64) <= 256) g.bm /= 2;
+  g.bm = dense_rows(M, N);
   set_top_k(g, 1);
   g.E = 1;
   // In parts that one launch has the threads for, up to 512 of them for 16 columns of a

@@ -1720,6 +1720,62 @@ def _dispatch_int8(A, B, C, A_scale, B_scale, B_zp, topk_weights, sorted_token_i
 
 
 # ---------------------------------------------------------------------------
+# The dense product in 8-bit floating point with a scale for each block of 128
+# ---------------------------------------------------------------------------
+
+FP8_MAX_K = (1 << 23) - 16
+
+
+def fp8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
+                  bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = dequantised a @ dequantised b^T + bias, [M, N] in ``out_dtype`` (bf16 or
+    fp16): a [M, K] and b [N, K] e4m3fn with a scale for each row and 128 columns of a
+    ([M, ceil(K/128)] fp32, as per_token_group_quant_fp8 gives them) and for each 128 x
+    128 block of b ([ceil(N/128), ceil(K/128)], as quantize_block128).  Any M and N, 1
+    <= K < 2^23 - 15; a last block may be partial.  Rows of a, b and ``out`` may be strided (rows of a
+    and b that are not whole 16-byte chunks at 16-byte aligned addresses are copied in
+    the call); bias [N] in out_dtype.
+
+    The dot of a block of 128 is the FP8 matrix instruction's, which cuts each group of
+    8 products 13 bits below the largest; blocks are scaled and added in fp32 and the
+    sum is rounded once.  A code or scale that is NaN makes its rows or columns NaN."""
+    if a.dim() != 2 or b.dim() != 2 or a.size(1) != b.size(1):
+        raise ValueError(f"a must be [M, K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
+    if a.dtype != FP8 or b.dtype != FP8:
+        raise TypeError(f"a and b must be {FP8}, got {a.dtype} and {b.dtype}")
+    M, K = a.shape
+    N = b.size(0)
+    if not 1 <= K <= FP8_MAX_K:
+        raise ValueError(f"K must be in [1, {FP8_MAX_K}], got {K}")
+    out_dtype = out.dtype if out is not None else out_dtype
+    if out_dtype not in _DTYPE_CODE:
+        raise TypeError(f"the output must be torch.bfloat16 or torch.float16, got {out_dtype}")
+    _need(a_scale, "a_scale", torch.float32, (M, _blocks128(K)), anywhere=True)
+    _need(b_scale, "b_scale", torch.float32, (_blocks128(N), _blocks128(K)), anywhere=True)
+    if bias is not None:
+        _need(bias, "bias", out_dtype, (N,), anywhere=True)
+    if out is not None and tuple(out.shape) != (M, N):
+        raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
+    _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
+    if out is None:
+        out = a.new_empty((M, N), dtype=out_dtype)
+        ldy = N
+    else:
+        ldy = _row_stride(out, "out")
+    at, lda, bt, ldb = a.data_ptr(), _row_stride(a, "a"), b.data_ptr(), _row_stride(b, "b")
+    size = int(lib().moe_fp8_scaled_mm_workspace_bytes(at, lda, bt, ldb, M, N, K))
+    if size < 0:
+        check(size, "moe_fp8_scaled_mm")
+    work = torch.empty(size, dtype=torch.uint8, device=a.device) if size else None
+    check(lib().moe_fp8_scaled_mm(at, lda, a_scale.data_ptr(), bt, ldb, b_scale.data_ptr(),
+                                  None if bias is None else bias.data_ptr(), M, N, K, _DTYPE_CODE[out_dtype],
+                                  out.data_ptr(), ldy, None if work is None else work.data_ptr(), _stream_handle()),
+          "moe_fp8_scaled_mm")
+    return out
+
+
+# ---------------------------------------------------------------------------
 # The gated feed-forward block in 16-bit floats, with its gradients
 # ---------------------------------------------------------------------------
 
