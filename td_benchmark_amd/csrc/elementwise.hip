@@ -251,15 +251,16 @@ MOE_DEVICE uint32_t slot_pair(float a, float b) {
 }
 
 // VEC: a thread has 4 columns of a token, and KMAX > 0 keeps its rows' loads in
-// flight together; else one column.
+// flight together; else one column.  n threads, fewer than 2^31, have work.
 template <bool FP16, bool VEC, int KMAX>
-__global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ d, int64_t ldd, int64_t T, int k,
+__global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ d, int64_t ldd, uint32_t n, int k,
                                                        int64_t H, uint16_t* __restrict__ y) {
   constexpr int W = VEC ? 4 : 1;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t cpr = H / W;
-  if (idx >= T * cpr) return;
-  const int64_t t = idx / cpr, c = (idx - t * cpr) * W;
+  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
+  if (idx >= n) return;
+  // a division of 64-bit words by each thread took half of the kernel's time
+  const uint32_t cpr = (uint32_t)(H / W), ti = idx / cpr;
+  const int64_t t = ti, c = (int64_t)(idx - ti * cpr) * W;
   const float* src = d + t * k * ldd + c;
   if constexpr (VEC) {
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -297,11 +298,11 @@ static int slot_sum(const float* d, int64_t ldd, int64_t T, int32_t k, int64_t H
     const float* dt = d + t * k * ldd;
     uint16_t* yt = y + t * H;
     if (!vec)
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, false, 0>), grid, threads, 0, st, dt, ldd, (uint32_t)(n * per_t), (int)k, H, yt);
     else if (k <= 8)
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 8>), grid, threads, 0, st, dt, ldd, (uint32_t)(n * per_t), (int)k, H, yt);
     else
-      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, dt, ldd, n, (int)k, H, yt);
+      hipLaunchKernelGGL((slot_sum_kernel<FP16, true, 0>), grid, threads, 0, st, dt, ldd, (uint32_t)(n * per_t), (int)k, H, yt);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
   }
   return kOk;

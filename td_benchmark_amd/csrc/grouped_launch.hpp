@@ -268,7 +268,7 @@ static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {
     using T = MmTile<128, 256, 4, 2, 3, 2, 64>;
     return dtype == MOE_FP16 ? launch_tile<Fp16, true, FORM, T>(g, st) : launch_tile<Bf16, false, FORM, T>(g, st);
   }
-  using T = MmTile<256, 256, 8, 4, 4, 1, 64>;
+  using T = MmTile<256, 256, 8, 4, 2, 1>;
   return dtype == MOE_FP16 ? launch_tile<Fp16, true, FORM, T>(g, st) : launch_tile<Bf16, false, FORM, T>(g, st);
 }
 

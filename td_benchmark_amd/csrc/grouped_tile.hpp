@@ -272,11 +272,25 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KB = (int)((length + STEP - 1) / STEP);
 
+  // A ring of two: the stage is handed over in two parts, A with the first half of
+  // every wave's columns, and their second half (below).
+  constexpr bool PHASED = KS == 2;
+  static_assert(!PHASED || (T::H == 2 && T::WN == 2 && T::CS == 8 && T::NW == 8 && TM == 256), "halves of a stage");
+
   // ---- addresses of this lane's part of the loads ----
-  // Instruction i of a wave is load wave + NW i of its operand.
+  // Instruction i of a wave is load wave + NW i of its operand; of a phased B, load
+  // wave + NW (i mod 2) of the first or second half of the columns, of which a
+  // column-staged half lies by itself.
   const uint8_t* a_ptr[T::NA_W];
   const uint8_t* b_ptr[T::NB_W];
-  constexpr int ACPR = TM / 8, BCPR = TN / 8;  // chunks of a column-staged row
+  constexpr int BW = PHASED ? TN / 2 : TN;            // columns of a column-staged part of B
+  constexpr int ACPR = TM / 8, BCPR = BW / 8;         // chunks of a column-staged row
+  auto b_load = [&](int i) {
+    if constexpr (!PHASED) return wave + T::NW * i;
+    else if constexpr (B_COLS) return wave + T::NW * (i & 1);
+    else return wave + T::NW * (2 * (i & 1) + (i >> 1));
+  };
+  auto b_place = [&](int i) { return T::A_BYTES + (PHASED && B_COLS ? (i >> 1) * (T::B_BYTES / 2) : 0) + b_load(i) * 1024; };
   const uint8_t* b_base = g.B + (WEIGHTS ? 0 : (int64_t)e * g.b_es * EB);
   const uint8_t* zeros = reinterpret_cast<const uint8_t*>(&kZeroChunk);
   constexpr int LPR = SB / 16, RPI = 64 / LPR;  // lanes of a row, rows of a load
@@ -284,6 +298,19 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // contraction row and column chunk of a column-staged load
   auto col_row = [&](int gi, int cpr) { return gi * (64 / cpr) + lane / cpr; };
   auto col_of = [&](int gi, int cpr) { return ((lane % cpr) ^ (col_swz<SB>(col_row(gi, cpr)) & (cpr - 1))) * 8; };
+  // Weights: the element of the contraction that a staged row of step kk holds.  A step
+  // of two instructions takes 32 elements with each; its step 0 is the contraction's
+  // last, partial run of 32 and, where the others' steps leave one over, the first run:
+  // the sum's order is that of steps of 32, so tiles of either length give the same bits.
+  constexpr bool PAIRS = WEIGHTS && T::H == 2;
+  const int64_t last_run = (length - 1) / 32 * 32;
+  const int spare = PAIRS && last_run % 64 ? 32 : 0;
+  auto element = [&](int kk, int row) -> int64_t {
+    const int h = PAIRS ? row >> 3 & 1 : 0, i = PAIRS ? (row >> 4) * 8 + (row & 7) : row;
+    if (kk == 0) return h ? i : last_run + i;
+    return (int64_t)(kk - 1) * STEP + spare + 32 * h + i;
+  };
+  auto in_first = [&](int row) { return PAIRS && (row >> 3 & 1) ? spare != 0 : element(0, row) < length; };
 #pragma unroll
   for (int i = 0; i < T::NA_W; ++i) {
     const int gi = wave + T::NW * i;
@@ -299,9 +326,11 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   }
 #pragma unroll
   for (int i = 0; i < T::NB_W; ++i) {
-    const int gi = wave + T::NW * i;
+    const int gi = b_load(i);
     if constexpr (B_COLS) {
-      const int64_t c = j0 + col_of(gi, BCPR);
+      int in = col_of(gi, BCPR);
+      if constexpr (PHASED) in = (in / (8 * T::CS)) * (16 * T::CS) + (i >> 1) * (8 * T::CS) + in % (8 * T::CS);
+      const int64_t c = j0 + in;
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
       if constexpr (COLUMNS) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
     } else {
@@ -317,20 +346,20 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       b_ptr[i] = b_base + j * g.sbj * EB + row_chunk(gi) * 16;
     }
   }
-  // Rows of A in subtiles without a slot are not fetched where every step waits for all of its loads.
-  const int a_rows = KS == 2 ? (nvalid + 15) / 16 * 16 : TM;
-
   // kWgrad: the slots of this lane's rows of a step, read ahead of its loads; square
   // tiles place both operands alike
+  constexpr bool SAME = TM == BW;
   uint32_t slot_a[T::NA_W], slot_b[T::NB_W];
   auto read_slots = [&](int kk) {
     if constexpr (FORM == kWgradDense) {  // row c of the contraction is slot c
-      const uint32_t c0 = (uint32_t)((kk == 0 ? KB - 1 : kk - 1) * STEP), end = (uint32_t)length - 1;
-      auto at = [&](int row) { return c0 + row < end ? c0 + row : end; };
+      auto at = [&](int row) {
+        const uint32_t c = (uint32_t)element(kk, row), end = (uint32_t)length - 1;
+        return c < end ? c : end;
+      };
 #pragma unroll
       for (int i = 0; i < T::NA_W; ++i) slot_a[i] = at(col_row(wave + T::NW * i, ACPR));
 #pragma unroll
-      for (int i = 0; i < T::NB_W; ++i) slot_b[i] = TM == TN ? slot_a[i < T::NA_W ? i : 0] : at(col_row(wave + T::NW * i, BCPR));
+      for (int i = 0; i < T::NB_W; ++i) slot_b[i] = SAME ? slot_a[i < T::NA_W ? i : 0] : at(col_row(b_load(i), BCPR));
       return;
     }
 #pragma unroll
@@ -338,7 +367,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       slot_a[i] = (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, ACPR)];
 #pragma unroll
     for (int i = 0; i < T::NB_W; ++i)
-      slot_b[i] = TM == TN ? slot_a[i < T::NA_W ? i : 0] : (uint32_t)smSlot[(kk & 7) * STEP + col_row(wave + T::NW * i, BCPR)];
+      slot_b[i] = SAME ? slot_a[i < T::NA_W ? i : 0] : (uint32_t)smSlot[(kk & 7) * STEP + col_row(b_load(i), BCPR)];
   };
 
   // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
@@ -352,16 +381,18 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     constexpr bool first = decltype(first_c)::value;
     const uint32_t dst = lds0 + stage * T::STAGE;
     const int left = first ? tail : STEP;
-    constexpr bool is_b = d < T::NB_W;
-    constexpr int i = is_b ? d : d - T::NB_W;
-    const int gi = wave + T::NW * i;
+    // B before A; phased: B's first half, A, B's second half
+    constexpr int first_b = PHASED ? T::NB_W / 2 : T::NB_W;
+    constexpr bool is_b = d < first_b || d >= first_b + T::NA_W;
+    constexpr int i = d < first_b ? d : is_b ? d - T::NA_W : d - first_b;
+    const int gi = is_b ? b_load(i) : wave + T::NW * i;
     if constexpr (WEIGHTS) {
       const uint8_t* p;
       if constexpr (is_b) p = b_ptr[i] + (uint64_t)(FORM == kWgrad ? slot_row(g, slot_b[i]) : slot_b[i]) * (uint32_t)(g.sbc * EB);
       else p = a_ptr[i] + (uint64_t)(FORM == kWgradTok ? slot_row(g, slot_a[i]) : slot_a[i]) * (uint32_t)(g.lda * EB);
-      if constexpr (first) p = col_row(gi, is_b ? BCPR : ACPR) < left ? p : zeros;
+      if constexpr (first) p = in_first(col_row(gi, is_b ? BCPR : ACPR)) ? p : zeros;
       if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
-        lds_load16(p, dst + (is_b ? T::A_BYTES : 0) + gi * 1024);
+        lds_load16(p, dst + (is_b ? b_place(i) : gi * 1024));
     } else if constexpr (is_b) {
       const uint8_t* p = b_ptr[i];
       if constexpr (first) {
@@ -371,7 +402,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       } else {
         b_ptr[i] += b_step;
       }
-      if (T::NB % T::NW == 0 || gi < T::NB) lds_load16(p, dst + T::A_BYTES + gi * 1024);
+      if (T::NB % T::NW == 0 || gi < T::NB) lds_load16(p, dst + b_place(i));
     } else {
       const uint8_t* p = a_ptr[i];
       if constexpr (first) {
@@ -380,7 +411,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       } else {
         a_ptr[i] += SB;
       }
-      if ((T::NA % T::NW == 0 || gi < T::NA) && RPI * gi < a_rows) lds_load16(p, dst + gi * 1024);
+      if (T::NA % T::NW == 0 || gi < T::NA) lds_load16(p, dst + gi * 1024);
     }
   };
   // Loads [from, to) of step kk.
@@ -394,9 +425,8 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   constexpr int kAhead = 3;
   auto issue_ids = [&](int kk) {
     if (wave == T::NW - 1 && kk < KB && lane < STEP) {
-      const int64_t c0 = kk == 0 ? (int64_t)(KB - 1) * STEP : (int64_t)(kk - 1) * STEP;
-      const int64_t c = c0 + lane < length ? c0 + lane : length - 1;
-      lds_load4(g.sorted + pos0 + c, (uint32_t)(uintptr_t)(lds_ptr)smem + (kk & 7) * STEP * 4);
+      const int64_t c = element(kk, lane);
+      lds_load4(g.sorted + pos0 + (c < length ? c : length - 1), (uint32_t)(uintptr_t)(lds_ptr)smem + (kk & 7) * STEP * 4);
     }
   };
 
@@ -411,7 +441,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     return (uint32_t)(t_row * w * 2 + (((base / 8 + ((fr & 3) >> 1)) ^ (col_swz<SB>(t_row) & (w / 8 - 1))) << 4) + (fr & 1) * 8);
   };
   const uint32_t a_lane = A_COLS ? by_col(row_base, TM) : row_base * SB + by_row;
-  const uint32_t b_lane = T::A_BYTES + (B_COLS ? by_col(col_base, TN) : col_base * SB + by_row);
+  const uint32_t b_lane = T::A_BYTES + (B_COLS ? by_col(PHASED ? col_base / 2 : col_base, BW) : col_base * SB + by_row);
 
   typename OP::Acc acc[T::RS][T::CS] = {};
   int ra = (nvalid - row_base + 15) / 16;
@@ -439,7 +469,17 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // slots before the step's end, when every fragment of this stage has been read:
   // the last two slots' instructions cover the reads of the next stage's first
   // fragments, and this stage's buffer is filled again from there on, a load a slot.
-  constexpr int NQ = T::H * T::CS;
+  //
+  // Phased: the first half of a step's slots takes the first half of the columns, both
+  // instructions along the contraction, and the second half the other, with the rows'
+  // fragments in registers all the step.  A second barrier, two slots before the
+  // middle, hands over the second half of the columns; behind it the stage's A and
+  // first half of B are filled again, behind the step's barrier its second half, so
+  // that every load has one and a half steps to arrive and a stage's worth of younger
+  // ones stays in flight at each wait.
+  constexpr int NQ = T::H * T::CS, MID = NQ / 2 - 2;
+  constexpr auto half_of = [](int q) { return PHASED ? q % (NQ / 2) / (T::CS / 2) : q / T::CS; };
+  constexpr auto column_of = [](int q) { return PHASED ? q / (NQ / 2) * (T::CS / 2) + q % (T::CS / 2) : q % T::CS; };
   constexpr int DPQ = (ND + NQ - 1) / NQ;  // loads of a slot
   static_assert(NQ >= 4 && NQ % 4 == 0, "four fragment registers in turn");
   auto kloop = [&](auto ra_c) {
@@ -453,12 +493,19 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     };
     auto read_b = [&](int stage, int q) {
       const uint32_t st = lds0 + stage * T::STAGE;
-      const int h = q / T::CS, c = q % T::CS;
-      if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 8 * TN * 2, TN * 2);
+      const int h = half_of(q), c = column_of(q);
+      if constexpr (B_COLS && PHASED) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c % (T::CS / 2) * 32)) + c / (T::CS / 2) * (T::B_BYTES / 2) + h * 8 * BW * 2, BW * 2);
+      else if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 8 * TN * 2, TN * 2);
       else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 16)) + c * 16 * SB);
     };
     // stage 0; of the others every wave has at least so many loads behind it
-    mm_wait_stages<KS - 1, KS == 2 ? T::NB / T::NW : T::VM>(KB - 1);
+    constexpr int VM2 = T::NB / T::NW / 2, VM1 = T::VM - VM2;  // loads of the two parts
+    if constexpr (PHASED) {
+      if (KB > 1) mm_wait<VM2 + T::VM>();
+      else mm_wait<VM2>();
+    } else {
+      mm_wait_stages<KS - 1, T::VM>(KB - 1);
+    }
     mm_barrier();
     if constexpr (RA > 0) {
 #pragma unroll
@@ -475,7 +522,12 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         constexpr int Q = decltype(qc)::value;
         if constexpr (Q == NQ - 2) {
           if (kk + 1 < KB) {
-            mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
+            if constexpr (PHASED) {
+              if (kk + 2 < KB) mm_wait<VM2 + VM1>();
+              else mm_wait<VM2>();
+            } else {
+              mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
+            }
             mm_barrier();
             if constexpr (RA > 0) {
 #pragma unroll
@@ -483,7 +535,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
               read_b(next, 0);
               read_b(next, 1);
             }
-            if constexpr (WEIGHTS) {
+            if constexpr (WEIGHTS && !PHASED) {
               if (kk + KS < KB) {
                 read_slots(kk + KS);
                 if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
@@ -491,18 +543,40 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
             }
           }
         }
+        if constexpr (PHASED && Q == MID) {
+          if (kk + 1 < KB) mm_wait<T::VM>();
+          else mm_wait<0>();
+          mm_barrier();
+          if constexpr (WEIGHTS) {
+            if (kk + KS < KB) {
+              read_slots(kk + KS);
+              if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
+            }
+          }
+        }
         if constexpr (RA > 0 && Q < NQ - 2) {
           read_b(stage, Q + 2);
+          // phased: the second half's rows in the first two slots
+          if constexpr (PHASED && Q < 2) {
+#pragma unroll
+            for (int r = 0; r < RA; ++r)
+              if ((r < 2) == (Q == 0)) read_a(1, stage, 1, r);
+          }
           // the second half's rows: one a slot up to two slots ahead, or together
-          if constexpr (T::H == 2 && T::CS > RA + 1 && Q + RA >= T::CS - 1 && Q < T::CS - 1) read_a(1, stage, 1, Q + RA - (T::CS - 1));
-          if constexpr (T::H == 2 && T::CS <= RA + 1 && Q == 0) {
+          if constexpr (!PHASED && T::H == 2 && T::CS > RA + 1 && Q + RA >= T::CS - 1 && Q < T::CS - 1) read_a(1, stage, 1, Q + RA - (T::CS - 1));
+          if constexpr (!PHASED && T::H == 2 && T::CS <= RA + 1 && Q == 0) {
 #pragma unroll
             for (int r = 0; r < RA; ++r) read_a(1, stage, 1, r);
           }
         }
         // loads of stage kk + KS in this step's last two slots, of the stage before it in the others
-        constexpr int from = (Q + 2) % NQ * DPQ, to = from + DPQ < ND ? from + DPQ : ND;
-        if constexpr (from < ND) {
+        constexpr int from = PHASED ? (Q >= NQ - 2 ? Q - (NQ - 2) + VM1 : Q - MID) : (Q + 2) % NQ * DPQ;
+        constexpr int to = PHASED ? from + 1 : from + DPQ < ND ? from + DPQ : ND;
+        if constexpr (PHASED) {  // of stage kk + KS
+          if constexpr ((from >= 0 && from < VM1) || Q >= NQ - 2) {
+            if (kk + KS < KB) loads(kk + KS, stage, std::integral_constant<int, from>{}, std::integral_constant<int, to>{}, std::false_type{});
+          }
+        } else if constexpr (from < ND) {
           const std::integral_constant<int, from> f;
           const std::integral_constant<int, to> t;
           if constexpr (Q >= NQ - 2) {
@@ -514,7 +588,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         // the reads stay ahead of the instructions, which the compiler would undo
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (RA > 0) {
-          constexpr int at = T::H == 2 ? Q / T::CS : P, c = Q % T::CS;
+          constexpr int at = T::H == 2 ? half_of(Q) : P, c = column_of(Q);
 #pragma unroll
           for (int r = 0; r < RA; ++r) acc[r][c] = OP::mfma(bf[Q & 3], af[at][r], acc[r][c]);
         }
