@@ -529,18 +529,20 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
               mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
             }
             mm_barrier();
-            if constexpr (RA > 0) {
-#pragma unroll
-              for (int r = 0; r < RA; ++r) read_a(T::H == 2 ? 0 : P ^ 1, next, 0, r);
-              read_b(next, 0);
-              read_b(next, 1);
-            }
             if constexpr (WEIGHTS && !PHASED) {
               if (kk + KS < KB) {
                 read_slots(kk + KS);
                 if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
               }
             }
+          }
+          // behind the last step nothing uses these: under the condition, the compiler
+          // would wait for them before this slot's instructions
+          if constexpr (RA > 0) {
+#pragma unroll
+            for (int r = 0; r < RA; ++r) read_a(T::H == 2 ? 0 : P ^ 1, next, 0, r);
+            read_b(next, 0);
+            read_b(next, 1);
           }
         }
         if constexpr (PHASED && Q == MID) {
