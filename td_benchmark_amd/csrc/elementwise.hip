@@ -250,37 +250,42 @@ MOE_DEVICE uint32_t slot_pair(float a, float b) {
   else return pack_bf16x2(a, b);
 }
 
-// VEC: a thread has 4 columns of a token, and KMAX > 0 keeps its rows' loads in
-// flight together; else one column.  n threads, fewer than 2^31, have work.
+// VEC: a thread has 4 columns of a token at a time, and KMAX > 0 keeps its rows' loads
+// in flight together; else one column.  n pieces, fewer than 2^31.  The workgroups are
+// those that the CUs hold and go through the pieces in turn: a workgroup for each 256
+// pieces read 3.1 TB/s, the launch of workgroups being the limit, and so 6.0 (4093 tokens
+// of 8 slots, 4096 columns: 180 and 94 us).
+constexpr int kSlotSumGrid = 2048;
+
 template <bool FP16, bool VEC, int KMAX>
 __global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ d, int64_t ldd, uint32_t n, int k,
                                                        int64_t H, uint16_t* __restrict__ y) {
   constexpr int W = VEC ? 4 : 1;
-  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
-  if (idx >= n) return;
-  // a division of 64-bit words by each thread took half of the kernel's time
-  const uint32_t cpr = (uint32_t)(H / W), ti = idx / cpr;
-  const int64_t t = ti, c = (int64_t)(idx - ti * cpr) * W;
-  const float* src = d + t * k * ldd + c;
-  if constexpr (VEC) {
-    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (KMAX > 0) {
-      v4f rows[KMAX];
+  const uint32_t cpr = (uint32_t)(H / W);
+  for (uint32_t idx = blockIdx.x * 256 + threadIdx.x; idx < n; idx += gridDim.x * 256) {
+    const uint32_t ti = idx / cpr;
+    const int64_t t = ti, c = (int64_t)(idx - ti * cpr) * W;
+    const float* src = d + t * k * ldd + c;
+    if constexpr (VEC) {
+      v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (KMAX > 0) {
+        v4f rows[KMAX];
 #pragma unroll
-      for (int i = 0; i < KMAX; ++i)
-        if (i < k) rows[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + i * ldd));
+        for (int i = 0; i < KMAX; ++i)
+          if (i < k) rows[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + i * ldd));
 #pragma unroll
-      for (int i = 0; i < KMAX; ++i)
-        if (i < k) acc = acc + rows[i];
+        for (int i = 0; i < KMAX; ++i)
+          if (i < k) acc = acc + rows[i];
+      } else {
+        for (int i = 0; i < k; ++i) acc = acc + *reinterpret_cast<const v4f*>(src + i * ldd);
+      }
+      const v2u out = {slot_pair<FP16>(acc[0], acc[1]), slot_pair<FP16>(acc[2], acc[3])};
+      *reinterpret_cast<v2u*>(y + t * H + c) = out;
     } else {
-      for (int i = 0; i < k; ++i) acc = acc + *reinterpret_cast<const v4f*>(src + i * ldd);
+      float acc = 0.0f;
+      for (int i = 0; i < k; ++i) acc += src[i * ldd];
+      y[t * H + c] = (uint16_t)slot_pair<FP16>(acc, 0.0f);
     }
-    const v2u out = {slot_pair<FP16>(acc[0], acc[1]), slot_pair<FP16>(acc[2], acc[3])};
-    *reinterpret_cast<v2u*>(y + t * H + c) = out;
-  } else {
-    float acc = 0.0f;
-    for (int i = 0; i < k; ++i) acc += src[i * ldd];
-    y[t * H + c] = (uint16_t)slot_pair<FP16>(acc, 0.0f);
   }
 }
 
@@ -294,7 +299,8 @@ static int slot_sum(const float* d, int64_t ldd, int64_t T, int32_t k, int64_t H
   const dim3 threads(256);
   for (int64_t t = 0; t < T; t += part) {
     const int64_t n = T - t < part ? T - t : part;
-    const dim3 grid((unsigned)((n * per_t + 255) / 256));
+    const int64_t groups = (n * per_t + 255) / 256;
+    const dim3 grid((unsigned)(groups < kSlotSumGrid ? groups : kSlotSumGrid));
     const float* dt = d + t * k * ldd;
     uint16_t* yt = y + t * H;
     if (!vec)
