@@ -35,31 +35,61 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const float* __restrict__
 // ---- rows that are not whole 16-byte chunks --------------------------------------
 // dst [B][rows_d][cols_d] = src [B][rows_s][cols_s] with zeros past its ends, or its
 // first rows and columns: widths that the products cannot take are copied to whole
-// chunks and their results back.  8 columns a thread, one by one on the odd side.
+// chunks and their results back, all of a pass's operands in one launch.  A wave a row,
+// 8 columns a lane: the odd side goes element by element, the other in 16-byte chunks.
 struct Copy {
   const uint16_t* src;
   uint16_t* dst;
   int64_t B, rows_s, cols_s, ld_s, batch_s, rows_d, cols_d, ld_d, batch_d;
 };
-__global__ __launch_bounds__(256) void copy_kernel(Copy c) {
-  const int64_t cpr = (c.cols_d + 7) / 8, n = c.B * c.rows_d * cpr;
-  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
-    const int64_t r = idx / cpr, col = (idx - r * cpr) * 8, b = r / c.rows_d, row = r - b * c.rows_d;
-    const uint16_t* src = c.src + b * c.batch_s + row * c.ld_s + col;
-    uint16_t* dst = c.dst + b * c.batch_d + row * c.ld_d + col;
+struct Copies {
+  Copy c[4];
+  int64_t first[5];  // rows of the copies before each
+  int n = 0;
+  void add(const Copy& x) {
+    if (n == 0) first[0] = 0;
+    c[n] = x;
+    first[n + 1] = first[n] + x.B * x.rows_d;
+    ++n;
+  }
+};
+__global__ __launch_bounds__(256) void copy_kernel(Copies all) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = all.first[all.n];
+  for (int64_t r0 = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r0 < rows; r0 += (int64_t)gridDim.x * 4) {
+    int i = 0;
+    while (i + 1 < all.n && r0 >= all.first[i + 1]) ++i;
+    const Copy& c = all.c[i];
+    const int64_t r = r0 - all.first[i], b = r / c.rows_d, row = r - b * c.rows_d;
+    const uint16_t* src = c.src + b * c.batch_s + row * c.ld_s;
+    uint16_t* dst = c.dst + b * c.batch_d + row * c.ld_d;
+    const int64_t end = row < c.rows_s ? c.cols_s : 0;  // columns of the row that there are
+    const bool from16 = ((uintptr_t)src & 15) == 0, to16 = ((uintptr_t)dst & 15) == 0;
+    for (int64_t col = lane * 8; col < c.cols_d; col += 512) {
+      uint32_t v[4] = {};
+      if (from16 && col + 8 <= end) {
+        const v4i x = *reinterpret_cast<const v4i*>(src + col);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < c.cols_d) dst[i] = row < c.rows_s && col + i < c.cols_s ? src[i] : (uint16_t)0;
+        for (int k = 0; k < 4; ++k) v[k] = (uint32_t)x[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (col + k < end) v[k / 2] |= (uint32_t)src[col + k] << (16 * (k & 1));
+      }
+      if (to16 && col + 8 <= c.cols_d) {
+        *reinterpret_cast<v4i*>(dst + col) = (v4i){(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (col + k < c.cols_d) dst[col + k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+      }
+    }
   }
 }
-static unsigned grid_for(int64_t threads) {
-  const int64_t g = (threads + 255) / 256;
-  return (unsigned)(g < 8192 ? g : 8192);
-}
-static int launch_copy(const Copy& c, hipStream_t st) {
-  const int64_t n = c.B * c.rows_d * ((c.cols_d + 7) / 8);
-  if (n == 0) return kOk;
-  hipLaunchKernelGGL(copy_kernel, dim3(grid_for(n)), dim3(256), 0, st, c);
+static int launch_copies(const Copies& c, hipStream_t st) {
+  if (c.n == 0 || c.first[c.n] == 0) return kOk;
+  const int64_t groups = (c.first[c.n] + 3) / 4;
+  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, c);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
@@ -95,23 +125,23 @@ struct Ffn {
   int64_t w2_bytes() const { return up_to_256(2 * f.E * Ip * Hp); }
   int64_t rows_bytes() const { return f.top_k > 1 ? up_to_256(4 * S * Hp) : 0; }
 
-  int pad_rows(const void* x, int64_t ldx, void* to) const {
-    return launch_copy({(const uint16_t*)x, (uint16_t*)to, 1, f.T, f.H, ldx, 0, f.T, Hp, Hp, 0}, st);
+  Copy pad_rows(const void* x, int64_t ldx, void* to) const {
+    return {(const uint16_t*)x, (uint16_t*)to, 1, f.T, f.H, ldx, 0, f.T, Hp, Hp, 0};
   }
-  int pad_w13(const void* w, void* to) const {
-    return launch_copy({(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, f.H, f.I * f.H, Ip, Hp, Hp, Ip * Hp}, st);
+  Copy pad_w13(const void* w, void* to) const {
+    return {(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, f.H, f.I * f.H, Ip, Hp, Hp, Ip * Hp};
   }
-  int pad_w2(const void* w, void* to) const {
-    return launch_copy({(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, f.I, f.H * f.I, Hp, Ip, Ip, Hp * Ip}, st);
+  Copy pad_w2(const void* w, void* to) const {
+    return {(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, f.I, f.H * f.I, Hp, Ip, Ip, Hp * Ip};
   }
-  int crop_rows(const void* y, void* to) const {
-    return launch_copy({(const uint16_t*)y, (uint16_t*)to, 1, f.T, f.H, Hp, 0, f.T, f.H, f.H, 0}, st);
+  Copy crop_rows(const void* y, void* to) const {
+    return {(const uint16_t*)y, (uint16_t*)to, 1, f.T, f.H, Hp, 0, f.T, f.H, f.H, 0};
   }
-  int crop_w13(const void* w, void* to) const {
-    return launch_copy({(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, Hp, Ip * Hp, f.I, f.H, f.H, f.I * f.H}, st);
+  Copy crop_w13(const void* w, void* to) const {
+    return {(const uint16_t*)w, (uint16_t*)to, 2 * f.E, f.I, f.H, Hp, Ip * Hp, f.I, f.H, f.H, f.I * f.H};
   }
-  int crop_w2(const void* w, void* to) const {
-    return launch_copy({(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, Ip, Hp * Ip, f.H, f.I, f.I, f.H * f.I}, st);
+  Copy crop_w2(const void* w, void* to) const {
+    return {(const uint16_t*)w, (uint16_t*)to, f.E, f.H, f.I, Ip, Hp * Ip, f.H, f.I, f.I, f.H * f.I};
   }
 
   // A product over the slots, of J columns.
@@ -224,19 +254,21 @@ static int ffn_forward(const Ffn& b, void* y) {
   const Forward ws(b, parts);
   const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
   int64_t ldx = f.ldx;
+  Copies in;
   if (ws.x) {
-    MOE_TRY(b.pad_rows(x, ldx, ws.x));
+    in.add(b.pad_rows(x, ldx, ws.x));
     x = ws.x;
     ldx = b.Hp;
   }
   if (ws.w13) {
-    MOE_TRY(b.pad_w13(w13, ws.w13));
+    in.add(b.pad_w13(w13, ws.w13));
     w13 = ws.w13;
   }
   if (ws.w2) {
-    MOE_TRY(b.pad_w2(w2, ws.w2));
+    in.add(b.pad_w2(w2, ws.w2));
     w2 = ws.w2;
   }
+  MOE_TRY(launch_copies(in, b.st));
   MmArgs g = b.args(b.Ip);
   g.A = (const uint8_t*)x;
   g.B = (const uint8_t*)w13;
@@ -257,7 +289,10 @@ static int ffn_forward(const Ffn& b, void* y) {
   }
   const bool direct = b.Hp == f.H && aligned(y, 16);
   MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, false, direct ? y : ws.y));
-  return direct ? kOk : b.crop_rows(ws.y, y);
+  if (direct) return kOk;
+  Copies out;
+  out.add(b.crop_rows(ws.y, y));
+  return launch_copies(out, b.st);
 }
 
 static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void* dw2, float* dweight) {
@@ -266,20 +301,27 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
   const Backward ws(b, parts);
   const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
   int64_t ldx = f.ldx;
+  const bool rows = dx || dw13 || dweight;  // whether the gradient of the projections is needed
+  Copies in, out;
   if (b.Hp != f.H || !aligned(dy, 16)) {
-    MOE_TRY(b.pad_rows(dy, f.H, ws.dy));
+    in.add(b.pad_rows(dy, f.H, ws.dy));
     dy = ws.dy;
   }
   if (ws.x && dw13) {
-    MOE_TRY(b.pad_rows(x, ldx, ws.x));
+    in.add(b.pad_rows(x, ldx, ws.x));
     x = ws.x;
     ldx = b.Hp;
   }
-  if (dx || dw13 || dweight) {
-    if (ws.w2) {
-      MOE_TRY(b.pad_w2(w2, ws.w2));
-      w2 = ws.w2;
-    }
+  if (ws.w2 && rows) {
+    in.add(b.pad_w2(w2, ws.w2));
+    w2 = ws.w2;
+  }
+  if (ws.w13 && dx) {
+    in.add(b.pad_w13(w13, ws.w13));
+    w13 = ws.w13;
+  }
+  MOE_TRY(launch_copies(in, b.st));
+  if (rows) {
     if (b.S > 0) {
       MmArgs g = b.args(b.Ip);
       g.A = (const uint8_t*)dy;
@@ -303,32 +345,28 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
     }
   }
   if (dx && b.S > 0) {
-    if (ws.w13) {
-      MOE_TRY(b.pad_w13(w13, ws.w13));
-      w13 = ws.w13;
-    }
     if (f.top_k > 1) {
       MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, true, ws.rows));
       MOE_TRY(b.token_rows((const float*)ws.rows, dx));
     } else {
       const bool direct = b.Hp == f.H && aligned(dx, 16);
       MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, false, direct ? dx : ws.dx));
-      if (!direct) MOE_TRY(b.crop_rows(ws.dx, dx));
+      if (!direct) out.add(b.crop_rows(ws.dx, dx));
     }
   }
   if (dw13) {
     const bool direct = !b.odd && aligned(dw13, 16);
     if (!direct && !ws.dw13) return kErrBadShape;
     MOE_TRY(b.weights(ws.dgu, 2 * b.Ip, x, ldx, 2 * b.Ip, b.Hp, false, direct ? dw13 : ws.dw13));
-    if (!direct) MOE_TRY(b.crop_w13(ws.dw13, dw13));
+    if (!direct) out.add(b.crop_w13(ws.dw13, dw13));
   }
   if (dw2) {
     const bool direct = !b.odd && aligned(dw2, 16);
     if (!direct && !ws.dw2) return kErrBadShape;
     MOE_TRY(b.weights(dy, b.Hp, f.h, b.Ip, b.Hp, b.Ip, true, direct ? dw2 : ws.dw2));
-    if (!direct) MOE_TRY(b.crop_w2(ws.dw2, dw2));
+    if (!direct) out.add(b.crop_w2(ws.dw2, dw2));
   }
-  return kOk;
+  return launch_copies(out, b.st);
 }
 
 }  // namespace moe
