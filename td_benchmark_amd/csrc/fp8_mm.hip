@@ -51,6 +51,16 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   const int nvalid = (int)(g.S - i0 < TM ? g.S - i0 : TM);
   const int KB = (int)((g.Cn + 127) / 128);
   const int tail = (int)(g.Cn - (int64_t)(KB - 1) * 128);
+  // A ring of two is handed over in parts: a with the first half of every wave's columns
+  // of b, and their second half (below), which is the second half of a wave's loads of b.
+  constexpr bool PHASED = KS == 2;
+  static_assert(!PHASED || (T::NB % NW == 0 && T::NA % NW == 0 && T::NB_W % 2 == 0 && CS == 8), "halves of a stage");
+  constexpr int BH = PHASED ? T::NB_W / 2 : T::NB_W;
+  auto b_load = [&](int i) {
+    if constexpr (!PHASED) return wave + NW * i;
+    const int n = wave + NW * (i % BH);
+    return n / CS * 2 * CS + i / BH * CS + n % CS;
+  };
 
   // A step's 1 KiB loads hold 8 rows of 128 bytes; rows past the ends repeat the last one.
   uint32_t a_off[T::NA_W], b_off[T::NB_W];
@@ -63,7 +73,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   const int cols = (int)(g.J - j0 < TN ? g.J - j0 : TN);
 #pragma unroll
   for (int i = 0; i < T::NB_W; ++i) {
-    const int gi = wave + NW * i, row = 8 * gi + lane / 8;
+    const int gi = b_load(i), row = 8 * gi + lane / 8;
     b_off[i] = (uint32_t)((row < cols ? row : cols - 1) * g.sbj) + row_chunk(gi) * 16;
   }
   const uint8_t* a_base = g.A + i0 * g.lda;
@@ -75,9 +85,10 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   constexpr int ND = T::NA_W + T::NB_W, DPQ = (ND + CS - 1) / CS;
   auto load = [&](int kk, int stage, auto dc, auto first_c) {
     constexpr int d = decltype(dc)::value;
-    constexpr bool first = decltype(first_c)::value, is_b = d < T::NB_W;
-    constexpr int i = is_b ? d : d - T::NB_W;
-    const int gi = wave + NW * i;
+    // b before a; phased: b's first half, a, b's second half
+    constexpr bool first = decltype(first_c)::value, is_b = d < BH || d >= BH + T::NA_W;
+    constexpr int i = d < BH ? d : is_b ? d - T::NA_W : d - BH;
+    const int gi = is_b ? b_load(i) : wave + NW * i;
     if ((is_b ? T::NB : T::NA) % NW != 0 && gi >= (is_b ? T::NB : T::NA)) return;
     const uint32_t dst = lds0 + stage * T::STAGE + (is_b ? T::A_BYTES : 0) + gi * 1024;
     const int64_t at = (int64_t)(first ? KB - 1 : kk - 1) * 128;
@@ -117,15 +128,23 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
   v4f acc[RS][CS] = {};
   const std::integral_constant<int, 0> none;
   const std::integral_constant<int, ND> all;
+  const std::integral_constant<int, PHASED ? ND - BH : ND> ahead;  // phased: not the second half of b
   load_scales(0);
   loads(0, 0, none, all, std::true_type{});
 #pragma unroll
   for (int s = 1; s < KS; ++s)
-    if (s < KB) loads(s, s, none, all, std::false_type{});
+    if (s < KB) loads(s, s, none, ahead, std::false_type{});
 
   // A step is CS slots of RS instructions.  The weights' fragment of a slot is read one
   // slot ahead, the rows' of a step as the last slot of the step before is done with
   // its own.  A block's dot is added to the sum LAG instructions behind its own.
+  //
+  // Phased: the barrier before the last slot hands over the next step's a and first half
+  // of b, one before the middle this step's second half.  Behind the middle one the
+  // second half of the next step is loaded and a of the one after, behind the last one
+  // its first half of b: what they overwrite was used by instructions before their
+  // barrier, and every load has a step or more to arrive.  With one hand-over a step, its
+  // loads spread over the step before, 8192 x 7168 to 4096 took 254 us.
   constexpr int LAG = RS >= 2 ? 2 : 1;
   v8i af[RS], bf[2];
   v4f dot[LAG];
@@ -147,7 +166,12 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     for (int r = 0; r < RS; ++r) sa[r] = *(lds_float)(uintptr_t)(at + (row_base + r * 16 + fr) * 16);
     sb = *(lds_float)(uintptr_t)(at + (TM + b_group) * 16);
   };
-  mm_wait_stages<KS - 1, T::VM>(KB - 1);
+  if constexpr (PHASED) {
+    if (KB > 1) mm_wait<2 * BH + T::NA_W>();
+    else mm_wait<BH>();
+  } else {
+    mm_wait_stages<KS - 1, T::VM>(KB - 1);
+  }
   mm_barrier();
 #pragma unroll
   for (int r = 0; r < RS; ++r) read_a(0, r);
@@ -159,10 +183,26 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
     const int next = stage == KS - 1 ? 0 : stage + 1, prev = stage == 0 ? KS - 1 : stage - 1;
     auto slot = [&](auto qc) {
       constexpr int Q = decltype(qc)::value;
+      constexpr int MID = CS / 2 - 1;
+      // the scales that this step loads, before the other loads, are two or three a wave
+      const bool more = (kk & 3) == 1 && 4 * (kk / 4 + 1) < KB;
+      if constexpr (PHASED && Q == MID) {
+        if (kk + 1 >= KB) mm_wait<0>();
+        else if (more) mm_wait<BH + T::NA_W + 2>();
+        else mm_wait<BH + T::NA_W>();
+        mm_barrier<15>();
+      }
       if constexpr (Q == CS - 1) {
         // behind the last step nothing uses what is read here
-        mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
-        mm_barrier();
+        if constexpr (PHASED) {
+          if (kk + 2 >= KB) mm_wait<BH>();
+          else if (more) mm_wait<BH + T::NA_W + 2>();
+          else mm_wait<BH + T::NA_W>();
+          mm_barrier<15>();
+        } else {
+          mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
+          mm_barrier();
+        }
         read_b(next, 0, 0);
       } else {
         read_b(stage, Q + 1, (Q + 1) & 1);
@@ -170,15 +210,27 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::W
       if constexpr (Q == 0) {
         if ((kk & 3) == 1 && 4 * (kk / 4 + 1) < KB) load_scales(kk / 4 + 1);
       }
-      // loads of stage kk + KS in this step's last slot, of the stage before it in the others
-      constexpr int from = (Q + 1) % CS * DPQ, to = from + DPQ < ND ? from + DPQ : ND;
-      if constexpr (from < ND) {
-        const std::integral_constant<int, from> fc;
-        const std::integral_constant<int, to> tc;
-        if constexpr (Q == CS - 1) {
-          if (kk + KS < KB) loads(kk + KS, stage, fc, tc, std::false_type{});
-        } else {
-          if (refill) loads(kk - 1 + KS, prev, fc, tc, std::false_type{});
+      if constexpr (PHASED) {
+        auto part = [&](int kk_to, int to, auto from, auto until) {
+          if (kk_to < KB) loads(kk_to, to, from, until, std::false_type{});
+        };
+        constexpr int A0 = BH, PER = (T::NA_W + CS - 2 - MID - 1) / (CS - 2 - MID);  // loads of a in each slot between
+        if constexpr (Q == MID) part(kk + 1, next, ahead, all);
+        else if constexpr (Q == CS - 1) part(kk + 2, stage, none, std::integral_constant<int, A0>{});
+        else if constexpr (Q > MID && (Q - MID - 1) * PER < T::NA_W)
+          part(kk + 2, stage, std::integral_constant<int, A0 + (Q - MID - 1) * PER>{},
+               std::integral_constant<int, A0 + ((Q - MID) * PER < T::NA_W ? (Q - MID) * PER : T::NA_W)>{});
+      } else {
+        // loads of stage kk + KS in this step's last slot, of the stage before it in the others
+        constexpr int from = (Q + 1) % CS * DPQ, to = from + DPQ < ND ? from + DPQ : ND;
+        if constexpr (from < ND) {
+          const std::integral_constant<int, from> fc;
+          const std::integral_constant<int, to> tc;
+          if constexpr (Q == CS - 1) {
+            if (kk + KS < KB) loads(kk + KS, stage, fc, tc, std::false_type{});
+          } else {
+            if (refill) loads(kk - 1 + KS, prev, fc, tc, std::false_type{});
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);

@@ -80,7 +80,9 @@ MOE_DEVICE int col_swz(int row) {
   return ((row & 3) << 1) | ((SB == 128 ? row >> 1 : row) & 8);
 }
 
-MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// A barrier, behind which all but the wave's last LGKM reads of LDS have arrived (15: any).
+template <int LGKM = 0>
+MOE_DEVICE void mm_barrier() { asm volatile("s_waitcnt lgkmcnt(%0)\n\ts_barrier" ::"n"(LGKM) : "memory"); }
 template <int N>
 MOE_DEVICE void mm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // Waits for the oldest stage in flight: of the `younger` ones behind it, at most
