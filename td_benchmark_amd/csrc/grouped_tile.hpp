@@ -517,15 +517,17 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     }
     int stage = 0;
     // P: with one instruction a step, which of the two sets of row fragments it takes
-    auto step = [&](int kk, auto pc) {
+    // STEADY: the steps whose loads there are, without a branch for each
+    auto step = [&](int kk, auto pc, auto steady_c) {
       constexpr int P = decltype(pc)::value;
+      constexpr bool STEADY = decltype(steady_c)::value;
       const int next = stage == KS - 1 ? 0 : stage + 1, prev = stage == 0 ? KS - 1 : stage - 1;
       auto slot = [&](auto qc) {
         constexpr int Q = decltype(qc)::value;
         if constexpr (Q == NQ - 2) {
-          if (kk + 1 < KB) {
+          if (STEADY || kk + 1 < KB) {
             if constexpr (PHASED) {
-              if (kk + 2 < KB) mm_wait<VM2 + VM1>();
+              if (STEADY || kk + 2 < KB) mm_wait<VM2 + VM1>();
               else mm_wait<VM2>();
             } else {
               mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
@@ -548,11 +550,11 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
           }
         }
         if constexpr (PHASED && Q == MID) {
-          if (kk + 1 < KB) mm_wait<T::VM>();
+          if (STEADY || kk + 1 < KB) mm_wait<T::VM>();
           else mm_wait<0>();
           mm_barrier();
           if constexpr (WEIGHTS) {
-            if (kk + KS < KB) {
+            if (STEADY || kk + KS < KB) {
               read_slots(kk + KS);
               if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
             }
@@ -578,7 +580,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         constexpr int to = PHASED ? from + 1 : from + DPQ < ND ? from + DPQ : ND;
         if constexpr (PHASED) {  // of stage kk + KS
           if constexpr ((from >= 0 && from < VM1) || Q >= NQ - 2) {
-            if (kk + KS < KB) loads(kk + KS, stage, std::integral_constant<int, from>{}, std::integral_constant<int, to>{}, std::false_type{});
+            if (STEADY || kk + KS < KB) loads(kk + KS, stage, std::integral_constant<int, from>{}, std::integral_constant<int, to>{}, std::false_type{});
           }
         } else if constexpr (from < ND) {
           const std::integral_constant<int, from> f;
@@ -604,11 +606,14 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       stage = next;
     };
     if constexpr (T::H == 2) {
-      for (int kk = 0; kk < KB; ++kk) step(kk, std::integral_constant<int, 0>{});
+      int kk = 0;
+      if constexpr (PHASED && RA == T::RS)
+        for (; kk + KS < KB; ++kk) step(kk, std::integral_constant<int, 0>{}, std::true_type{});
+      for (; kk < KB; ++kk) step(kk, std::integral_constant<int, 0>{}, std::false_type{});
     } else {
       for (int kk = 0; kk < KB; kk += 2) {
-        step(kk, std::integral_constant<int, 0>{});
-        if (kk + 1 < KB) step(kk + 1, std::integral_constant<int, 1>{});
+        step(kk, std::integral_constant<int, 0>{}, std::false_type{});
+        if (kk + 1 < KB) step(kk + 1, std::integral_constant<int, 1>{}, std::false_type{});
       }
     }
   };
