@@ -323,7 +323,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       const int row = RPI * gi + lane / LPR;
       const int slot = gi < T::NA ? smSlot[row] : -1;
       const int64_t ar = slot < 0 ? 0 : g.a_by_pos ? pos0 + row : (int64_t)slot_row(g, (uint32_t)slot);
-      a_ptr[i] = g.A + ar * g.lda * EB + row_chunk(gi) * 16;
+      a_ptr[i] = g.A + ar * g.lda * EB + row_chunk(gi) * 16 - SB;
     }
   }
 #pragma unroll
@@ -334,7 +334,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       if constexpr (PHASED) in = (in / (8 * T::CS)) * (16 * T::CS) + (i >> 1) * (8 * T::CS) + in % (8 * T::CS);
       const int64_t c = j0 + in;
       b_ptr[i] = b_base + (c < g.J ? c : 0) * EB;
-      if constexpr (COLUMNS) b_ptr[i] += (int64_t)col_row(gi, BCPR) * g.sbc * EB;
+      if constexpr (COLUMNS) b_ptr[i] += ((int64_t)col_row(gi, BCPR) - STEP) * g.sbc * EB;
     } else {
       const int row = RPI * gi + lane / LPR;
       int64_t j;
@@ -345,7 +345,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
         j = j0 + row;
         j = j < g.J ? j : g.J - 1;
       }
-      b_ptr[i] = b_base + j * g.sbj * EB + row_chunk(gi) * 16;
+      b_ptr[i] = b_base + j * g.sbj * EB + row_chunk(gi) * 16 - SB;
     }
   }
   // kWgrad: the slots of this lane's rows of a step, read ahead of its loads; square
@@ -374,7 +374,9 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
 
   // Load d of this wave's share of step kk into its stage.  Step 0 is the last,
   // partial run of the contraction, so that no other step has to look for its
-  // end; the addresses of the others advance from load to load.
+  // end; the addresses of the others start a step before the contraction and advance
+  // ahead of each load, in their registers (two additions a load if the compiler derives
+  // them from the step's number).
   const int tail = (int)(length - (int64_t)(KB - 1) * STEP);  // elements of step 0
   const int64_t b_step = COLUMNS ? STEP * g.sbc * EB : SB;
   constexpr int ND = T::NA_W + T::NB_W;
@@ -396,22 +398,24 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       if ((is_b ? T::NB : T::NA) % T::NW == 0 || gi < (is_b ? T::NB : T::NA))
         lds_load16(p, dst + (is_b ? b_place(i) : gi * 1024));
     } else if constexpr (is_b) {
-      const uint8_t* p = b_ptr[i];
+      const uint8_t* p;
       if constexpr (first) {
-        p += (KB - 1) * b_step;
         const bool in = COLUMNS ? col_row(gi, BCPR) < left : row_chunk(gi) * 16 < left * EB;
-        p = in ? p : zeros;
+        p = in ? b_ptr[i] + KB * b_step : zeros;
       } else {
         b_ptr[i] += b_step;
+        asm volatile("" : "+v"(b_ptr[i]));
+        p = b_ptr[i];
       }
       if (T::NB % T::NW == 0 || gi < T::NB) lds_load16(p, dst + b_place(i));
     } else {
-      const uint8_t* p = a_ptr[i];
+      const uint8_t* p;
       if constexpr (first) {
-        p += (int64_t)(KB - 1) * SB;
-        p = row_chunk(gi) * 16 < left * EB ? p : zeros;
+        p = row_chunk(gi) * 16 < left * EB ? a_ptr[i] + (int64_t)KB * SB : zeros;
       } else {
         a_ptr[i] += SB;
+        asm volatile("" : "+v"(a_ptr[i]));
+        p = a_ptr[i];
       }
       if (T::NA % T::NW == 0 || gi < T::NA) lds_load16(p, dst + gi * 1024);
     }
@@ -488,18 +492,38 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
     constexpr int RA = decltype(ra_c)::value;
     if (KB == 0) return;
     v4i af[2][RA > 0 ? RA : 1], bf[4];
+    // Phased: a stage's addresses, from which its reads have constant offsets; the
+    // compiler would add up each of them by itself.
+    constexpr int VA = PHASED ? (A_COLS ? T::RS : 2) : 1, VB = PHASED ? (B_COLS ? T::CS / 2 : 2) : 1;
+    uint32_t a_at[VA], b_at[VB];
+    auto place = [&](int stage) {
+      if constexpr (PHASED) {
+        const uint32_t st = lds0 + stage * T::STAGE;
+#pragma unroll
+        for (int v = 0; v < VA; ++v) {
+          a_at[v] = st + (a_lane ^ (v * (A_COLS ? 32 : 16)));
+          asm volatile("" : "+v"(a_at[v]));
+        }
+#pragma unroll
+        for (int v = 0; v < VB; ++v) {
+          b_at[v] = st + (b_lane ^ (v * (B_COLS ? 32 : 16)));
+          asm volatile("" : "+v"(b_at[v]));
+        }
+      }
+    };
     auto read_a = [&](int to, int stage, int h, int r) {
       const uint32_t st = lds0 + stage * T::STAGE;
-      if constexpr (A_COLS) af[to][r] = lds_frag_t(st + (a_lane ^ (r * 32)) + h * 8 * TM * 2, TM * 2);
-      else af[to][r] = lds_frag(st + (a_lane ^ (h * 16)) + r * 16 * SB);
+      if constexpr (A_COLS) af[to][r] = lds_frag_t((PHASED ? a_at[r % VA] : st + (a_lane ^ (r * 32))) + h * 8 * TM * 2, TM * 2);
+      else af[to][r] = lds_frag((PHASED ? a_at[h % VA] : st + (a_lane ^ (h * 16))) + r * 16 * SB);
     };
     auto read_b = [&](int stage, int q) {
       const uint32_t st = lds0 + stage * T::STAGE;
       const int h = half_of(q), c = column_of(q);
-      if constexpr (B_COLS && PHASED) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c % (T::CS / 2) * 32)) + c / (T::CS / 2) * (T::B_BYTES / 2) + h * 8 * BW * 2, BW * 2);
+      if constexpr (B_COLS && PHASED) bf[q & 3] = lds_frag_t(b_at[c % VB] + c / VB * (T::B_BYTES / 2) + h * 8 * BW * 2, BW * 2);
       else if constexpr (B_COLS) bf[q & 3] = lds_frag_t(st + (b_lane ^ (c * 32)) + h * 8 * TN * 2, TN * 2);
-      else bf[q & 3] = lds_frag(st + (b_lane ^ (h * 16)) + c * 16 * SB);
+      else bf[q & 3] = lds_frag((PHASED ? b_at[h % VB] : st + (b_lane ^ (h * 16))) + c * 16 * SB);
     };
+    place(0);
     // stage 0; of the others every wave has at least so many loads behind it
     constexpr int VM2 = T::NB / T::NW / 2, VM1 = T::VM - VM2;  // loads of the two parts
     if constexpr (PHASED) {
@@ -530,11 +554,12 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
               if (STEADY || kk + 2 < KB) mm_wait<VM2 + VM1>();
               else mm_wait<VM2>();
             } else {
-              mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
+              if constexpr (STEADY) mm_wait<(KS - 2) * T::VM>();
+              else mm_wait_stages<KS - 2, T::VM>(KB - 2 - kk);
             }
             mm_barrier();
             if constexpr (WEIGHTS && !PHASED) {
-              if (kk + KS < KB) {
+              if (STEADY || kk + KS < KB) {
                 read_slots(kk + KS);
                 if constexpr (FORM != kWgradDense) issue_ids(kk + KS + kAhead);
               }
@@ -542,6 +567,7 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
           }
           // behind the last step nothing uses these: under the condition, the compiler
           // would wait for them before this slot's instructions
+          place(next);
           if constexpr (RA > 0) {
 #pragma unroll
             for (int r = 0; r < RA; ++r) read_a(T::H == 2 ? 0 : P ^ 1, next, 0, r);
@@ -586,9 +612,9 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
           const std::integral_constant<int, from> f;
           const std::integral_constant<int, to> t;
           if constexpr (Q >= NQ - 2) {
-            if (kk + KS < KB) loads(kk + KS, stage, f, t, std::false_type{});
+            if (STEADY || kk + KS < KB) loads(kk + KS, stage, f, t, std::false_type{});
           } else {
-            if (kk > 0 && kk - 1 + KS < KB) loads(kk - 1 + KS, prev, f, t, std::false_type{});
+            if (STEADY || (kk > 0 && kk - 1 + KS < KB)) loads(kk - 1 + KS, prev, f, t, std::false_type{});
           }
         }
         // the reads stay ahead of the instructions, which the compiler would undo
@@ -605,16 +631,27 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
       }(std::make_integer_sequence<int, NQ>{});
       stage = next;
     };
+    const std::integral_constant<int, 0> p0;
+    const std::integral_constant<int, 1> p1;
+    const std::false_type any;
+    int kk = 0;
     if constexpr (T::H == 2) {
-      int kk = 0;
-      if constexpr (PHASED && RA == T::RS)
-        for (; kk + KS < KB; ++kk) step(kk, std::integral_constant<int, 0>{}, std::true_type{});
-      for (; kk < KB; ++kk) step(kk, std::integral_constant<int, 0>{}, std::false_type{});
-    } else {
-      for (int kk = 0; kk < KB; kk += 2) {
-        step(kk, std::integral_constant<int, 0>{}, std::false_type{});
-        if (kk + 1 < KB) step(kk + 1, std::integral_constant<int, 1>{}, std::false_type{});
+      if constexpr (RA == T::RS) {
+        if constexpr (!PHASED) step(kk++, p0, any);  // which has nothing of the stage before it to load
+        for (; kk + KS < KB; ++kk) step(kk, p0, std::true_type{});
       }
+      for (; kk < KB; ++kk) step(kk, p0, any);
+    } else {
+      auto two = [&](auto steady) {
+        step(kk, p0, steady);
+        if (decltype(steady)::value || kk + 1 < KB) step(kk + 1, p1, steady);
+        kk += 2;
+      };
+      if constexpr (RA == T::RS) {
+        two(any);
+        while (kk + 1 + KS < KB) two(std::true_type{});
+      }
+      while (kk < KB) two(any);
     }
   };
   switch (ra) {
