@@ -468,9 +468,9 @@ int moe_fp8_scaled_mm(const void* a, int64_t lda, const float* a_scale, const vo
  *   y_t = sum_s h_s w2_e^T
  * Sums are fp32; h and the gradient of [Wg Wu]'s outputs are rounded to dtype, y
  * and the gradients once from their fp32 sums (a token's over its slots' fp32
- * rows).  Slots without an expert add nothing.  Any H and I >= 1: widths, strides
- * and addresses that are not of whole 16-byte chunks go through copies in the
- * workspace.
+ * rows).  Slots without an expert add nothing.  1 <= H <= 2^29, 1 <= I <= 2^28;
+ * widths, strides and addresses that are not of whole 16-byte chunks go through
+ * copies in the workspace.
  *
  * With sorted_ids, expert_ids and ntpp NULL the block is dense: E = 1, top_k = 1,
  * every row through the one expert. */
@@ -498,7 +498,8 @@ int64_t moe_ffn_workspace_bytes(const moe_ffn* ffn, int32_t backward);
 /* y [T, H] of dtype. */
 int moe_ffn_forward(const moe_ffn* ffn, void* y, void* stream);
 /* From dy [T, H] the gradients dx [T, H], dw13, dw2 (of dtype) and dtopk_weights
- * [T * top_k] (fp32), each where not NULL.  h and gu are the forward pass's, and
+ * [T * top_k] (fp32), each where not NULL; where H and I are multiples of 8, dw13 and
+ * dw2 are 16-byte aligned.  h and gu are the forward pass's, and
  * expert_ids ascend over the blocks as for moe_grouped_mm_wgrad. */
 int moe_ffn_backward(const moe_ffn* ffn, const void* dy, void* dx, void* dw13, void* dw2, float* dtopk_weights,
                      void* stream);

@@ -13,6 +13,19 @@
 // matrix instructions take 16 bits; G and U are kept in fp32, which costs 8 I bytes
 // more a slot than in 16 bits (3 % of a training step) and leaves the gradient of
 // the router's weights, an fp32 value, as exact as its sums.
+//
+// Launches: the product of both projections with the activation in its epilogue (the
+// tile's columns pair 16 of the gate with 16 of the up projection), the product of h,
+// and with several slots a token the sum of their rows; backward the product of dy with
+// the activation's gradient and dw's parts in its epilogue, the product by rows, and the
+// two gradients by weights.  With the activation in kernels of its own over fp32 rows a
+// prompt of 4093 tokens of 8 on 64 experts took 978 us for 911.
+//
+// What bounds it (us, least of a trace): one token, 7168 x 2048, the weights' stream, 12.5
+// and 7.3 (4.7 and 4.0 TB/s); 4096 tokens of one expert the matrix cores at the board's
+// power, 180, 106, 120, 197, 211, 119 for the six products, 1.01 to 1.34 PF; 128
+// experts of 240 slots, 2048 x 768, the weights, their gradients and the fp32 rows, about
+// 5.4 GB a step at 3.6 TB/s.
 #include "grouped_launch.hpp"
 
 namespace moe {

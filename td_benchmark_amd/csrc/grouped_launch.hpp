@@ -246,10 +246,11 @@ static int dense_rows(int64_t M, int64_t N) {
 // The gradient by weights.
 template <int FORM>
 static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {
-  // Steps of 32 slots in rings of three or four: rows of a column-staged step are
-  // whole lines at any length, so the finer ring costs nothing (256 slots an expert
-  // of 128: 381 us, 403 with steps of 64 in a ring of two; 1024 of 8 even).  The rows
-  // forms lose with it, whose row-staged lines it reads in halves.
+  // Square tiles take steps of 64 slots in a ring of two that is handed over in parts,
+  // 8 experts of 28672 x 4096, 1024 slots 1970 us, with steps of 32 in a ring of four
+  // 2130; those of 128 rows, whose stages have no halves, steps of 32 in a ring of three.
+  // Rows of a column-staged step are whole lines at any length; the rows forms lose with
+  // steps of 32, whose row-staged lines they read in halves.
   //
   // Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
   // sums, where runs are short and most of the time is the gradient's own bytes, or
@@ -257,7 +258,8 @@ static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {
   // They read half as much again, which long runs lose.  Over 1471 calls of 16 shapes
   // (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
   // 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
-  // the others only; limits of 192 to 640 slots are alike within 0.3 %.  By rounds, 128
+  // the others only; limits of 192 to 640 slots are alike within 0.3 % (square tiles
+  // timed with steps of 32, which cost them 8 % in long runs).  By rounds, 128
   // and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
   // 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
   // 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
