@@ -477,7 +477,7 @@ int moe_fp8_scaled_mm(const void* a, int64_t lda, const float* a_scale, const vo
 typedef struct moe_ffn {
   int64_t T, H, I;
   int64_t ldx;                 /* row stride of x, elements */
-  int64_t max_padded;          /* as for the grouped products; dense: 0 */
+  int64_t max_padded;          /* as for the grouped products, a block at least where T > 0; dense: 0 */
   int32_t top_k, E;
   int32_t block_size_m;        /* dense: any */
   int32_t dtype;               /* MOE_BF16 or MOE_FP16 */

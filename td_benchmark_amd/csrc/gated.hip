@@ -118,6 +118,7 @@ static int check_ffn(const moe_ffn& f) {
   } else {
     if (!f.sorted_ids || !f.expert_ids || !f.ntpp) return kErrNullPointer;
     if (!block_m_ok(f.block_size_m)) return kErrBadBlockSize;
+    if (f.T > 0 && f.max_padded < f.block_size_m) return kErrBadShape;  // slots, but no block for them
   }
   return kOk;
 }

@@ -151,6 +151,7 @@ def test_c_ffn_refuses(L):
     base = dict(T=4, H=16, I=12, ldx=16, max_padded=48, top_k=2, E=3, block_size_m=16, dtype=0, x=p, w13=p, w2=p, topk_weights=p,
                 sorted_ids=p, expert_ids=p, ntpp=p, expert_table=p, h=p, gu=p, workspace=p)
     common = ((bad, dict(T=-1)), (bad, dict(H=0)), (bad, dict(I=0)), (bad, dict(ldx=15)), (bad, dict(dtype=2)), (bad, dict(max_padded=-1)),
+              (bad, dict(max_padded=0)), (bad, dict(max_padded=15)),
               (bad, dict(H=(1 << 29) + 1, ldx=(1 << 29) + 1)), (bad, dict(I=(1 << 28) + 1)), (bad, dict(T=1 << 30)),
               (topk, dict(top_k=0)), (experts, dict(E=0)), (block, dict(block_size_m=48)), (null, dict(ntpp=None)),
               (null, dict(sorted_ids=None)), (null, dict(expert_ids=None)),
