@@ -259,14 +259,17 @@ static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {
   // (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
   // 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
   // the others only; limits of 192 to 640 slots are alike within 0.3 % (square tiles
-  // timed with steps of 32, which cost them 8 % in long runs).  By rounds, 128
+  // timed with steps of 32, which cost them 8 % in long runs).  Now whole training steps
+  // by the limit, 128 rows and 256: 16 experts of 4096 x 2048, 256 slots 1042 and 1074
+  // us, 384 alike, 640 1743 and 1721; 60 of 2048 x 1408, 267 slots 1418 and 1437; 128 of
+  // 2048 x 768, 256 slots alike, 384 2054 and 2028, 512 2568 and 2517.  By rounds, 128
   // and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
   // 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
   // 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
   // slots 2039 and 1988.
   const int64_t cols = (g.J + 255) / 256;
   const int64_t half = (g.E * ((g.Cn + 127) / 128) * cols + 511) / 512, square = (g.E * ((g.Cn + 255) / 256) * cols + 255) / 256;
-  if (half < square || half == 1 || g.S <= 224 * (int64_t)g.E) {
+  if (half < square || half == 1 || g.S <= 300 * (int64_t)g.E) {
     using T = MmTile<128, 256, 4, 2, 3, 2, 64>;
     return dtype == MOE_FP16 ? launch_tile<Fp16, true, FORM, T>(g, st) : launch_tile<Bf16, false, FORM, T>(g, st);
   }
