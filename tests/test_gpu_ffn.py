@@ -78,6 +78,17 @@ def test_routing(T, k, E):
     check(T, k, E, 40, 24, BF16, weighted=False)
 
 
+def test_an_expert_chosen_twice():
+    """A token whose slots go to the same expert, and operands that are one tensor."""
+    from td_benchmark_amd import ops
+    x, w13, w2, ids, weight, _ = make(90, 4, 5, 136, 72, BF16)
+    ids[::2, 1] = ids[::2, 0]
+    ids[::3] = 2
+    got = train(x, w13, w2, ops.ExpertSlots(ids, 5), weight, x)
+    for name, a, b in zip(("y", "dx", "dw13", "dw2", "dweights"), got, exact(x, w13, w2, ids, weight, x)):
+        assert over(a, b) <= 0, name
+
+
 def test_weights_streams():
     """Few rows on long rows of weights, in each of the two kernels for them."""
     for T, k, E, H, I in ((1, 1, 0, 2048, 1536), (19, 1, 0, 1536, 1032), (1, 4, 8, 1024, 1160), (5, 4, 64, 1032, 520),
