@@ -34,15 +34,24 @@ static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 static int64_t up_to_256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // ---- the gradient of the router's weights -------------------------------------------
-// dweight[s] = the sum of the slot's n parts: a wave a slot, lanes in order.
+// dweight[s] = the sum of the slot's n parts: a wave a slot at a time, lanes in order.
+// A launch has fewer than 2^32 threads: past kPartSumGrid workgroups (4 million slots)
+// each goes through several slots a wave.
+constexpr int64_t kPartSumGrid = 1 << 20;
+
 __global__ __launch_bounds__(256) void part_sum_kernel(const float* __restrict__ parts, int64_t S, int64_t n, float* __restrict__ dweight) {
-  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (s >= S) return;
-  float sum = 0.0f;
-  for (int64_t i = threadIdx.x & 63; i < n; i += 64) sum += parts[s * n + i];
+  for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < S; s += (int64_t)gridDim.x * 4) {
+    float sum = 0.0f;
+    for (int64_t i = threadIdx.x & 63; i < n; i += 64) sum += parts[s * n + i];
 #pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-  if ((threadIdx.x & 63) == 0) dweight[s] = sum;
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) dweight[s] = sum;
+  }
+}
+static int launch_part_sum(const float* parts, int64_t S, int64_t n, float* dweight, hipStream_t st) {
+  const int64_t groups = (S + 3) / 4;
+  hipLaunchKernelGGL(part_sum_kernel, dim3((unsigned)(groups < kPartSumGrid ? groups : kPartSumGrid)), dim3(256), 0, st, parts, S, n, dweight);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
 // ---- rows that are not whole 16-byte chunks --------------------------------------
@@ -352,10 +361,7 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
       g.ldc = 2 * b.Ip;
       set_top_k(g, f.top_k);
       MOE_TRY(b.rows<kActGrad>(g));
-      if (dweight) {
-        hipLaunchKernelGGL(part_sum_kernel, dim3((unsigned)((b.S + 3) / 4)), dim3(256), 0, b.st, (const float*)ws.parts, b.S, (b.Ip + 31) / 32, dweight);
-        if (hipGetLastError() != hipSuccess) return kErrLaunch;
-      }
+      if (dweight) MOE_TRY(launch_part_sum((const float*)ws.parts, b.S, (b.Ip + 31) / 32, dweight, b.st));
     }
   }
   if (dx && b.S > 0) {
