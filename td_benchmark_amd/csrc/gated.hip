@@ -121,7 +121,8 @@ static int check_ffn(const moe_ffn& f) {
   if (f.dtype != kBf16 && f.dtype != kFp16) return kErrBadShape;
   if (f.top_k < 1) return kErrBadTopK;
   if (f.E < 1) return kErrBadExperts;
-  if (f.T * f.top_k > 0x7FFFFFFE || f.max_padded < 0 || f.max_padded > 0x7FFFFFFF) return kErrBadShape;
+  if (f.T > 0x7FFFFFFE / f.top_k || f.max_padded < 0 || f.max_padded > 0x7FFFFFFF) return kErrBadShape;
+  if (f.E > ((int64_t)1 << 58) / (up8(f.H) * up8(f.I))) return kErrBadShape;  // the weights' bytes, below 2^61
   if (!f.sorted_ids && !f.expert_ids && !f.ntpp) {
     if (f.E != 1 || f.top_k != 1) return kErrBadExperts;
   } else {
@@ -227,12 +228,13 @@ struct Ffn {
   int token_rows(const float* rows32, void* out) const { return slot_sum_rows(rows32, Hp, f.T, f.top_k, f.H, f.dtype, out, st); }
 };
 
-// Parts of a workspace in order.
+// Parts of a workspace in order, each of up to 2^62 bytes; past kMost together they do not fit.
 struct Parts {
+  static constexpr int64_t kMost = (int64_t)1 << 61;
   uint8_t* base;
   int64_t at = 0;
   void* take(int64_t bytes, bool on = true) {
-    if (!on) return nullptr;
+    if (!on || at > kMost) return nullptr;
     uint8_t* p = base ? base + at : nullptr;
     at += up_to_256(bytes);
     return p;
@@ -401,7 +403,7 @@ extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t backward) {
   const Ffn b(*f);
   if (backward) Backward(b, p);
   else Forward(b, p);
-  return p.at;
+  return p.at > Parts::kMost ? kErrBadShape : p.at;
 }
 
 static int check_pointers(const moe_ffn& f, bool backward) {
@@ -410,8 +412,9 @@ static int check_pointers(const moe_ffn& f, bool backward) {
   if (!aligned(f.x, 2) || !aligned(f.w13, 2) || !aligned(f.w2, 2) || !aligned(f.topk_weights, 4) || !aligned(f.h, 16) ||
       !aligned(f.gu, 16) || !aligned(f.workspace, 16))
     return kErrBadShape;
-  if (!f.workspace && moe_ffn_workspace_bytes(&f, backward) > 0) return kErrNullPointer;
-  return kOk;
+  const int64_t work = moe_ffn_workspace_bytes(&f, backward);
+  if (work < 0) return (int)work;
+  return !f.workspace && work > 0 ? kErrNullPointer : kOk;
 }
 
 extern "C" int moe_ffn_forward(const moe_ffn* f, void* y, void* stream) {

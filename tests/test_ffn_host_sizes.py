@@ -1,0 +1,47 @@
+"""CPU: sizes that the C entries of the feed-forward block and of the block-scaled FP8
+product refuse because their bytes do not fit 64 bits, and refusals that come before
+any device work."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+pytest.importorskip("torch")
+
+from td_benchmark_amd import _lib  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("native library not built")
+    return _lib.lib()
+
+
+BY_NAME = {name: code for code, name in _lib.STATUS.items()}
+BAD = BY_NAME["MOE_ERR_BAD_SHAPE"]
+BUF = (ctypes.c_int32 * 256)()  # host memory: only ever passed to a rejected call
+P = (ctypes.addressof(BUF) + 15) // 16 * 16
+BASE = dict(T=4, H=16, I=16, ldx=16, max_padded=48, top_k=2, E=3, block_size_m=16, dtype=0, x=P, w13=P, w2=P, topk_weights=P,
+            sorted_ids=P, expert_ids=P, ntpp=P, expert_table=P, h=P, gu=P, workspace=P)
+
+
+@pytest.mark.parametrize("passes,sizes", [
+    # slots
+    ((0, 1), dict(T=1 << 62, top_k=4)), ((0, 1), dict(T=1 << 61, top_k=1 << 30)), ((0, 1), dict(T=(1 << 63) - 1, top_k=3)),
+    # the weights
+    ((0, 1), dict(H=1 << 29, ldx=1 << 29, I=1 << 28, E=1 << 30)), ((0, 1), dict(H=1 << 29, ldx=1 << 29, I=1 << 28, E=1 << 7)),
+    # all parts of the backward pass together
+    ((1,), dict(T=1 << 30, top_k=1, max_padded=1 << 30, H=1 << 29, ldx=1 << 29, I=1 << 28, E=2, dtype=1, w13=P + 2, w2=P + 2))])
+def test_c_ffn_refuses_sizes_past_64_bits(L, passes, sizes):
+    f = _lib.MoeFfn(**{**BASE, **sizes})
+    for backward in passes:
+        assert L.moe_ffn_workspace_bytes(f, backward) == BAD
+        assert (L.moe_ffn_backward(f, P, P, P, P, P, None) if backward else L.moe_ffn_forward(f, P, None)) == BAD
+
+
+def test_c_ffn_takes_the_longest_widths_it_documents(L):
+    """2^29 and 2^28 columns of one expert, whose weights' copies have 2^60 bytes."""
+    f = _lib.MoeFfn(**{**BASE, "H": 1 << 29, "ldx": 1 << 29, "I": 1 << 28, "E": 1, "w13": P + 2})
+    assert L.moe_ffn_workspace_bytes(f, 0) > 1 << 59
