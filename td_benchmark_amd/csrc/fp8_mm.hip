@@ -450,6 +450,8 @@ static int pad_codes(const uint8_t* src, int64_t rows, int64_t cols, int64_t lds
 // Rows that are not whole 16-byte chunks, or too far apart for a lane's 32-bit offset, are copied.
 static bool take_rows(const void* p, int64_t ld, int64_t K) { return K % 16 == 0 && chunks(p, ld, 1) && ld < (1 << 23); }
 static int64_t padded_bytes(int64_t rows, int64_t K) { return (rows * ((K + 15) / 16 * 16) + 255) / 256 * 256; }
+// M rows and N columns whose padded codes, up to 2^23 bytes a row, have sizes in 64 bits.
+static bool sizes_ok(int64_t M, int64_t N) { return M >= 0 && M <= 0x7FFFFF00 && N >= 0 && N <= (int64_t)1 << 38; }
 
 }  // namespace moe
 
@@ -457,14 +459,14 @@ using namespace moe;
 
 extern "C" int64_t moe_fp8_scaled_mm_workspace_bytes(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M,
                                                      int64_t N, int64_t K) {
-  if (M < 0 || N < 0 || K < 0 || K > (1 << 23) - 16 || lda < K || ldb < K) return kErrBadShape;
+  if (!sizes_ok(M, N) || K < 0 || K > (1 << 23) - 16 || lda < K || ldb < K) return kErrBadShape;
   return (take_rows(a, lda, K) ? 0 : padded_bytes(M, K)) + (take_rows(b, ldb, K) ? 0 : padded_bytes(N, K));
 }
 
 extern "C" int moe_fp8_scaled_mm(const void* a, int64_t lda, const float* a_scale, const void* b, int64_t ldb,
                                  const float* b_scale, const void* bias, int64_t M, int64_t N, int64_t K, int32_t dtype,
                                  void* y, int64_t ldy, void* workspace, void* stream) {
-  if (M < 0 || N < 0 || K < 1 || K > (1 << 23) - 16 || lda < K || ldb < K || ldy < N || M > 0x7FFFFF00) return kErrBadShape;
+  if (!sizes_ok(M, N) || K < 1 || K > (1 << 23) - 16 || lda < K || ldb < K || ldy < N) return kErrBadShape;
   if (dtype != kBf16 && dtype != kFp16) return kErrBadShape;
   if (M == 0 || N == 0) return kOk;
   if (!y || !a || !b || !a_scale || !b_scale) return kErrNullPointer;

@@ -45,3 +45,10 @@ def test_c_ffn_takes_the_longest_widths_it_documents(L):
     """2^29 and 2^28 columns of one expert, whose weights' copies have 2^60 bytes."""
     f = _lib.MoeFfn(**{**BASE, "H": 1 << 29, "ldx": 1 << 29, "I": 1 << 28, "E": 1, "w13": P + 2})
     assert L.moe_ffn_workspace_bytes(f, 0) > 1 << 59
+
+
+def test_c_fp8_refuses_sizes_past_64_bits(L):
+    """Rows and columns whose padded codes have more bytes than 64 bits hold; the size and the call refuse alike."""
+    for M, N, K in ((1 << 62, 24, 160), (1 << 31, 24, 160), (4, 1 << 62, 160), (4, (1 << 63) - 1, 160), (4, 1 << 41, (1 << 23) - 16)):
+        assert L.moe_fp8_scaled_mm_workspace_bytes(P + 1, K + 1, P + 1, K + 1, M, N, K) == BAD
+        assert L.moe_fp8_scaled_mm(P + 1, K + 1, P, P + 1, K + 1, P, None, M, N, K, 0, P, N, P, None) == BAD
