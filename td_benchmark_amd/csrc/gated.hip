@@ -377,16 +377,12 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
     }
   }
   if (dw13) {
-    const bool direct = !b.odd && aligned(dw13, 16);
-    if (!direct && !ws.dw13) return kErrBadShape;
-    MOE_TRY(b.weights(ws.dgu, 2 * b.Ip, x, ldx, 2 * b.Ip, b.Hp, false, direct ? dw13 : ws.dw13));
-    if (!direct) out.add(b.crop_w13(ws.dw13, dw13));
+    MOE_TRY(b.weights(ws.dgu, 2 * b.Ip, x, ldx, 2 * b.Ip, b.Hp, false, b.odd ? ws.dw13 : dw13));
+    if (b.odd) out.add(b.crop_w13(ws.dw13, dw13));
   }
   if (dw2) {
-    const bool direct = !b.odd && aligned(dw2, 16);
-    if (!direct && !ws.dw2) return kErrBadShape;
-    MOE_TRY(b.weights(dy, b.Hp, f.h, b.Ip, b.Hp, b.Ip, true, direct ? dw2 : ws.dw2));
-    if (!direct) out.add(b.crop_w2(ws.dw2, dw2));
+    MOE_TRY(b.weights(dy, b.Hp, f.h, b.Ip, b.Hp, b.Ip, true, b.odd ? ws.dw2 : dw2));
+    if (b.odd) out.add(b.crop_w2(ws.dw2, dw2));
   }
   return launch_copies(out, b.st);
 }
@@ -434,5 +430,7 @@ extern "C" int moe_ffn_backward(const moe_ffn* f, const void* dy, void* dx, void
   MOE_TRY(check_pointers(*f, true));
   if ((f->T > 0 && !dy) || (dtopk_weights && !f->topk_weights)) return kErrNullPointer;
   if (!aligned(dy, 2) || !aligned(dx, 2) || !aligned(dw13, 2) || !aligned(dw2, 2) || !aligned(dtopk_weights, 4)) return kErrBadShape;
-  return ffn_backward(Ffn(*f, stream), dy, dx, dw13, dw2, dtopk_weights);
+  const Ffn b(*f, stream);
+  if (!b.odd && (!aligned(dw13, 16) || !aligned(dw2, 16))) return kErrBadShape;  // written where they are
+  return ffn_backward(b, dy, dx, dw13, dw2, dtopk_weights);
 }

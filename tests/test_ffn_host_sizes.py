@@ -52,3 +52,13 @@ def test_c_fp8_refuses_sizes_past_64_bits(L):
     for M, N, K in ((1 << 62, 24, 160), (1 << 31, 24, 160), (4, 1 << 62, 160), (4, (1 << 63) - 1, 160), (4, 1 << 41, (1 << 23) - 16)):
         assert L.moe_fp8_scaled_mm_workspace_bytes(P + 1, K + 1, P + 1, K + 1, M, N, K) == BAD
         assert L.moe_fp8_scaled_mm(P + 1, K + 1, P, P + 1, K + 1, P, None, M, N, K, 0, P, N, P, None) == BAD
+
+
+@pytest.mark.parametrize("which", ["dw13", "dw2"])
+def test_c_ffn_refuses_unaligned_weights_gradients_first(L, which):
+    """Where the widths are multiples of 8 the weights' gradients are 16-byte aligned: found before any launch (which
+    fails by another code without a GPU), also where the gradients by the tokens and the router's weights are asked for."""
+    f = _lib.MoeFfn(**BASE)
+    dw = dict(dw13=P, dw2=P)
+    dw[which] = P + 2
+    assert L.moe_ffn_backward(f, P, P, dw["dw13"], dw["dw2"], P, None) == BAD
