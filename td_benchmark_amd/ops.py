@@ -1337,6 +1337,19 @@ def _no_tangent(a: torch.Tensor, b: torch.Tensor) -> None:
         raise NotImplementedError("the grouped products have no forward-mode derivative")
 
 
+def _no_derivative(name: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses operands of an operator without derivatives that would lose one: a
+    result without a graph or a tangent would count as one with a derivative of zero."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{name} has no gradient: detach its operands or call it under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous."""
     if t.is_contiguous():
@@ -1653,6 +1666,7 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
         _need(bias, "bias", out_dtype, (N,), anywhere=True)
     if out is not None and tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
+    _no_derivative("fp8_scaled_mm", a, b, a_scale, b_scale, bias, out)
     _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
     if out is None:
         out = a.new_empty((M, N), dtype=out_dtype)
@@ -1739,7 +1753,10 @@ def fp8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
 
     The dot of a block of 128 is the FP8 matrix instruction's, which cuts each group of
     8 products 13 bits below the largest; blocks are scaled and added in fp32 and the
-    sum is rounded once.  A code or scale that is NaN makes its rows or columns NaN."""
+    sum is rounded once.  A code or scale that is NaN makes its rows or columns NaN.
+    Not differentiable: an operand that requires a gradient (a parameter as ``bias``)
+    while gradients are recorded, or has a forward-mode tangent, raises
+    NotImplementedError; serve under torch.no_grad()."""
     if a.dim() != 2 or b.dim() != 2 or a.size(1) != b.size(1):
         raise ValueError(f"a must be [M, K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
     if a.dtype != FP8 or b.dtype != FP8:
@@ -1757,6 +1774,7 @@ def fp8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
         _need(bias, "bias", out_dtype, (N,), anywhere=True)
     if out is not None and tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
+    _no_derivative("fp8_scaled_mm", a, b, a_scale, b_scale, bias, out)
     _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
     if out is None:
         out = a.new_empty((M, N), dtype=out_dtype)
