@@ -241,29 +241,31 @@ struct Parts {
   }
 };
 
+// A pass's workspace.  Last come the copies of y, or of dx and dy, for addresses or widths
+// that are not of whole 16-byte chunks: where there is neither, their room is not needed.
 struct Forward {
   void *x, *w13, *w2, *rows, *y;
-  Forward(const Ffn& b, Parts& p) {
+  Forward(const Ffn& b, Parts& p, bool aligned_y) {
     x = p.take(b.x_bytes(), b.copy_x());
     w13 = p.take(b.w13_bytes(), b.copy_w(b.f.w13));
     w2 = p.take(b.w2_bytes(), b.copy_w(b.f.w2));
     rows = p.take(b.rows_bytes(), b.f.top_k > 1);
-    y = p.take(b.x_bytes(), b.f.top_k == 1);  // for an output that is not of whole chunks
+    y = p.take(b.x_bytes(), b.f.top_k == 1 && (b.Hp != b.f.H || !aligned_y));
   }
 };
 struct Backward {
-  void *x, *dy, *w13, *w2, *parts, *dgu, *rows, *dx, *dw13, *dw2;
-  Backward(const Ffn& b, Parts& p) {
+  void *x, *w13, *w2, *parts, *dgu, *rows, *dw13, *dw2, *dx, *dy;
+  Backward(const Ffn& b, Parts& p, bool aligned_dx, bool aligned_dy) {
     x = p.take(b.x_bytes(), b.copy_x());
-    dy = p.take(b.x_bytes());
     w13 = p.take(b.w13_bytes(), b.copy_w(b.f.w13));
     w2 = p.take(b.w2_bytes(), b.copy_w(b.f.w2));
     parts = p.take(4 * b.S * ((b.Ip + 31) / 32), b.f.topk_weights);
     dgu = p.take(4 * b.S * b.Ip);
     rows = p.take(b.rows_bytes(), b.f.top_k > 1);
-    dx = p.take(b.x_bytes(), b.f.top_k == 1);
     dw13 = p.take(b.w13_bytes(), b.odd);
     dw2 = p.take(b.w2_bytes(), b.odd);
+    dx = p.take(b.x_bytes(), b.f.top_k == 1 && (b.Hp != b.f.H || !aligned_dx));
+    dy = p.take(b.x_bytes(), b.Hp != b.f.H || !aligned_dy);
   }
 };
 
@@ -276,7 +278,8 @@ struct Backward {
 static int ffn_forward(const Ffn& b, void* y) {
   const moe_ffn& f = b.f;
   Parts parts{(uint8_t*)f.workspace};
-  const Forward ws(b, parts);
+  const Forward ws(b, parts, aligned(y, 16));
+  if (!f.workspace && parts.at > 0) return kErrNullPointer;
   const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
   int64_t ldx = f.ldx;
   Copies in;
@@ -312,9 +315,8 @@ static int ffn_forward(const Ffn& b, void* y) {
     MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, true, ws.rows));
     return b.token_rows((const float*)ws.rows, y);
   }
-  const bool direct = b.Hp == f.H && aligned(y, 16);
-  MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, false, direct ? y : ws.y));
-  if (direct) return kOk;
+  MOE_TRY(b.product(f.h, b.Ip, 1, w2, b.Hp, b.Ip, false, false, ws.y ? ws.y : y));
+  if (!ws.y) return kOk;
   Copies out;
   out.add(b.crop_rows(ws.y, y));
   return launch_copies(out, b.st);
@@ -323,12 +325,13 @@ static int ffn_forward(const Ffn& b, void* y) {
 static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void* dw2, float* dweight) {
   const moe_ffn& f = b.f;
   Parts parts{(uint8_t*)f.workspace};
-  const Backward ws(b, parts);
+  const Backward ws(b, parts, aligned(dx, 16), aligned(dy, 16));
+  if (!f.workspace && parts.at > 0) return kErrNullPointer;
   const void *x = f.x, *w13 = f.w13, *w2 = f.w2;
   int64_t ldx = f.ldx;
   const bool rows = dx || dw13 || dweight;  // whether the gradient of the projections is needed
   Copies in, out;
-  if (b.Hp != f.H || !aligned(dy, 16)) {
+  if (ws.dy) {
     in.add(b.pad_rows(dy, f.H, ws.dy));
     dy = ws.dy;
   }
@@ -371,9 +374,8 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
       MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, true, ws.rows));
       MOE_TRY(b.token_rows((const float*)ws.rows, dx));
     } else {
-      const bool direct = b.Hp == f.H && aligned(dx, 16);
-      MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, false, direct ? dx : ws.dx));
-      if (!direct) out.add(b.crop_rows(ws.dx, dx));
+      MOE_TRY(b.product(ws.dgu, 2 * b.Ip, 1, w13, b.Hp, 2 * b.Ip, true, false, ws.dx ? ws.dx : dx));
+      if (ws.dx) out.add(b.crop_rows(ws.dx, dx));
     }
   }
   if (dw13) {
@@ -391,14 +393,15 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
 
 using namespace moe;
 
-extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t backward) {
+extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t pass) {
   if (!f) return kErrNullPointer;
   const int rc = check_ffn(*f);
   if (rc != kOk) return rc;
   Parts p{nullptr};
   const Ffn b(*f);
-  if (backward) Backward(b, p);
-  else Forward(b, p);
+  const bool whole = pass & MOE_FFN_ALIGNED;
+  if (pass & MOE_FFN_BACKWARD) Backward(b, p, whole, whole);
+  else Forward(b, p, whole);
   return p.at > Parts::kMost ? kErrBadShape : p.at;
 }
 
@@ -408,9 +411,8 @@ static int check_pointers(const moe_ffn& f, bool backward) {
   if (!aligned(f.x, 2) || !aligned(f.w13, 2) || !aligned(f.w2, 2) || !aligned(f.topk_weights, 4) || !aligned(f.h, 16) ||
       !aligned(f.gu, 16) || !aligned(f.workspace, 16))
     return kErrBadShape;
-  const int64_t work = moe_ffn_workspace_bytes(&f, backward);
-  if (work < 0) return (int)work;
-  return !f.workspace && work > 0 ? kErrNullPointer : kOk;
+  const int64_t work = moe_ffn_workspace_bytes(&f, backward ? MOE_FFN_BACKWARD : 0);
+  return work < 0 ? (int)work : kOk;
 }
 
 extern "C" int moe_ffn_forward(const moe_ffn* f, void* y, void* stream) {

@@ -1841,8 +1841,11 @@ def _ffn_saved_bytes(f: MoeFfn) -> tuple[int, int]:
     return 8 * n, 2 * n
 
 
-def _ffn_workspace(f: MoeFfn, backward: int) -> int:
-    n = int(lib().moe_ffn_workspace_bytes(f, backward))
+_FFN_BACKWARD, _FFN_ALIGNED = 1, 2  # MOE_FFN_* of include/moe_mi355x.h
+
+
+def _ffn_workspace(f: MoeFfn, which: int) -> int:
+    n = int(lib().moe_ffn_workspace_bytes(f, which))
     if n < 0:
         check(n, "moe_ffn_workspace_bytes")
     return n
@@ -1855,7 +1858,7 @@ def _ffn_forward(f: MoeFfn, x: torch.Tensor, save: bool) -> tuple[torch.Tensor, 
         gu = 0
     y = x.new_empty((f.T, f.H))
     saved = torch.empty(gu + h, dtype=torch.uint8, device=x.device)
-    work = torch.empty(_ffn_workspace(f, 0), dtype=torch.uint8, device=x.device)
+    work = torch.empty(_ffn_workspace(f, _FFN_ALIGNED), dtype=torch.uint8, device=x.device)  # y is new
     f.gu, f.h, f.workspace = saved.data_ptr() if save else None, saved.data_ptr() + gu, work.data_ptr()
     check(lib().moe_ffn_forward(f, y.data_ptr(), _stream_handle()), "moe_ffn_forward")
     return y, saved
@@ -1882,7 +1885,8 @@ class _FfnFunction(torch.autograd.Function):
         dw13 = torch.empty_like(w13) if need[1] else None
         dw2 = torch.empty_like(w2) if need[2] else None
         dweights = torch.empty_like(topk_weights) if need[3] else None
-        work = torch.empty(_ffn_workspace(f, 1), dtype=torch.uint8, device=x.device)
+        aligned = 0 if dy.data_ptr() % 16 else _FFN_ALIGNED  # dx is new
+        work = torch.empty(_ffn_workspace(f, _FFN_BACKWARD | aligned), dtype=torch.uint8, device=x.device)
         f.gu, f.h, f.workspace = saved.data_ptr(), saved.data_ptr() + _ffn_saved_bytes(f)[0], work.data_ptr()
         at = [None if t is None else t.data_ptr() for t in (dx, dw13, dw2, dweights)]
         check(lib().moe_ffn_backward(f, dy.data_ptr(), *at, _stream_handle()), "moe_ffn_backward")
