@@ -490,7 +490,7 @@ typedef struct moe_ffn {
   const int32_t* ntpp;
   const int32_t* expert_table; /* or NULL */
   void* h;                     /* [T * top_k, Ip] dtype, Ip = I up to a multiple of 8; written by the forward pass, read by the backward */
-  float* gu;                   /* [T * top_k, 2 Ip] fp32, likewise */
+  float* gu;                   /* [T * top_k, 2 Ip] fp32, likewise, or NULL where of the gradients at most dw2 is asked for */
   void* workspace;             /* of moe_ffn_workspace_bytes, 16-byte aligned; only within a call */
 } moe_ffn;
 /* The workspace of a pass: 0 the forward one, MOE_FFN_BACKWARD the backward one; with

@@ -405,9 +405,9 @@ extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t pass) {
   return p.at > Parts::kMost ? kErrBadShape : p.at;
 }
 
-static int check_pointers(const moe_ffn& f, bool backward) {
+static int check_pointers(const moe_ffn& f, bool backward, bool need_gu = false) {
   if (f.T == 0 && !backward) return kOk;
-  if ((f.T > 0 && (!f.x || !f.h || (backward && !f.gu))) || !f.w13 || !f.w2) return kErrNullPointer;
+  if ((f.T > 0 && (!f.x || !f.h || (need_gu && !f.gu))) || !f.w13 || !f.w2) return kErrNullPointer;
   if (!aligned(f.x, 2) || !aligned(f.w13, 2) || !aligned(f.w2, 2) || !aligned(f.topk_weights, 4) || !aligned(f.h, 16) ||
       !aligned(f.gu, 16) || !aligned(f.workspace, 16))
     return kErrBadShape;
@@ -429,7 +429,7 @@ extern "C" int moe_ffn_backward(const moe_ffn* f, const void* dy, void* dx, void
                                 void* stream) {
   if (!f) return kErrNullPointer;
   MOE_TRY(check_ffn(*f));
-  MOE_TRY(check_pointers(*f, true));
+  MOE_TRY(check_pointers(*f, true, dx || dw13 || dtopk_weights));
   if ((f->T > 0 && !dy) || (dtopk_weights && !f->topk_weights)) return kErrNullPointer;
   if (!aligned(dy, 2) || !aligned(dx, 2) || !aligned(dw13, 2) || !aligned(dw2, 2) || !aligned(dtopk_weights, 4)) return kErrBadShape;
   const Ffn b(*f, stream);

@@ -1868,7 +1868,9 @@ class _FfnFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor | None,
                 slots: ExpertSlots | None) -> torch.Tensor:
-        y, saved = _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x, True)
+        need = ctx.needs_input_grad
+        ctx.with_gu = need[0] or need[1] or need[3]  # the gradient by w2 alone reads h only
+        y, saved = _ffn_forward(_ffn(x, w13, w2, slots, topk_weights), x, ctx.with_gu)
         ctx.save_for_backward(x, w13, w2, topk_weights, saved)
         ctx.slots = slots
         return y
@@ -1887,7 +1889,8 @@ class _FfnFunction(torch.autograd.Function):
         dweights = torch.empty_like(topk_weights) if need[3] else None
         aligned = 0 if dy.data_ptr() % 16 else _FFN_ALIGNED  # dx is new
         work = torch.empty(_ffn_workspace(f, _FFN_BACKWARD | aligned), dtype=torch.uint8, device=x.device)
-        f.gu, f.h, f.workspace = saved.data_ptr(), saved.data_ptr() + _ffn_saved_bytes(f)[0], work.data_ptr()
+        gu = _ffn_saved_bytes(f)[0] if ctx.with_gu else 0
+        f.gu, f.h, f.workspace = saved.data_ptr() if gu else None, saved.data_ptr() + gu, work.data_ptr()
         at = [None if t is None else t.data_ptr() for t in (dx, dw13, dw2, dweights)]
         check(lib().moe_ffn_backward(f, dy.data_ptr(), *at, _stream_handle()), "moe_ffn_backward")
         return dx, dw13, dw2, dweights, None
@@ -1913,7 +1916,8 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> torch.Ten
     Sums are fp32; the intermediate rows are rounded to 16 bits once, y once from
     its fp32 sum, in the backward pass the gradient of the two projections once and
     each gradient once.  What the backward pass needs is kept from the forward one:
-    the projections in fp32 and the intermediate rows, 10 I bytes a token.  The same
+    the projections in fp32 and the intermediate rows, 10 I bytes a token (the rows
+    alone, 2 I, where only w2 requires a gradient).  The same
     call on equal inputs (alike in sizes and alignment) gives equal bits.  Once
     differentiable; for capture into a HIP graph as grouped_mm: torch.autograd.grad
     rather than ``backward()``.  An operand with a forward-mode tangent raises

@@ -80,3 +80,16 @@ def test_no_room_for_copies_that_no_pass_makes():
         return y, torch.autograd.grad(y, leaves, dy)
     # y and dx; gu, h and the gradient of the projections 14 bytes an element of [T, I]; the weights' gradients
     assert peak(step) <= 2 * row + 14 * T * I + 2 * (w13.numel() + w2.numel()) + slack
+
+
+def test_only_w2_requires_a_gradient():
+    """Without the projections kept: the same gradient, by experts and dense, and in C with gu NULL."""
+    from td_benchmark_amd import ops
+    for E in (0, 3):
+        x, w13, w2, ids, weight, dy = make(70, 2, E, 136, 72, BF16)
+        slots = ops.ExpertSlots(ids, E) if E else None
+        leaf = w2.detach().requires_grad_()
+        y = ops.gated_ffn(x, w13, leaf) if slots is None else ops.experts_ffn(x, w13, leaf, slots, weight)
+        got = torch.autograd.grad(y, leaf, dy)[0]
+        want = exact(x, w13, w2, ids, weight, dy)
+        assert over(y.detach(), want[0]) <= 0 and over(got, want[3]) <= 0
