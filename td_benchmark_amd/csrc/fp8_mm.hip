@@ -400,26 +400,23 @@ static int launch_fp8_few(MmArgs g, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
-// The tile by the rows and columns, by the rules of the other products' (launch_rows).
 template <bool FP16>
 static int launch_fp8_rows(const MmArgs& g, hipStream_t st) {
-  const double blocks = (double)g.n_blocks;
-  const double wide = rounds(blocks, g.J, 256, 1.0), half = rounds(blocks, g.J, 128, 0.65), slim = rounds(blocks, g.J, 64, 0.5);
-  if (g.bm <= 32 && g.Cn >= 2048 && blocks * ((g.J + 63) / 64) <= 128.0)
-    return g.bm == 16 ? launch_fp8_few<FP16, 1>(g, st) : launch_fp8_few<FP16, 2>(g, st);
+  const TileChoice t = fp8_choice(g.S, g.J, g.Cn, g.bm);
+  if (t.few) return g.bm == 16 ? launch_fp8_few<FP16, 1>(g, st) : launch_fp8_few<FP16, 2>(g, st);
   if (g.bm == 16) return launch_fp8<FP16, Fp8Tile<16, 64, 2, 1, 4, 2>>(g, st);
   if (g.bm == 32) return launch_fp8<FP16, Fp8Tile<32, 64, 4, 2, 4, 2>>(g, st);
   if (g.bm == 64) {
-    if (slim < half) return launch_fp8<FP16, Fp8Tile<64, 64, 4, 2, 4, 2>>(g, st);
+    if (t.columns == 64) return launch_fp8<FP16, Fp8Tile<64, 64, 4, 2, 4, 2>>(g, st);
     return launch_fp8<FP16, Fp8Tile<64, 128, 4, 1, 3, 2>>(g, st);
   }
   if (g.bm == 128) {
-    if (slim < half && slim < wide) return launch_fp8<FP16, Fp8Tile<128, 64, 8, 4, 3, 2>>(g, st);
-    if (half < wide) return launch_fp8<FP16, Fp8Tile<128, 128, 8, 4, 4, 1>>(g, st);
+    if (t.columns == 64) return launch_fp8<FP16, Fp8Tile<128, 64, 8, 4, 3, 2>>(g, st);
+    if (t.columns == 128) return launch_fp8<FP16, Fp8Tile<128, 128, 8, 4, 4, 1>>(g, st);
     return launch_fp8<FP16, Fp8Tile<128, 256, 8, 2, 3, 1>>(g, st);
   }
-  if (slim < half && slim < wide) return launch_fp8<FP16, Fp8Tile<256, 64, 8, 4, 3, 1>>(g, st);
-  if (half < wide) return launch_fp8<FP16, Fp8Tile<256, 128, 8, 4, 3, 1>>(g, st);
+  if (t.columns == 64) return launch_fp8<FP16, Fp8Tile<256, 64, 8, 4, 3, 1>>(g, st);
+  if (t.columns == 128) return launch_fp8<FP16, Fp8Tile<256, 128, 8, 4, 3, 1>>(g, st);
   return launch_fp8<FP16, Fp8Tile<256, 256, 8, 4, 2, 1>>(g, st);
 }
 

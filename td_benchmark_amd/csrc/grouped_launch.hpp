@@ -10,6 +10,13 @@ namespace moe {
 static bool fits_launch(int64_t workgroups, int threads) { return workgroups <= 0xFFFFFFFFll / threads; }
 
 // ---- whole, aligned chunks ---------------------------------------------------
+// Whether tiles of 256 rows are dealt by the experts' counts, and among how many
+// workgroups an expert's short last tile is shared (launch_tile).
+static bool by_counts(int64_t S, int64_t E, int64_t n_jt) { return S >= 768 * E && S / 256 * n_jt <= 1024; }
+static int short_parts(int64_t S, int64_t E, int64_t n_jt, int64_t row_bytes) {
+  return (S < E ? S : E) * n_jt <= 256 && row_bytes >= 64 * 128 ? 4 : 1;
+}
+
 template <class OP, bool FP16, int FORM, class T>
 static int launch_tile(MmArgs g, hipStream_t st) {
   constexpr int kColumns = out_columns(FORM, T::TN);
@@ -194,41 +201,53 @@ static double live_blocks_guess(const MmArgs& g) {
   return b < (double)g.n_blocks ? b : (double)g.n_blocks;
 }
 
-template <class OP, bool FP16, int FORM>
-static int launch_rows(const MmArgs& g, hipStream_t st) {
-  const double blocks = live_blocks_guess(g);
-  const int64_t J = FORM == kGated ? 2 * g.J : g.J;  // columns of B
+// Rows and columns of a tile; few: few_mm_kernel's split of the contraction.
+struct TileChoice {
+  int rows, columns;
+  bool few;
+};
+// The tile of the rows form: `blocks` blocks of bm rows that hold S slots, J columns of
+// B, whose rows (those along the contraction) have row_bytes.
+static TileChoice rows_choice(bool columns, double blocks, int64_t S, int bm, int64_t J, int64_t row_bytes) {
   const double wide = rounds(blocks, J, 256, 1.0), half = rounds(blocks, J, 128, 0.65), slim = rounds(blocks, J, 64, 0.5);
   // Few rows on long rows of weights: few tiles, or one or two slots a block (more
   // rows make it draw as much of A as of the weights).  int8, one row, 7168 x 4096:
   // 16.3 us, staged 24.5; 16 tokens on 128 experts 126 and 148; 9 slots a block of
   // 14336 272 and 226; rows of 768 bytes 123 and 79.
+  if (!columns && bm <= 32 && row_bytes >= 2048 && (blocks * ((J + 63) / 64) <= 128.0 || S <= 2.0 * blocks)) return {bm, 16, true};
+  if (bm <= 32) return {bm, !columns || wide <= 1.0 ? 64 : 256, false};
+  if (bm == 64) return {64, columns && half >= wide ? 256 : slim < half ? 64 : 128, false};
+  if (slim < half && slim < wide) return {bm, 64, false};
+  return {bm, half < wide ? 128 : 256, false};
+}
+
+template <class OP, bool FP16, int FORM>
+static int launch_rows(const MmArgs& g, hipStream_t st) {
+  const int64_t J = FORM == kGated ? 2 * g.J : g.J;  // columns of B
+  const TileChoice t = rows_choice(by_columns(FORM), live_blocks_guess(g), g.S, g.bm, J, g.Cn * OP::BYTES);
   if constexpr (!by_columns(FORM)) {
-    if (g.bm <= 32 && g.Cn * OP::BYTES >= 2048 && (blocks * ((J + 63) / 64) <= 128.0 || g.S <= 2.0 * blocks))
-      return g.bm == 16 ? launch_few<OP, FP16, 1, FORM>(g, st) : launch_few<OP, FP16, 2, FORM>(g, st);
+    if (t.few) return g.bm == 16 ? launch_few<OP, FP16, 1, FORM>(g, st) : launch_few<OP, FP16, 2, FORM>(g, st);
   }
-  if (g.bm <= 32) {
-    const bool stream = !by_columns(FORM) || wide <= 1.0;
-    if (g.bm == 16)
-      return stream ? launch_tile<OP, FP16, FORM, MmTile<16, 64, 2, 1, 4, 2>>(g, st)
-                    : launch_tile<OP, FP16, FORM, MmTile<16, 256, 8, 1, 3, 1>>(g, st);
-    return stream ? launch_tile<OP, FP16, FORM, MmTile<32, 64, 4, 2, 6, 2>>(g, st)
-                  : launch_tile<OP, FP16, FORM, MmTile<32, 256, 8, 1, 3, 1>>(g, st);
+  if (g.bm == 16) {
+    if (t.columns == 64) return launch_tile<OP, FP16, FORM, MmTile<16, 64, 2, 1, 4, 2>>(g, st);
+    return launch_tile<OP, FP16, FORM, MmTile<16, 256, 8, 1, 3, 1>>(g, st);
+  }
+  if (g.bm == 32) {
+    if (t.columns == 64) return launch_tile<OP, FP16, FORM, MmTile<32, 64, 4, 2, 6, 2>>(g, st);
+    return launch_tile<OP, FP16, FORM, MmTile<32, 256, 8, 1, 3, 1>>(g, st);
   }
   if (g.bm == 64) {
-    if (!by_columns(FORM) || half < wide) {
-      if (slim < half) return launch_tile<OP, FP16, FORM, MmTile<64, 64, 4, 2, 4, 2>>(g, st);
-      return launch_tile<OP, FP16, FORM, MmTile<64, 128, 4, 1, 3, 2>>(g, st);
-    }
+    if (t.columns == 64) return launch_tile<OP, FP16, FORM, MmTile<64, 64, 4, 2, 4, 2>>(g, st);
+    if (t.columns == 128) return launch_tile<OP, FP16, FORM, MmTile<64, 128, 4, 1, 3, 2>>(g, st);
     return launch_tile<OP, FP16, FORM, MmTile<64, 256, 8, 2, 3, 1>>(g, st);
   }
   if (g.bm == 128) {
-    if (slim < half && slim < wide) return launch_tile<OP, FP16, FORM, MmTile<128, 64, 8, 4, 3, 2>>(g, st);
-    if (half < wide) return launch_tile<OP, FP16, FORM, MmTile<128, 128, 8, 4, 4, 1>>(g, st);
+    if (t.columns == 64) return launch_tile<OP, FP16, FORM, MmTile<128, 64, 8, 4, 3, 2>>(g, st);
+    if (t.columns == 128) return launch_tile<OP, FP16, FORM, MmTile<128, 128, 8, 4, 4, 1>>(g, st);
     return launch_tile<OP, FP16, FORM, MmTile<128, 256, 8, 2, 3, 1>>(g, st);
   }
-  if (slim < half && slim < wide) return launch_tile<OP, FP16, FORM, MmTile<256, 64, 8, 4, 3, 1>>(g, st);
-  if (half < wide) return launch_tile<OP, FP16, FORM, MmTile<256, 128, 8, 4, 3, 1>>(g, st);
+  if (t.columns == 64) return launch_tile<OP, FP16, FORM, MmTile<256, 64, 8, 4, 3, 1>>(g, st);
+  if (t.columns == 128) return launch_tile<OP, FP16, FORM, MmTile<256, 128, 8, 4, 3, 1>>(g, st);
   return launch_tile<OP, FP16, FORM, MmTile<256, 256, 8, 4, 2, 1>>(g, st);
 }
 
@@ -243,33 +262,49 @@ static int dense_rows(int64_t M, int64_t N) {
   return bm;
 }
 
-// The gradient by weights.
+// The dense FP8 product's tile for M x N outputs from rows of K codes, by the rules above.
+static TileChoice fp8_choice(int64_t M, int64_t N, int64_t K, int bm) {
+  const double blocks = (double)((M + bm - 1) / bm);
+  const double wide = rounds(blocks, N, 256, 1.0), half = rounds(blocks, N, 128, 0.65), slim = rounds(blocks, N, 64, 0.5);
+  if (bm <= 32 && K >= 2048 && blocks * ((N + 63) / 64) <= 128.0) return {bm, 16, true};
+  if (bm <= 32) return {bm, 64, false};
+  if (bm == 64) return {64, slim < half ? 64 : 128, false};
+  if (slim < half && slim < wide) return {bm, 64, false};
+  return {bm, half < wide ? 128 : 256, false};
+}
+
+// The gradient by weights.  Whether its tiles are square:
+//
+// Square tiles take steps of 64 slots in a ring of two that is handed over in parts,
+// 8 experts of 28672 x 4096, 1024 slots 1970 us, with steps of 32 in a ring of four
+// 2130; those of 128 rows, whose stages have no halves, steps of 32 in a ring of three.
+// Rows of a column-staged step are whole lines at any length; the rows forms lose with
+// steps of 32, whose row-staged lines they read in halves.
+//
+// Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
+// sums, where runs are short and most of the time is the gradient's own bytes, or
+// where square tiles would take more rounds (never fewer) or leave CUs idle in one.
+// They read half as much again, which long runs lose.  Over 1471 calls of 16 shapes
+// (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
+// 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
+// the others only; limits of 192 to 640 slots are alike within 0.3 % (square tiles
+// timed with steps of 32, which cost them 8 % in long runs).  Now whole training steps
+// by the limit, 128 rows and 256: 16 experts of 4096 x 2048, 256 slots 1042 and 1074
+// us, 384 alike, 640 1743 and 1721; 60 of 2048 x 1408, 267 slots 1418 and 1437; 128 of
+// 2048 x 768, 256 slots alike, 384 2054 and 2028, 512 2568 and 2517.  By rounds, 128
+// and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
+// 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
+// 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
+// slots 2039 and 1988.
+static bool square_choice(int64_t E, int64_t Cn, int64_t J, int64_t S) {
+  const int64_t cols = (J + 255) / 256;
+  const int64_t half = (E * ((Cn + 127) / 128) * cols + 511) / 512, square = (E * ((Cn + 255) / 256) * cols + 255) / 256;
+  return !(half < square || half == 1 || S <= 300 * E);
+}
+
 template <int FORM>
 static int launch_weights(const MmArgs& g, int32_t dtype, hipStream_t st) {
-  // Square tiles take steps of 64 slots in a ring of two that is handed over in parts,
-  // 8 experts of 28672 x 4096, 1024 slots 1970 us, with steps of 32 in a ring of four
-  // 2130; those of 128 rows, whose stages have no halves, steps of 32 in a ring of three.
-  // Rows of a column-staged step are whole lines at any length; the rows forms lose with
-  // steps of 32, whose row-staged lines they read in halves.
-  //
-  // Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
-  // sums, where runs are short and most of the time is the gradient's own bytes, or
-  // where square tiles would take more rounds (never fewer) or leave CUs idle in one.
-  // They read half as much again, which long runs lose.  Over 1471 calls of 16 shapes
-  // (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
-  // 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
-  // the others only; limits of 192 to 640 slots are alike within 0.3 % (square tiles
-  // timed with steps of 32, which cost them 8 % in long runs).  Now whole training steps
-  // by the limit, 128 rows and 256: 16 experts of 4096 x 2048, 256 slots 1042 and 1074
-  // us, 384 alike, 640 1743 and 1721; 60 of 2048 x 1408, 267 slots 1418 and 1437; 128 of
-  // 2048 x 768, 256 slots alike, 384 2054 and 2028, 512 2568 and 2517.  By rounds, 128
-  // and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
-  // 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
-  // 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
-  // slots 2039 and 1988.
-  const int64_t cols = (g.J + 255) / 256;
-  const int64_t half = (g.E * ((g.Cn + 127) / 128) * cols + 511) / 512, square = (g.E * ((g.Cn + 255) / 256) * cols + 255) / 256;
-  if (half < square || half == 1 || g.S <= 300 * (int64_t)g.E) {
+  if (!square_choice(g.E, g.Cn, g.J, g.S)) {
     using T = MmTile<128, 256, 4, 2, 3, 2, 64>;
     return dtype == MOE_FP16 ? launch_tile<Fp16, true, FORM, T>(g, st) : launch_tile<Bf16, false, FORM, T>(g, st);
   }

@@ -55,6 +55,18 @@ int moe_probe_mfma_rate(int64_t waves, int32_t iters, int32_t form, float* sink,
  * of 8, 8-byte aligned) -> n bf16 bit patterns. */
 int moe_probe_fp8_to_bf16(const void* codes, int64_t n, void* out, void* stream);
 
+/* Host only: the tiles that the library's launches choose.
+ * The rows form `form` (enum Form of grouped_tile.hpp) of S slots on E experts (or dense rows), J output
+ * columns, K columns of the contraction in 16 bits -> out: rows and columns of B of a tile; 1 where the
+ * contraction is split over the waves; 0, or where an expert list's tiles are dealt by its counts, among how
+ * many workgroups a short last tile is shared (-1: no short tiles). */
+void moe_probe_rows_choice(int32_t form, int32_t dense, int64_t S, int32_t E, int32_t block_m, int64_t max_padded,
+                           int64_t J, int64_t K, int32_t* out);
+/* Whether the gradient by weights [E, N, J] over S slots takes square tiles. */
+int32_t moe_probe_square_choice(int32_t E, int64_t N, int64_t J, int64_t S);
+/* The dense FP8 product: rows, columns and split as above. */
+void moe_probe_fp8_choice(int64_t M, int64_t N, int64_t K, int32_t* out);
+
 #ifdef __cplusplus
 }
 #endif
