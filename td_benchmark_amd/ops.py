@@ -1745,8 +1745,9 @@ def fp8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """y = dequantised a @ dequantised b^T + bias, [M, N] in ``out_dtype`` (bf16 or
     fp16): a [M, K] and b [N, K] e4m3fn with a scale for each row and 128 columns of a
-    ([M, ceil(K/128)] fp32, as per_token_group_quant_fp8 gives them) and for each 128 x
-    128 block of b ([ceil(N/128), ceil(K/128)], as quantize_block128).  Any M and N, 1
+    ([M, ceil(K/128)] fp32, as per_token_group_quant_fp8 gives them, which takes bf16:
+    fp16 activations are cast before) and for each 128 x 128 block of b
+    ([ceil(N/128), ceil(K/128)], as quantize_block128).  Any M and N, 1
     <= K < 2^23 - 15; a last block may be partial.  Rows of a, b and ``out`` may be strided (rows of a
     and b that are not whole 16-byte chunks at 16-byte aligned addresses are copied in
     the call); bias [N] in out_dtype.
@@ -1935,5 +1936,7 @@ def experts_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, slots: Exp
     [T, top_k] fp32 (None: ones).  Slots without an expert add nothing, and their
     weights' gradients are zero.  The router's weight multiplies the intermediate
     row before its rounding; a token's sum is over fp32 rows of its slots, in
-    ascending slots.  Otherwise as gated_ffn, with 10 I bytes kept a slot."""
+    ascending slots.  In fp16 a weighted row below 6e-5 keeps steps of 2^-24, as a
+    result of that size itself does.  Otherwise as gated_ffn, with 10 I bytes kept a
+    slot."""
     return _run_ffn(x, w13, w2, topk_weights, slots)
