@@ -54,7 +54,7 @@ def test_the_split_of_the_contraction(tile, K):
     check(tile, M, N - K % 3, K, BF16 if K % 256 else FP16, bool(K % 128))
 
 
-@pytest.mark.parametrize("tile,M,N,K", [("256x256", 2000, 7168, 7168), ("64x64", 45, 14344, 4096), ("16x64", 1, 36864, 7168),
+@pytest.mark.parametrize("tile,M,N,K", [("256x256", 2000, 7168, 7168), ("64x64", 45, 14344, 4096), ("16 split", 1, 36864, 7168), ("16 split", 2, 14344, 4096), ("16x64", 3, 14344, 4096),
                                         ("128x128", 121, 16400, 4096)])
 def test_long_contractions(tile, M, N, K):
     """32 and 56 blocks, as layers have them."""

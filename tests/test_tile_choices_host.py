@@ -50,3 +50,12 @@ def test_the_tiles_of_large_calls_have_large_cases():
     have = set().union(*(tiles_of(*c) for c in long))
     assert {"gated 256x256", "actgrad 256x128", "actgrad 256x256", "product 256x256", "rows32 256x256", "dgrad 256x256",
             "dgrad32 256x256", "wgrad_dense 256x256"} <= have, have
+
+
+def test_one_or_two_rows_split_the_contraction_at_any_width():
+    """As the other products: staged tiles of 16 rows took 5 to 15 % longer."""
+    for M in (1, 2):
+        for N, K in ((4096, 7168), (14344, 4096), (36864, 7168), (1 << 18, 2048)):
+            assert fp8_tile(M, N, K) == "16 split"
+        assert fp8_tile(M, 36864, 2000) == "16x64"
+    assert fp8_tile(3, 14344, 4096) == "16x64"
