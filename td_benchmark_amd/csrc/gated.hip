@@ -298,6 +298,7 @@ static int ffn_forward(const Ffn& b, void* y) {
   }
   MOE_TRY(launch_copies(in, b.st));
   MmArgs g = b.args(b.Ip);
+  g.J_used = f.I;
   g.A = (const uint8_t*)x;
   g.B = (const uint8_t*)w13;
   g.C = (uint8_t*)f.h;
@@ -352,6 +353,7 @@ static int ffn_backward(const Ffn& b, const void* dy, void* dx, void* dw13, void
   if (rows) {
     if (b.S > 0) {
       MmArgs g = b.args(b.Ip);
+      g.J_used = f.I;
       g.A = (const uint8_t*)dy;
       g.B = (const uint8_t*)w2;
       g.C = (uint8_t*)ws.dgu;

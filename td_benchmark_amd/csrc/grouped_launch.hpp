@@ -139,8 +139,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_mm_kernel(MmArgs g) {
 #pragma unroll
       for (int w = 1; w < kFewWaves; ++w) up = up + part[w][r][l + 32];
       const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
-      const v2u pk = {pack2<FP16>(gated(sum[0], up[0], w), gated(sum[1], up[1], w)),
-                      pack2<FP16>(gated(sum[2], up[2], w), gated(sum[3], up[3], w))};
+      float h[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) h[v] = jj + v < g.J_used ? gated(sum[v], up[v], w) : 0.0f;
+      const v2u pk = {pack2<FP16>(h[0], h[1]), pack2<FP16>(h[2], h[3])};
       *reinterpret_cast<v2u*>(g.C + ((int64_t)slot * g.ldc + jj) * 2) = pk;
       return;
     }

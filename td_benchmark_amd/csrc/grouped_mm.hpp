@@ -112,6 +112,8 @@ struct MmArgs {
   int64_t shorts;       // rows form with a table: workgroups from this one on take the experts' short last tiles,
   int short_parts;      // so many of them each
   float* gu;            // feed-forward block: gate and up products of each slot, [S, 2 J], or null
+  int64_t J_used;       // feed-forward block: the columns behind these pad its width and count for nothing, also
+                        // where an infinity in a row makes NaN of them
   float* parts;         // kActGrad: parts of the gradient of topk_w, [S, (J + 31) / 32], or null
   int out32;            // kDgrad: rows of fp32, which are summed over a token's slots before they are rounded
   int bm, top_k, a_by_pos, E;

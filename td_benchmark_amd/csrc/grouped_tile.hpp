@@ -250,6 +250,9 @@ MOE_DEVICE bool table_tile(const MmArgs& g, int64_t& pos0, int64_t& j, int& e, i
   return true;
 }
 
+// The 16-bit halves of a pair of outputs at columns j and j + 1 that count.
+MOE_DEVICE int used_pair(const MmArgs& g, int64_t j) { return j + 1 < g.J_used ? -1 : j < g.J_used ? 0xFFFF : 0; }
+
 // One tile: rows [i0, i0 + nvalid) of the output, or the slots of the table's first
 // nvalid rows, by columns j0 on (col0 on of the columns' table), over `length` of the
 // contraction.  K: the tile of the launch, which T is or is a part of.
@@ -740,6 +743,10 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
             out[v] = (int)pack2<FP16>(gated(gl[2 * v], ul[2 * v], w), gated(gl[2 * v + 1], ul[2 * v + 1], w));
             out[2 + v] = (int)pack2<FP16>(gated(gh[2 * v], uh[2 * v], w), gated(gh[2 * v + 1], uh[2 * v + 1], w));
           }
+          if (jj + 8 > g.J_used) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) out[v] &= used_pair(g, jj + 2 * v);
+          }
           *reinterpret_cast<v4i*>(g.C + ((int64_t)slot * g.ldc + jj) * 2) = out;
         }
       } else {
@@ -765,7 +772,15 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
           const int64_t jj = j0 + col_base + 8 * u;
           float sum = 0.0f;
           if (slot >= 0) {
-            const v4f dl = chunk(row, 2 * u), dh = chunk(row, 2 * u + 1);
+            v4f dl = chunk(row, 2 * u), dh = chunk(row, 2 * u + 1);
+            if (jj + 8 > g.J_used) {
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                if (jj + n < g.J_used) continue;
+                (n < 4 ? dl : dh)[n & 3] = 0.0f;
+                gu[i][n < 4 ? 0 : 1][n & 3] = gu[i][n < 4 ? 2 : 3][n & 3] = 0.0f;
+              }
+            }
             const float w = g.topk_w ? g.topk_w[slot] : 1.0f;
             v4i dg, du;
 #pragma unroll
@@ -778,6 +793,13 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
               }
               dg[v] = (int)pack2<FP16>(a[0], a[1]);
               du[v] = (int)pack2<FP16>(b[0], b[1]);
+            }
+            if (jj + 8 > g.J_used) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                dg[v] &= used_pair(g, jj + 2 * v);
+                du[v] &= used_pair(g, jj + 2 * v);
+              }
             }
             uint8_t* to = g.C + ((int64_t)slot * g.ldc + jj) * 2;
             *reinterpret_cast<v4i*>(to) = dg;
