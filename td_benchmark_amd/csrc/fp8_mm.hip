@@ -5,10 +5,11 @@
 // cuts each group of 8 products 13 bits below its largest one's exponent); the
 // blocks are added in fp32 and the sum is rounded once.
 //
-// What bounds it (us, least of a trace): 1 row, 7168 to 4096, the weights' stream, 7.6
-// (3.9 TB/s); 45 rows, 4096 to 14344, 16.2 (3.6 TB/s); 8192 rows, 7168 to 4096, the matrix
-// cores and four FMAs for each of their instructions, 226 (2.13 PF), at the median 251 by
-// the clock that the board's power leaves.
+// What bounds it (us, least and median of a trace): 1 row, 7168 to 4096, the weights'
+// stream, 7.7 and 7.8 (3.8 TB/s); 45 rows, 4096 to 14344, 16.3 and 16.8, on another box 17.5
+// and 17.9 (3.3 to 3.6 TB/s); 8192 rows, 7168 to 4096, the matrix cores and four FMAs for
+// each of their instructions, 226 (2.13 PF) and 245 to 260 by the clock that the board's
+// power leaves (back to back 1399 W of 1400 at 1.91 GHz).
 #include "grouped_launch.hpp"
 
 namespace moe {

@@ -21,11 +21,12 @@
 // two gradients by weights.  With the activation in kernels of its own over fp32 rows a
 // prompt of 4093 tokens of 8 on 64 experts took 978 us for 911.
 //
-// What bounds it (us, least of a trace): one token, 7168 x 2048, the weights' stream, 12.5
-// and 7.3 (4.7 and 4.0 TB/s); 4096 tokens of one expert the matrix cores at the board's
-// power, 180, 106, 120, 197, 211, 119 for the six products, 1.01 to 1.34 PF; 128
-// experts of 240 slots, 2048 x 768, the weights, their gradients and the fp32 rows, about
-// 5.4 GB a step at 3.6 TB/s.
+// What bounds it (us, least and median of a trace): one token, 7168 x 2048, the weights'
+// stream, 12.4, 12.9 and 6.9, 7.2 (4.7 and 4.3 TB/s); 4096 tokens of one expert the matrix
+// cores at the board's power (1381 W of 1400), 182, 107, 121, 198, 208, 119 for the six
+// products, at the median 200, 118, 132, 225, 228, 128, 0.91 to 1.32 PF; 128 experts of 240
+// slots, 2048 x 768, the weights, their gradients and the fp32 rows, by the counters 4.6 GB
+// read and 2.1 written a step, 4.2 TB/s of the kernels' time.
 #include "grouped_launch.hpp"
 
 namespace moe {

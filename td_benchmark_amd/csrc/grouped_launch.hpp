@@ -293,18 +293,18 @@ static TileChoice fp8_choice(int64_t M, int64_t N, int64_t K, int bm) {
 // Two workgroups a CU with tiles of 128 rows: one writes its tile while the other
 // sums, where runs are short and most of the time is the gradient's own bytes, or
 // where square tiles would take more rounds (never fewer) or leave CUs idle in one.
-// They read half as much again, which long runs lose.  Over 1471 calls of 16 shapes
-// (384 to 28672 columns, 4 to 128 experts of 1 to 1024 slots on average) the time is
-// 1.2 % over the better tile's by this rule, 3.8 % with square tiles only, 1.3 % with
-// the others only; limits of 192 to 640 slots are alike within 0.3 % (square tiles
-// timed with steps of 32, which cost them 8 % in long runs).  Now whole training steps
-// by the limit, 128 rows and 256: 16 experts of 4096 x 2048, 256 slots 1042 and 1074
-// us, 384 alike, 640 1743 and 1721; 60 of 2048 x 1408, 267 slots 1418 and 1437; 128 of
-// 2048 x 768, 256 slots alike, 384 2054 and 2028, 512 2568 and 2517.  By rounds, 128
-// and 256 rows, us: one, 8 experts of 1024 x 1024, 700 slots 27 and 30; 2 and 3, 20 of
-// 384 x 3584, 600 slots 55 and 70; alike, 64 of 2048 x 4096, 24 slots 228 and 264; 24 of
-// 4096 x 2048, 100 slots 143 and 130, 300 slots 206 and 198; 8 of 28672 x 4096, 1024
-// slots 2039 and 1988.
+// They read half as much again, which long runs lose.  Over 243 calls of 16 shapes
+// (384 to 28672 columns, 1 to 256 experts of 1 to 4096 slots on average, each call on the
+// buffers of the one before) the time is 1.6 % over the better tile's by this rule, 2.9 %
+// by the limit without the rounds, 13.5 % with square tiles only, 1.5 % with the others
+// only; limits of 384 to 640 slots make it 0.7 to 0.8 %.  Whole training steps on buffers
+// in turn hold them back, 128 rows and 256, us: 16 experts of 4096 x 2048, 256 slots 1042
+// and 1074, 384 alike, 640 1743 and 1721; 60 of 2048 x 1408, 267 slots 1418 and 1437; 128
+// of 2048 x 768, 256 slots alike, 384 2054 and 2028, 512 2568 and 2517.  By rounds, 128 and
+// 256 rows, us: one, 4 experts of 1024 x 1024, 640 slots 18 and 22; 2 and 3, 20 of 384 x
+// 3584, 640 slots 47 and 62; by the limit, 24 of 4096 x 2048, 128 slots 107 and 125, 320
+// 159 and 182, 1024 427 and 393; 8 of 28672 x 4096, 320 slots 731 and 794, 1024 1910 and
+// 1795.
 static bool square_choice(int64_t E, int64_t Cn, int64_t J, int64_t S) {
   const int64_t cols = (J + 255) / 256;
   const int64_t half = (E * ((Cn + 127) / 128) * cols + 511) / 512, square = (E * ((Cn + 255) / 256) * cols + 255) / 256;

@@ -487,10 +487,11 @@ MOE_DEVICE void mm_tile(const MmArgs& g, uint8_t* smem, int64_t pos0, int64_t i0
   // that every load has one and a half steps to arrive and a stage's worth of younger
   // ones stays in flight at each wait.
   //
-  // What bounds it: a step's instructions take 2048 cycles of a SIMD, the step about 2900
-  // (4096 x 7168 to 4096 in 180 us, 1.34 PF), with barriers of 100-200 and none in waits
-  // for loads; LDS gives 250 bytes a cycle, of which the fragments take 66.  Fewer cycles
-  // lower the clock: 3300 a step ran at 1.96 GHz, 2900 at 1.81, at the board's power.
+  // What bounds it: a step's instructions take 2048 cycles of a SIMD, the step 2940
+  // (4096 x 7168 to 4096 in 182 us at the least, 1.32 PF, 200 at the median), with
+  // barriers of 100-200 and none in waits for loads; LDS gives 250 bytes a cycle, of
+  // which the fragments take 66.  Fewer cycles lower the clock: 3300 a step ran at 1.96
+  // GHz, 2940 at 1.82, at the board's power.
   // Four waves of 128 x 128, which read a third less from LDS, took 225 us for 196: one
   // wave a SIMD has nothing to run while it waits.
   constexpr int NQ = T::H * T::CS, MID = NQ / 2 - 2;
