@@ -493,10 +493,10 @@ typedef struct moe_ffn {
   float* gu;                   /* [T * top_k, 2 Ip] fp32, likewise, or NULL where of the gradients at most dw2 is asked for */
   void* workspace;             /* of moe_ffn_workspace_bytes, 16-byte aligned; only within a call */
 } moe_ffn;
-/* The workspace of a pass: 0 the forward one, MOE_FFN_BACKWARD the backward one; with
- * MOE_FFN_ALIGNED as well for calls whose y, or dy and dx, are at 16-byte aligned addresses, which
+/* The workspace of a pass: 0 the forward one, MOE_FFN_BACKWARD (or any other value) the backward
+ * one; either | MOE_FFN_ALIGNED for calls whose y, or dy and dx, are at 16-byte aligned addresses, which
  * where H is a multiple of 8 need no room for their copies.  Negative: a status code. */
-enum { MOE_FFN_BACKWARD = 1, MOE_FFN_ALIGNED = 2 };
+enum { MOE_FFN_BACKWARD = 1, MOE_FFN_ALIGNED = 256 };
 int64_t moe_ffn_workspace_bytes(const moe_ffn* ffn, int32_t pass);
 /* y [T, H] of dtype. */
 int moe_ffn_forward(const moe_ffn* ffn, void* y, void* stream);

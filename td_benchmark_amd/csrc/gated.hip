@@ -402,8 +402,8 @@ extern "C" int64_t moe_ffn_workspace_bytes(const moe_ffn* f, int32_t pass) {
   if (rc != kOk) return rc;
   Parts p{nullptr};
   const Ffn b(*f);
-  const bool whole = pass & MOE_FFN_ALIGNED;
-  if (pass & MOE_FFN_BACKWARD) Backward(b, p, whole, whole);
+  const bool whole = pass == MOE_FFN_ALIGNED || pass == (MOE_FFN_BACKWARD | MOE_FFN_ALIGNED);
+  if (pass != 0 && pass != MOE_FFN_ALIGNED) Backward(b, p, whole, whole);
   else Forward(b, p, whole);
   return p.at > Parts::kMost ? kErrBadShape : p.at;
 }

@@ -1842,7 +1842,7 @@ def _ffn_saved_bytes(f: MoeFfn) -> tuple[int, int]:
     return 8 * n, 2 * n
 
 
-_FFN_BACKWARD, _FFN_ALIGNED = 1, 2  # MOE_FFN_* of include/moe_mi355x.h
+_FFN_BACKWARD, _FFN_ALIGNED = 1, 256  # MOE_FFN_* of include/moe_mi355x.h
 
 
 def _ffn_workspace(f: MoeFfn, which: int) -> int:

@@ -70,10 +70,11 @@ def test_c_ffn_workspace_of_aligned_rows(L):
     rows = 1000 * 16 * 2 // 256 * 256 + (256 if 1000 * 16 * 2 % 256 else 0)
     one = dict(BASE, T=1000, top_k=1, max_padded=2000, topk_weights=None)
     f = _lib.MoeFfn(**one)
-    assert size(f, 2) == 0 and size(f, 0) == rows           # y
+    assert size(f, 256) == 0 and size(f, 0) == rows           # y
     dgu = 1000 * 2 * 16 * 2
-    assert size(f, 3) == dgu and size(f, 1) == dgu + 2 * rows  # dx and dy
+    assert size(f, 257) == dgu and size(f, 1) == dgu + 2 * rows  # dx and dy
     f = _lib.MoeFfn(**{**one, "top_k": 2, "max_padded": 4000})
-    assert size(f, 2) == size(f, 0) and size(f, 1) == size(f, 3) + rows  # dy; y and dx come from the slots' rows
+    assert size(f, 256) == size(f, 0) and size(f, 1) == size(f, 257) + rows  # dy; y and dx come from the slots' rows
+    assert size(f, 2) == size(f, 3) == size(f, -1) == size(f, 1)  # any other value is the backward pass's
     odd = _lib.MoeFfn(**{**one, "H": 15, "ldx": 16})
-    assert size(odd, 2) == size(odd, 0) > rows and size(odd, 3) == size(odd, 1) > 2 * rows
+    assert size(odd, 256) == size(odd, 0) > rows and size(odd, 257) == size(odd, 1) > 2 * rows

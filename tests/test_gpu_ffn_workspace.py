@@ -42,11 +42,11 @@ def test_c_calls_in_workspaces_of_their_size(k, H, shifts):
     y, dx, dyv = (place(s) for s in shifts)
     dyv[0].copy_(dy)
     dw13, dw2, dweight = torch.empty_like(w13), torch.empty_like(w2), torch.empty_like(weight)
-    ws, size = work(0 if shifts[0] else 2)
+    ws, size = work(0 if shifts[0] else 256)
     f.workspace = ws.data_ptr() if size else None
     _lib.check(_lib.lib().moe_ffn_forward(f, y[0].data_ptr(), ops._stream_handle()), "moe_ffn_forward")
     assert bool((ws[size:] == 0x5A).all())
-    ws, size = work(1 if shifts[1] or shifts[2] else 3)
+    ws, size = work(1 if shifts[1] or shifts[2] else 257)
     f.workspace = ws.data_ptr() if size else None
     _lib.check(_lib.lib().moe_ffn_backward(f, dyv[0].data_ptr(), dx[0].data_ptr(), dw13.data_ptr(), dw2.data_ptr(),
                                            dweight.data_ptr(), ops._stream_handle()), "moe_ffn_backward")
