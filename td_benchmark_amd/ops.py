@@ -1666,7 +1666,6 @@ def int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sc
         _need(bias, "bias", out_dtype, (N,), anywhere=True)
     if out is not None and tuple(out.shape) != (M, N):
         raise ValueError(f"out must be [{M}, {N}], got {tuple(out.shape)}")
-    _no_derivative("fp8_scaled_mm", a, b, a_scale, b_scale, bias, out)
     _need_here("a b a_scale b_scale bias out", a, b, a_scale, b_scale, bias, out)
     if out is None:
         out = a.new_empty((M, N), dtype=out_dtype)

@@ -56,3 +56,11 @@ def test_a_tangent_is_refused(calls, name):
         with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
             ops.fp8_scaled_mm(**args)
     assert not calls
+
+
+def test_the_int8_product_takes_what_it_took(calls):
+    """Its scales and bias may require gradients, as ever; the result has none."""
+    bias = torch.zeros(24, dtype=BF16, requires_grad=True)
+    scales = torch.ones(4, requires_grad=True), torch.ones(24)
+    y = ops.int8_scaled_mm(torch.zeros((4, 160), dtype=torch.int8), torch.zeros((24, 160), dtype=torch.int8), *scales, bias)
+    assert not y.requires_grad and calls == ["moe_int8_scaled_mm"]
